@@ -245,6 +245,84 @@ int ktmoe_layer_stage_times(ktmoe_layer* layer, double* ms, int32_t n_stages, in
  * 1: their scales [rows], 2: per-token combine outputs [rows][d_model] int32, 3: their scales [rows]). */
 int ktmoe_layer_debug_fetch(ktmoe_layer* layer, int32_t which, void* host, int64_t bytes);
 
+/* ── the paged KV cache and attention over it (the attention half's part between its linears) ──
+ * No counterpart of the cache's 8-bit form in the reference; the arithmetic is this library's own definition, in exact
+ * integers: RN24 and RN64 round to 24 and 53 significant bits and rne to a whole number, ties to even, and every other
+ * step is exact, so results do not depend on how the work is split.
+ *
+ * The cache: a row is one token's key or value of one KV head, int8 codes within +-127 at a scale sigma of 8
+ * significant bits (stored as bfloat16). Pools are device memory of the caller, the same layout for K and V: codes
+ * [n_pages][n_kv_heads][page_tokens][head_dim], scales [n_pages][n_kv_heads][page_tokens]. head_dim is a multiple of
+ * 16 from 16 to 256, page_tokens 16, 32, 64 or 128; the code pools are 16-byte aligned. */
+typedef struct ktmoe_kv_cache {
+    int8_t* k;
+    int8_t* v;
+    uint16_t* k_scale;
+    uint16_t* v_scale;
+    int64_t n_pages;
+    int32_t page_tokens;
+    int32_t n_kv_heads;
+    int32_t head_dim;
+} ktmoe_kv_cache;
+
+/* The new tokens of a batch of sequences, described in device memory: sequence b's rows are q_begin[b] to
+ * q_begin[b + 1] - 1 (ascending offsets) of the calls' buffers, which hold `rows` rows; its length with them is
+ * kv_len[b], so row t stands at position kv_len[b] - (q_begin[b + 1] - t); position p lies in pool page
+ * page_table[b * max_pages + p / page_tokens]. Rows before the first and behind the last sequence are left as they
+ * are. A row at a negative position (a length below the new tokens) has no place in the cache: append and read skip
+ * it, attention gives zeros. What only the device can see wrong (a page outside the pool, offsets that do not ascend
+ * or leave the rows, a length beyond the page table, a position beyond the rotation table) touches nothing outside
+ * the buffers and makes the next ktmoe_sync on the context return KTMOE_ERR_ARG; results of that batch are undefined. */
+typedef struct ktmoe_kv_batch {
+    int32_t n_seqs;
+    int32_t max_pages;
+    const int32_t* q_begin;    /* [n_seqs + 1] */
+    const int32_t* kv_len;     /* [n_seqs] */
+    const int32_t* page_table; /* [n_seqs][max_pages] */
+    int64_t rows;
+} ktmoe_kv_batch;
+
+/* Rotary positions: table [positions][rot_dim / 2][2] in device memory, cosine and sine times 2^30 (ktmoe_rope_table
+ * makes it on the host). The first rot_dim elements of a head are rotated in pairs (i, i + rot_dim / 2), or (2i, 2i + 1)
+ * when `interleaved`; a pair (a, b) becomes (a c - b s, b c + a s) and every other element x becomes 2^30 x, exactly. */
+typedef struct ktmoe_rope {
+    const int32_t* table;
+    int64_t positions;
+    int32_t rot_dim;
+    int32_t interleaved;
+} ktmoe_rope;
+/* round(cos(p theta^(-2i/rot_dim)) 2^30), round(sin(..) 2^30) in f64 on the host, for p < positions. */
+int ktmoe_rope_table(double theta, int32_t rot_dim, int64_t positions, int32_t* table);
+
+/* Write the batch's new keys and values: k, v [rows][n_kv_heads][head_dim] int32 codes with row strides ld_k and ld_v
+ * (in elements) at scale[row * scale_stride] (scale_stride 1: a scale per row; 0: one for all), keys rotated when rope
+ * is not NULL. With y a row's codes after the rotation and s its scale (2^-30 of it after a rotation):
+ * t = RN64(RN64(max|y| s) / 127) held within [2^-64, 2^63], sigma = t rounded up to 8 significant bits, codes
+ * rne(RN64(y RN64(s / sigma))) held within +-127. A scale's shift counts as at least -900 and at most 2000, here and in
+ * ktmoe_attention_dev. Stream-ordered (NULL: the context stream), not synchronised. Two
+ * rows of one call must not share a place in the cache. */
+int ktmoe_kv_append_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* k,
+                        int64_t ld_k, const int32_t* v, int64_t ld_v, const ktmoe_scale* scale, int32_t scale_stride,
+                        const ktmoe_rope* rope, void* stream);
+/* Read the same rows back: k, v [rows][n_kv_heads][head_dim] f32, code * sigma (exact). A whole sequence is read with
+ * q_begin spanning its kv_len tokens. */
+int ktmoe_kv_read_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, float* k, int64_t ld_k,
+                      float* v, int64_t ld_v, void* stream);
+/* Attention of the batch's new tokens over the cache (which holds them already: append first). q [rows][n_heads]
+ * [head_dim] int32 codes, query head h reading KV head h / (n_heads / n_kv_heads); o [rows][n_heads][head_dim] int32
+ * codes, o_scale [rows][n_kv_heads] the scale of each KV head's group of outputs. A row at position p sees the
+ * positions j <= p, and with window > 0 only those with j > p - window or j < sinks. Per row and head, with y and s as
+ * for the cache: codes rne(RN64(y RN64(127 / max|y|))), theta = RN24(min(2^60, RN64(RN64(RN64(max|y| s) / 127)
+ * RN64(softmax_scale log2 e)))); x_j = RN24((q . k_j) sigma_j), d_j = RN24(max x - x_j), z_j = min(32 * 2^10,
+ * rne(2^10 d_j theta)), n_j = rne(z_j / 2^10), r_j = n_j - z_j / 2^10, w_j = 2^-n_j e(r_j), where e, about 32512 * 2^r,
+ * is RN24(RN24(RN24(c3 r + c2) r + c1) r + 32512) with c1, c2, c3 = 127/256 times 45435, 15874, 3605; L = sum rne(w_j);
+ * 2^E the least power of two no smaller than any visible sigma of V; O = sum rne(w_j sigma_j 2^-E) v_j;
+ * o = rne(RN64(O RN64(2^21 / L))) (within +-2^28) at the scale {1, 21 - E}. A row that sees nothing is zeros at {0, 0}. */
+int ktmoe_attention_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* q,
+                        int64_t ld_q, const ktmoe_scale* scale, int32_t scale_stride, const ktmoe_rope* rope,
+                        int32_t n_heads, double softmax_scale, int32_t window, int32_t sinks, int32_t* o, int64_t ld_o,
+                        ktmoe_scale* o_scale, void* stream);
+
 /* ── host-side, offline preparation (f64, as the reference does it once on the host) ── */
 int ktmoe_quantize_weights(const float* w, int64_t n, int32_t* codes, ktmoe_scale* scale);
 /* Returns KTMOE_OK; *has_bias = 0 when the bias is all zero (the reference then keeps none). */

@@ -8,6 +8,8 @@ The host-side mirror of the reference's operator interfaces, over the C ABI of `
 * :class:`QuantLinear`, :class:`SwiGluMlp`,
   :class:`MoeMlp`, :class:`MoeRoute`               — crates/01-engine/kt-core/src/layers.rs:211-1106
 * :class:`B200Linear`                             — a ``LinearBackend`` (crates/01-engine/kt-core/src/backend.rs:46-59)
+* :class:`KvCache`, :class:`KvBatch`, :class:`Rope` — the paged 8-bit KV cache and the attention over it (this library's
+  own definition; ``kv_cache.py``)
 
 Every integer a forward produces comes from the sm_100a kernels in libktmoe.so; the only host arithmetic is the
 reference's own offline f64 preparation (weight and entry quantisers, code tables), done in C++ in the same library.
@@ -25,13 +27,14 @@ import numpy as np
 
 from . import _native
 from ._native import KtmoeError, KtmoeLayerConfig, KtmoeScale, check, lib
+from .kv_cache import KvBatch, KvCache, Rope, rope_table
 
 __all__ = [
     "WLEVELS", "ACT_LEVELS", "ROUTER_CODE_BITS", "Scale", "IntTensor", "QuantLinear", "SwiGluMlp", "MoeMlp", "MoeRoute", "RouterScore",
     "B200Linear", "Context", "DeviceLayer", "LayerSlot", "MoeStack", "device_count", "synth_normal", "synth_normal_portable", "lcg_uniform", "table",
     "route_margins", "hash_int", "repro_hash",
     "KtmoeError",
-    "ep_unique_id",
+    "ep_unique_id", "KvCache", "KvBatch", "Rope", "rope_table",
 ]
 
 WLEVELS = 265720  # (3^12 - 1) / 2, layers.rs:16

@@ -33,6 +33,39 @@ class KtmoeLayerConfig(ctypes.Structure):
     ]
 
 
+class KtmoeKvCache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("n_pages", ctypes.c_int64),
+        ("page_tokens", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+    ]
+
+
+class KtmoeKvBatch(ctypes.Structure):
+    _fields_ = [
+        ("n_seqs", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("q_begin", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+    ]
+
+
+class KtmoeRope(ctypes.Structure):
+    _fields_ = [
+        ("table", ctypes.c_void_p),
+        ("positions", ctypes.c_int64),
+        ("rot_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+    ]
+
+
 # Every symbol include/ktmoe.h declares, with its ctypes signature.
 _P = ctypes.POINTER
 _vp, _i32p, _i64p, _f32p = ctypes.c_void_p, _P(ctypes.c_int32), _P(ctypes.c_int64), _P(ctypes.c_float)
@@ -95,6 +128,12 @@ SIGNATURES = {
     "ktmoe_from_reals": ([_f32p, _i64, _i32p, _P(KtmoeScale)], ctypes.c_int),
     "ktmoe_table": ([_i32, _i64p, _P(KtmoeScale), _i64p, _P(KtmoeScale)], ctypes.c_int),
     "ktmoe_synth_normal": ([_u64, ctypes.c_float, _u64, _i64, _f32p], ctypes.c_int),
+    "ktmoe_rope_table": ([ctypes.c_double, _i32, _i64, _i32p], ctypes.c_int),
+    "ktmoe_kv_append_dev": ([_vp, _P(KtmoeKvCache), _P(KtmoeKvBatch), _vp, _i64, _vp, _i64, _vp, _i32, _P(KtmoeRope),
+                             _vp], ctypes.c_int),
+    "ktmoe_kv_read_dev": ([_vp, _P(KtmoeKvCache), _P(KtmoeKvBatch), _vp, _i64, _vp, _i64, _vp], ctypes.c_int),
+    "ktmoe_attention_dev": ([_vp, _P(KtmoeKvCache), _P(KtmoeKvBatch), _vp, _i64, _vp, _i32, _P(KtmoeRope), _i32,
+                             ctypes.c_double, _i32, _i32, _vp, _i64, _vp, _vp], ctypes.c_int),
     "ktmoe_lcg_uniform": ([_u64, _i64, _i64, _i64, _i32p], ctypes.c_int),
 }
 

@@ -18,9 +18,10 @@ BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libktmoe.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-SOURCES_CU = ["ktmoe.cu", "noalloc.cu"]
+SOURCES_CU = ["ktmoe.cu", "kv_cache.cu", "noalloc.cu"]
 SOURCES_CPP = ["host_prep.cpp", "wire.cpp"]
-HEADERS = ["fixed_point.cuh", "digit_gemm.cuh", "digit_gemm_pair.cuh", "moe_kernels.cuh", "ep_peer.cuh", "synth.cuh",
+KV_HEADERS = ["kv_kernels.cuh", "kv_attend_simple.cuh"]  # of kv_cache.cu alone
+HEADERS = ["context.cuh", "fixed_point.cuh", "digit_gemm.cuh", "digit_gemm_pair.cuh", "moe_kernels.cuh", "ep_peer.cuh", "synth.cuh",
            "host_prep.h"]
 
 
@@ -72,7 +73,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
         s = os.path.join(CSRC, src)
         o = os.path.join(BUILD, src + ".o")
         objs.append(o)
-        if force or _stale(o, [s] + header_deps):
+        deps = header_deps + ([os.path.join(CSRC, h) for h in KV_HEADERS] if src == "kv_cache.cu" else [])
+        if force or _stale(o, [s] + deps):
             cmd = [nvcc, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-ffp-contract=off",
                    "-I", os.path.join(ROOT, "include"), "-I", CSRC, *nccl_inc, "-c", s, "-o", o]
             if verbose:

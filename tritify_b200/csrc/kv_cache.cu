@@ -1,0 +1,166 @@
+// The paged KV cache's entry points of include/ktmoe.h: writing new keys and values, reading them back, and attention
+// over the cache. All on device buffers, ordered on the caller's stream, nothing allocated and no workspace kept, so
+// calls on several streams and captured graphs share nothing but the caller's own buffers.
+
+#include <cmath>
+#include <cstdint>
+
+#include "context.cuh"
+#include "kv_attend_simple.cuh"
+#include "kv_kernels.cuh"
+
+namespace {
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+kv::Error error_of(ktmoe_ctx* ctx) {
+    return kv::Error{ctx->d_err, ktc::ERR_BAD_PAGE, ktc::ERR_BAD_LENGTH, ktc::ERR_BAD_POSITION};
+}
+
+// The cache and the batch of a call; KTMOE_OK, or the status of what is wrong with them.
+int check_cache(ktmoe_ctx* ctx, const ktmoe_kv_cache* c, const ktmoe_kv_batch* b, kv::Cache* kc, kv::Batch* kb) {
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(ctx, KTMOE_ERR_ARG, "a pool of the cache is null");
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 2) || !aligned(c->v_scale, 2))
+        return fail(ctx, KTMOE_ERR_ARG, "the cache's pools need 16-byte (codes) and 2-byte (scales) alignment");
+    if (c->head_dim < 16 || c->head_dim > kv::MAX_DIM || c->head_dim % 16 != 0)
+        return fail(ctx, KTMOE_ERR_UNSUPPORTED, "head_dim must be a multiple of 16 from 16 to 256");
+    int shift = 4;
+    while (shift < 7 && (1 << shift) != c->page_tokens) ++shift;
+    if ((1 << shift) != c->page_tokens) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "page_tokens must be 16, 32, 64 or 128");
+    if (c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->n_pages < 1 || c->n_pages > INT32_MAX)
+        return fail(ctx, KTMOE_ERR_ARG, "the cache needs 1 to 1024 KV heads and 1 to 2^31 - 1 pages");
+    if (b->n_seqs < 0 || b->rows < 0 || b->rows > (int64_t)1 << 30 || b->max_pages < 0 ||
+        (int64_t)b->max_pages * c->page_tokens > (int64_t)1 << 30)
+        return fail(ctx, KTMOE_ERR_ARG, "a batch holds at most 2^30 rows and 2^30 tokens a sequence, none of them negative");
+    if (b->n_seqs > 0 && (!b->q_begin || !b->kv_len || (b->max_pages > 0 && !b->page_table)))
+        return fail(ctx, KTMOE_ERR_ARG, "the batch's offsets, lengths or page table are null");
+    *kc = kv::Cache{c->k, c->v, c->k_scale, c->v_scale, c->n_pages, shift, c->n_kv_heads, c->head_dim};
+    *kb = kv::Batch{b->q_begin, b->kv_len, b->page_table, b->n_seqs, b->max_pages, b->rows};
+    return KTMOE_OK;
+}
+
+int check_rope(ktmoe_ctx* ctx, const ktmoe_rope* r, int head_dim, kv::Rope* out) {
+    *out = kv::Rope{nullptr, 0, 0, 0};
+    if (!r) return KTMOE_OK;
+    if (!r->table || !aligned(r->table, 8) || r->positions < 1)
+        return fail(ctx, KTMOE_ERR_ARG, "the rotation table is null, not 8-byte aligned or empty");
+    if (r->rot_dim < 2 || r->rot_dim % 2 != 0 || r->rot_dim > head_dim)
+        return fail(ctx, KTMOE_ERR_ARG, "rot_dim must be even, from 2 to head_dim");
+    *out = kv::Rope{(const int2*)r->table, r->positions, r->rot_dim / 2, r->interleaved ? 1 : 0};
+    return KTMOE_OK;
+}
+
+int check_scale(ktmoe_ctx* ctx, const ktmoe_scale* s, int32_t stride) {
+    if (!aligned(s, 16) || (stride != 0 && stride != 1))
+        return fail(ctx, KTMOE_ERR_ARG, "scales need 16-byte alignment and a stride of 0 (one scale) or 1 (one a row)");
+    return KTMOE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ktmoe_rope_table(double theta, int32_t rot_dim, int64_t positions, int32_t* table) {
+    if (!table || rot_dim < 2 || rot_dim % 2 != 0 || positions < 1 || !(theta > 0.0) || !std::isfinite(theta))
+        return KTMOE_ERR_ARG;
+    const int half = rot_dim / 2;
+    for (int i = 0; i < half; ++i) {
+        const double f = std::pow(theta, -(double)i / half);
+        for (int64_t p = 0; p < positions; ++p) {
+            table[2 * (p * half + i)] = (int32_t)std::nearbyint(std::cos(p * f) * 1073741824.0);
+            table[2 * (p * half + i) + 1] = (int32_t)std::nearbyint(std::sin(p * f) * 1073741824.0);
+        }
+    }
+    return KTMOE_OK;
+}
+
+int ktmoe_kv_append_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* k,
+                        int64_t ld_k, const int32_t* v, int64_t ld_v, const ktmoe_scale* scale, int32_t scale_stride,
+                        const ktmoe_rope* rope, void* stream) {
+    if (!ctx || !cache || !batch) return KTMOE_ERR_ARG;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    kv::AppendArgs a{};
+    if (int r = check_cache(ctx, cache, batch, &a.c, &a.b)) return r;
+    if (int r = check_rope(ctx, rope, a.c.dim, &a.rope)) return r;
+    if (int r = check_scale(ctx, scale, scale_stride)) return r;
+    const int64_t width = (int64_t)a.c.heads * a.c.dim;
+    if (ld_k < width || ld_v < width) return fail(ctx, KTMOE_ERR_ARG, "a row stride is below n_kv_heads * head_dim");
+    if (batch->n_seqs == 0 || batch->rows == 0) return KTMOE_OK;
+    if (!k || !v || !scale || !aligned(k, 4) || !aligned(v, 4))
+        return fail(ctx, KTMOE_ERR_ARG, "keys, values or scales are null or not aligned");
+    if (int r = set_device(ctx)) return r;
+    a.err = error_of(ctx);
+    a.k = k;
+    a.v = v;
+    a.ld_k = ld_k;
+    a.ld_v = ld_v;
+    a.scale = (const longlong2*)scale;
+    a.scale_stride = scale_stride;
+    a.vec = aligned(k, 16) && aligned(v, 16) && ld_k % 4 == 0 && ld_v % 4 == 0;
+    cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
+    KLAUNCH(st, (unsigned)batch->rows, 32 * kv::APPEND_WARPS, 0, (kv::append_kernel), a);
+    return KTMOE_OK;
+}
+
+int ktmoe_kv_read_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, float* k, int64_t ld_k,
+                      float* v, int64_t ld_v, void* stream) {
+    if (!ctx || !cache || !batch) return KTMOE_ERR_ARG;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    kv::ReadArgs a{};
+    if (int r = check_cache(ctx, cache, batch, &a.c, &a.b)) return r;
+    const int64_t width = (int64_t)a.c.heads * a.c.dim;
+    if (ld_k < width || ld_v < width) return fail(ctx, KTMOE_ERR_ARG, "a row stride is below n_kv_heads * head_dim");
+    if (batch->n_seqs == 0 || batch->rows == 0) return KTMOE_OK;
+    if (!k || !v || !aligned(k, 4) || !aligned(v, 4)) return fail(ctx, KTMOE_ERR_ARG, "an output is null or not aligned");
+    if (int r = set_device(ctx)) return r;
+    a.err = error_of(ctx);
+    a.k = k;
+    a.v = v;
+    a.ld_k = ld_k;
+    a.ld_v = ld_v;
+    a.vec = aligned(k, 16) && aligned(v, 16) && ld_k % 4 == 0 && ld_v % 4 == 0;
+    cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
+    KLAUNCH(st, (unsigned)batch->rows, 32 * kv::APPEND_WARPS, 0, (kv::read_kernel), a);
+    return KTMOE_OK;
+}
+
+int ktmoe_attention_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* q,
+                        int64_t ld_q, const ktmoe_scale* scale, int32_t scale_stride, const ktmoe_rope* rope,
+                        int32_t n_heads, double softmax_scale, int32_t window, int32_t sinks, int32_t* o, int64_t ld_o,
+                        ktmoe_scale* o_scale, void* stream) {
+    if (!ctx || !cache || !batch) return KTMOE_ERR_ARG;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    kv::AttendArgs a{};
+    if (int r = check_cache(ctx, cache, batch, &a.c, &a.b)) return r;
+    if (int r = check_rope(ctx, rope, a.c.dim, &a.rope)) return r;
+    if (int r = check_scale(ctx, scale, scale_stride)) return r;
+    if (n_heads < 1 || n_heads % a.c.heads != 0)
+        return fail(ctx, KTMOE_ERR_ARG, "n_heads must be a positive multiple of n_kv_heads");
+    if (!(softmax_scale > 0.0) || !std::isfinite(softmax_scale) || window < 0 || sinks < 0)
+        return fail(ctx, KTMOE_ERR_ARG, "softmax_scale must be positive and finite, window and sinks not negative");
+    const int64_t width = (int64_t)n_heads * a.c.dim;
+    if (ld_q < width || ld_o < width) return fail(ctx, KTMOE_ERR_ARG, "a row stride is below n_heads * head_dim");
+    if (batch->n_seqs == 0 || batch->rows == 0) return KTMOE_OK;
+    if (!q || !o || !o_scale || !scale || !aligned(q, 4) || !aligned(o, 4) || !aligned(o_scale, 16))
+        return fail(ctx, KTMOE_ERR_ARG, "queries, scales or outputs are null or not aligned");
+    if (int r = set_device(ctx)) return r;
+    a.err = error_of(ctx);
+    a.q = q;
+    a.ld_q = ld_q;
+    a.scale = (const longlong2*)scale;
+    a.scale_stride = scale_stride;
+    a.vec = aligned(q, 16) && ld_q % 4 == 0;
+    a.group = n_heads / a.c.heads;
+    a.soft = softmax_scale * 1.4426950408889634;
+    a.window = window;
+    a.sinks = sinks;
+    a.o = o;
+    a.ld_o = ld_o;
+    a.o_scale = (longlong2*)o_scale;
+    cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
+    dim3 grid((unsigned)batch->rows, (unsigned)a.c.heads, (unsigned)((a.group + kv::SIMPLE_HEADS - 1) / kv::SIMPLE_HEADS));
+    KLAUNCH(st, grid, 128, 0, (kv::attend_simple_kernel), a);
+    return KTMOE_OK;
+}
+
+}  // extern "C"
