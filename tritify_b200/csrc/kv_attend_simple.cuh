@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(128) attend_simple_kernel(const AttendArgs a) 
     const int2* cs = rope_row(a.rope, a.err, p.pos);
     const double s = scale_value(a.scale[(long long)t * a.scale_stride], cs ? 30 : 0);
     for (int i = warp; i < ng; i += 4) {
-        const float th = quantise_query(q8[i], stage[warp],
+        const float th = quantise_query<false>(q8[i], stage[warp],
                                         a.q + (long long)t * a.ld_q + (long long)(h * a.group + g0 + i) * dim, dim,
                                         a.vec, a.rope, cs, s, a.soft);
         if (lane == 0) theta[i] = th;

@@ -1,0 +1,711 @@
+// Attention over the paged cache for many query rows: a block takes 128 rows (token, query head) of one sequence and KV
+// head and walks the keys they see in tiles of 128.
+//
+// The maximum of a row has to be known before its first weight is rounded, so the keys are walked twice: pass 0 forms
+// the scores for the row maxima (and the largest visible value scale), pass 1 forms them again and the weights. That
+// costs the score products twice and K's bytes from L2 twice; in return every weight is final when it is formed, and the
+// sums over the keys are plain integer sums that no later tile rescales.
+//
+// Per tile: S = Q K^T, 128 x 128 int32 in TMEM (tcgen05.mma kind::i8, K by TMA with the 128-byte swizzle); the weights
+// as two balanced 8-bit digits, w = 256 hi + lo, in shared memory; O_hi += P_hi V, O_lo += P_lo V in TMEM (V as it lies
+// in its pages, the MN-major operand). The int32 sums hold 132104 keys (127 * 128 each); every 131072 keys the carry of
+// lo goes into hi and that of hi into a 16-bit word of shared memory, which holds 2^25 keys.
+//
+// Roles (352 threads): warps 0-7 softmax (warp w: TMEM lanes 32 (w % 4) .., keys 64 (w / 4) .. of the tile), warp 8 TMA,
+// warp 9 MMA, warp 10 the keys' scales. Waits are bounded as in digit_gemm.cuh.
+#pragma once
+
+#include <cuda.h>
+
+#include "digit_gemm.cuh"
+#include "kv_kernels.cuh"
+
+namespace kv {
+
+using dg::mbar_arrive;
+using dg::mbar_arrive_expect_tx;
+using dg::mbar_init;
+using dg::smem_u32;
+using dg::umma_commit;
+
+constexpr int TILE_KEYS = 128;
+constexpr int TILE_ROWS = 128;
+
+// A bounded wait (2 s): false when it expires, or when another wait of the context has (the error word then holds a
+// code below 100; what a kernel finds wrong in a batch does not end waits).
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+    if (dg::mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = dg::globaltimer();
+    for (uint32_t it = 1;; ++it) {
+        if (dg::mbar_try_wait(bar, parity)) return true;
+        if ((it & 255u) == 0) {
+            const int e = *(volatile int*)err;
+            if (e > 0 && e < 100) return false;
+            if (dg::globaltimer() - t0 > 2000000000ull) {
+                atomicCAS(err, 0, code);
+                return false;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                            uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Shared-memory descriptor of an MN-major operand one 128-byte block wide, with the 128-byte swizzle: rows are steps of
+// K, 8-row groups 1024 bytes apart (the other stride, between blocks, is not used).
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(1024 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// kind::i8, s32 += s8 x s8, M = 128, N = n; `mn` bits 15 and 16: A, B MN-major.
+__device__ __forceinline__ uint32_t idesc_i8(int n, uint32_t mn) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | mn | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+// ── pairs of binary32 in one instruction ──
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 pk(float a, float b) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void upk(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+template <bool V>
+struct Bool {
+    static constexpr bool value = V;
+};
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const int32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
+}
+
+constexpr float MAGIC = 12582912.0f;  // 3 * 2^22: adding it rounds to a whole number, left in the low bits
+constexpr uint32_t MAGIC_BITS = 0x4B400000u;
+
+// A dot product s (|s| <= 2^22) of two adjacent keys times their scales, RN24: s + 3 * 2^22 as a float is an integer
+// addition, and (3 * 2^22 + s) sigma - 3 * 2^22 sigma is one fused operation, whose constant is exact.
+__device__ __forceinline__ f2 scaled2(int32_t s0, int32_t s1, f2 sigma, f2 csigma) {
+    return fma2(pk(__int_as_float(s0 + (int)MAGIC_BITS), __int_as_float(s1 + (int)MAGIC_BITS)), sigma, csigma);
+}
+
+// What a row's weights need: the maximum, -theta, the cubic's coefficients times 2^-E, and 2^E.
+struct RowWeights {
+    f2 top, ntheta, c0, c1, c2, c3, two_e;
+};
+
+__device__ __forceinline__ RowWeights row_weights(float top, float theta, int e) {
+    const float l = pow2f(-e);
+    RowWeights r;
+    r.top = pk(top, top);
+    r.ntheta = pk(-theta, -theta);
+    r.c0 = pk(W_C0 * l, W_C0 * l);
+    r.c1 = pk(W_C1 * l, W_C1 * l);
+    r.c2 = pk(W_C2 * l, W_C2 * l);
+    r.c3 = pk(W_C3 * l, W_C3 * l);
+    r.two_e = pk(pow2f(e), pow2f(e));
+    return r;
+}
+
+// weight() for a pair, times 2^-E. MASK: keys whose bit of `seen` is clear weigh nothing.
+template <bool MASK>
+__device__ __forceinline__ f2 weight2(f2 x, const RowWeights& w, uint32_t seen) {
+    const f2 minus = pk(-1.0f, -1.0f);
+    const f2 d = fma2(x, minus, w.top);
+    float a, b;
+    upk(fma2(d, w.ntheta, pk(12288.0f, 12288.0f)), a, b);
+    a = fmaxf(a, 12256.0f);
+    b = fmaxf(b, 12256.0f);
+    if (MASK) {
+        a = (seen & 1) ? a : 12256.0f;
+        b = (seen & 2) ? b : 12256.0f;
+    }
+    const f2 f = pk(a, b);
+    const f2 f0 = add2(f, pk(12570624.0f, 12570624.0f));
+    const f2 r = fma2(add2(f0, pk(-12570624.0f, -12570624.0f)), minus, f);
+    f2 e = fma2(w.c3, r, w.c2);
+    e = fma2(e, r, w.c1);
+    e = fma2(e, r, w.c0);
+    float e0, e1, n0, n1;
+    upk(e, e0, e1);
+    upk(f0, n0, n1);
+    return pk(__uint_as_float(__float_as_uint(e0) + (__float_as_uint(n0) << 23)),
+              __uint_as_float(__float_as_uint(e1) + (__float_as_uint(n1) << 23)));
+}
+
+// The keys that a tile's rows at positions p0 .. p1 see, as a list of 128-key tiles: first those of the sinks, then
+// those from the first row's window on.
+struct KeyTiles {
+    int n, n_sink, first;
+    __device__ __forceinline__ KeyTiles(int p0, int p1, int window, int sinks) {
+        const int lo = window ? max(0, p0 + 1 - window) : 0;
+        first = lo / TILE_KEYS;
+        n_sink = min((min(sinks, lo) + TILE_KEYS - 1) / TILE_KEYS, first);
+        n = p1 < 0 ? 0 : n_sink + p1 / TILE_KEYS - first + 1;
+    }
+    __device__ __forceinline__ int at(int i) const { return i < n_sink ? i : i - n_sink + first; }
+};
+
+// Bit k set: key j0 + k (k < 64) is visible to a row at position pos.
+__device__ __forceinline__ uint64_t seen_bits(int j0, int pos, int window, int sinks) {
+    auto below = [&](int end) -> uint64_t {  // keys j < end
+        const int k = end - j0;
+        return k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1;
+    };
+    if (pos < 0) return 0;
+    uint64_t m = below(pos + 1);
+    if (window && pos >= window) m &= ~below(pos + 1 - window) | below(sinks);
+    return m;
+}
+
+// The last i in [0, n) with f(i) <= target (f ascends), by a whole warp; 0 when there is none.
+template <class F>
+__device__ __forceinline__ int warp_search(int n, long long target, F f) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int i = min(lo + lane * step, hi - 1);
+        const bool in = lo + lane * step < hi;
+        const unsigned le = __ballot_sync(0xffffffffu, in && f(i) <= target);
+        const int k = max(1, 32 - __clz(le));
+        lo = lo + (k - 1) * step;
+        hi = min(lo + step, hi);
+    }
+    return lo;
+}
+
+// NK: 128-byte blocks of a key row (head_dim up to 128, or up to 256).
+template <int NK>
+struct TileCfg {
+    static constexpr int SLOT = TILE_KEYS * 128;  // bytes of one block of a key or value tile
+    static constexpr int SLOTS = NK == 1 ? 6 : 5;
+    static constexpr int SCALES = 4;  // tiles of key scales in flight
+    static constexpr int Q = 0;
+    static constexpr int P = Q + NK * SLOT;           // [2][hi, lo]
+    static constexpr int RING = P + 4 * SLOT;
+    static constexpr int CARRY = RING + SLOTS * SLOT;  // int16 [128 columns][128 rows]
+    static constexpr int KEY_SCALES = CARRY + TILE_ROWS * 128 * 2;  // [SCALES][sigma_k, -MAGIC sigma_k, sigma_v][128]
+    static constexpr int ROWS = KEY_SCALES + SCALES * 3 * TILE_KEYS * 4;  // theta, max [2], largest sigma [2], L [2]
+    static constexpr int BARS = ROWS + TILE_ROWS * (4 + 8 + 8 + 16);
+    static constexpr int BYTES = 1024 + BARS + 512;
+    static_assert(BYTES <= 232448, "shared memory per block");
+};
+
+constexpr int TILE_THREADS = 352;
+constexpr int FLUSH_TILES = 1024;  // 131072 keys: |sum| <= 131072 * 127 * 128 < 2^31
+
+template <int NK>
+__global__ void __launch_bounds__(TILE_THREADS, 1)
+    attend_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const AttendArgs a, long long slots) {
+    kt::pdl_enter();
+    using C = TileCfg<NK>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float* s_theta = (float*)(sm + C::ROWS);
+    float* s_top = s_theta + TILE_ROWS;
+    uint32_t* s_sig = (uint32_t*)(s_top + 2 * TILE_ROWS);
+    unsigned long long* s_total = (unsigned long long*)(s_sig + 2 * TILE_ROWS);
+    uint64_t* full = (uint64_t*)(sm + C::BARS);  // [SLOTS] a block of K or V has landed
+    uint64_t* empty = full + C::SLOTS;           // [SLOTS] its products are done
+    uint64_t* s_full = empty + C::SLOTS;         // [2] scores in TMEM
+    uint64_t* s_free = s_full + 2;               // [2] scores read
+    uint64_t* p_full = s_free + 2;               // [2] digits of the weights in shared memory
+    uint64_t* p_free = p_full + 2;               // [2] their products are done
+    uint64_t* k_full = p_free + 2;               // [SCALES]
+    uint64_t* k_free = k_full + C::SCALES;       // [SCALES]
+    uint64_t* q_full = k_free + C::SCALES;
+    uint64_t* o_full = q_full + 1;
+    uint64_t* o_free = o_full + 1;
+    uint64_t* done = o_free + 1;
+    uint32_t* tmem_slot = (uint32_t*)(done + 1);
+    int* s_job = (int*)(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = a.group, dim = a.c.dim;
+    const int head = (int)(blockIdx.x % (unsigned)a.c.heads);
+    // later tiles of a sequence see more keys: they start first
+    const long long slot = slots - 1 - (long long)(blockIdx.x / (unsigned)a.c.heads);
+    // Sequence b's tiles stand at slots begin_b g / 128 + b and on: there is room for them before the next sequence's,
+    // and the few slots that stay empty leave at once.
+    if (warp == 0) {
+        auto first_slot = [&](int b) { return (long long)a.b.begin[b] * g / TILE_ROWS + b; };
+        const int b = warp_search(a.b.n_seqs, slot, first_slot);
+        const int begin = a.b.begin[b], end = a.b.begin[b + 1], len = a.b.kv_len[b];
+        const long long row0 = (slot - first_slot(b)) * TILE_ROWS;
+        bool live = row0 >= 0 && row0 < (long long)(end - begin) * g;
+        if (begin < 0 || begin > end || end > a.b.begin[a.b.n_seqs] || end > a.b.rows || len < 0 ||
+            ((len + (1 << a.c.page_shift) - 1) >> a.c.page_shift) > a.b.max_pages) {
+            if (lane == 0) a.err.raise(a.err.bad_length);
+            live = false;
+        }
+        if (lane == 0) {
+            s_job[0] = live ? b : -1;
+            s_job[1] = begin;
+            s_job[2] = end - begin;
+            s_job[3] = len;
+            s_job[4] = (int)row0;
+        }
+    }
+    if (threadIdx.x == 32) {
+        for (int i = 0; i < C::SLOTS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&s_free[i], 8);
+            mbar_init(&p_full[i], 8);
+            mbar_init(&p_free[i], 1);
+        }
+        for (int i = 0; i < C::SCALES; ++i) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_free[i], 8);
+        }
+        mbar_init(q_full, 8);
+        mbar_init(o_full, 1);
+        mbar_init(o_free, 8);
+        mbar_init(done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    const int seq = s_job[0];
+    if (seq < 0) return;
+    const int begin = s_job[1], n_new = s_job[2], len = s_job[3], row0 = s_job[4];
+    const int n_rows = min(TILE_ROWS, n_new * g - row0);
+    const int t0 = row0 / g;
+    const int p0 = len - n_new + t0, p1 = len - n_new + (row0 + n_rows - 1) / g;
+    const KeyTiles kt_(p0, p1, a.window, a.sinks);
+    const int n = kt_.n;
+    const int n_pass = n > 0 ? 1 + NK : 0;  // the maxima, then the values of each 128-column block
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.fence::before_thread_sync;");
+    }
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    const uint32_t tmem = *tmem_slot;
+    const int ps = 1 << a.c.page_shift;
+
+    if (warp == 8) {
+        // K of pass 0; then, per value block, K of tile i + 1 ahead of V of tile i, as the products take them
+        const int per_tile = TILE_KEYS >> a.c.page_shift;
+        uint32_t q = 0;
+        bool alive = true;
+        auto load = [&](const CUtensorMap* map, int tile, int x) {
+            const int s = q % C::SLOTS;
+            // pages that hold keys up to the last row's position; the others' keys are not visible
+            const int i0 = tile * per_tile, np = min(per_tile, (p1 >> a.c.page_shift) - i0 + 1);
+            int page = 0;
+            if (lane < np) page = (int)pool_page(a.b, a.c, a.err, seq, i0 + lane);
+            bool ok = true;
+            if (lane == 0) {
+                ok = wait(&empty[s], ((q / C::SLOTS) & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_EMPTY);
+                if (ok) mbar_arrive_expect_tx(&full[s], (uint32_t)(np * ps * 128));
+            }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+            if (!ok) {
+                alive = false;
+                return;
+            }
+            if (lane < np)
+                tma_load_4d(smem_u32(sm + C::RING + s * C::SLOT + lane * ps * 128), map, x, 0, head, page, &full[s]);
+            ++q;
+        };
+        for (int pass = 0; alive && pass < n_pass; ++pass) {
+            for (int i = 0; alive && i < n; ++i) {
+                if (pass == 0 || i == 0)
+                    for (int x = 0; alive && x < NK; ++x) load(&map_k, kt_.at(i), x * 128);
+                if (pass > 0) {
+                    if (i + 1 < n)
+                        for (int x = 0; alive && x < NK; ++x) load(&map_k, kt_.at(i + 1), x * 128);
+                    if (alive) load(&map_v, kt_.at(i), (pass - 1) * 128);
+                }
+            }
+        }
+        if (lane == 0)  // copies still in flight land before the block leaves
+            for (uint32_t j = q > (uint32_t)C::SLOTS ? q - C::SLOTS : 0; j < q; ++j)
+                dg::mbar_wait_drain(&full[j % C::SLOTS], (j / C::SLOTS) & 1u, a.err.word, dg::ERR_TIMEOUT_FULL);
+    } else if (warp == 9) {
+        if (lane == 0) {
+            const int ksteps = (dim + 31) / 32;
+            uint32_t q = 0, sc = 0, pc = 0, oc = 0;
+            const uint32_t id_s = idesc_i8(TILE_KEYS, 0);
+            auto scores = [&]() -> bool {
+                const uint32_t b = sc & 1;
+                if (!wait(&s_free[b], ((sc >> 1) & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM)) return false;
+#pragma unroll
+                for (int x = 0; x < NK; ++x) {
+                    const int s = q % C::SLOTS;
+                    if (!wait(&full[s], (q / C::SLOTS) & 1u, a.err.word, dg::ERR_TIMEOUT_FULL)) return false;
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                    const uint32_t qa = smem_u32(sm + C::Q + x * C::SLOT), kb = smem_u32(sm + C::RING + s * C::SLOT);
+                    for (int kk = 0; kk < min(4, ksteps - 4 * x); ++kk)
+                        dg::umma_i8(tmem + b * 128, dg::smem_desc_sw128(qa + kk * 32), dg::smem_desc_sw128(kb + kk * 32), id_s,
+                                    x + kk > 0);
+                    umma_commit(&empty[s]);
+                    ++q;
+                }
+                umma_commit(&s_full[b]);
+                ++sc;
+                return true;
+            };
+            auto values = [&](int i, int cols) -> bool {
+                const uint32_t b = pc & 1;
+                const int s = q % C::SLOTS;
+                if (!wait(&p_full[b], (pc >> 1) & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM)) return false;
+                if (!wait(&full[s], (q / C::SLOTS) & 1u, a.err.word, dg::ERR_TIMEOUT_FULL)) return false;
+                asm volatile("tcgen05.fence::after_thread_sync;");
+                const uint32_t id_o = idesc_i8(cols, 1u << 16);
+                const uint32_t pa = smem_u32(sm + C::P + b * 2 * C::SLOT), vb = smem_u32(sm + C::RING + s * C::SLOT);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    const uint64_t dv = desc_mn_sw128(vb + kk * 32 * 128);
+                    dg::umma_i8(tmem + 256, dg::smem_desc_sw128(pa + kk * 32), dv, id_o, i + kk > 0);
+                    dg::umma_i8(tmem + 384, dg::smem_desc_sw128(pa + C::SLOT + kk * 32), dv, id_o, i + kk > 0);
+                }
+                umma_commit(&empty[s]);
+                umma_commit(&p_free[b]);
+                ++q;
+                ++pc;
+                return true;
+            };
+            bool ok = n_pass == 0 || wait(q_full, 0, a.err.word, dg::ERR_TIMEOUT_FULL);
+            for (int pass = 0; ok && pass < n_pass; ++pass) {
+                const int cols = min(128, dim - (pass - 1) * 128);
+                for (int i = 0; ok && i < n; ++i) {
+                    if (pass == 0 || i == 0) ok = ok && scores();
+                    if (pass > 0) {
+                        if (i + 1 < n) ok = ok && scores();
+                        ok = ok && values(i, cols);
+                        // the sums are read at the end of the block, and carried on every FLUSH_TILES tiles
+                        if (ok && (i + 1 == n || (i + 1) % FLUSH_TILES == 0)) {
+                            umma_commit(o_full);
+                            if (i + 1 < n || pass + 1 < n_pass) {
+                                ok = wait(o_free, oc & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+                                asm volatile("tcgen05.fence::after_thread_sync;");
+                            }
+                            ++oc;
+                        }
+                    }
+                }
+            }
+            umma_commit(done);
+            dg::mbar_wait_drain(done, 0u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+        }
+    } else if (warp == 10) {
+        // the scales of each tile's keys, four keys a lane
+        uint32_t kc = 0;
+        bool alive = true;
+        for (int pass = 0; alive && pass < n_pass; ++pass) {
+            for (int i = 0; alive && i < n; ++i, ++kc) {
+                const int st = kc % C::SCALES;
+                const int j = kt_.at(i) * TILE_KEYS + 4 * lane;
+                ushort4 k4 = {0, 0, 0, 0}, v4 = {0, 0, 0, 0};
+                if (j <= p1) {
+                    const long long page = pool_page(a.b, a.c, a.err, seq, j >> a.c.page_shift);
+                    const long long row = ((page * a.c.heads + head) << a.c.page_shift) + (j & (ps - 1));
+                    k4 = *(const ushort4*)(a.c.ks + row);
+                    v4 = *(const ushort4*)(a.c.vs + row);
+                }
+                alive = wait(&k_free[st], ((kc / C::SCALES) & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_EMPTY);
+                alive = __all_sync(0xffffffffu, alive);
+                if (!alive) break;
+                float* f = (float*)(sm + C::KEY_SCALES) + st * 3 * TILE_KEYS;
+                const float4 kf = {bf16_value(k4.x), bf16_value(k4.y), bf16_value(k4.z), bf16_value(k4.w)};
+                *(float4*)(f + 4 * lane) = kf;
+                *(float4*)(f + TILE_KEYS + 4 * lane) = {-MAGIC * kf.x, -MAGIC * kf.y, -MAGIC * kf.z, -MAGIC * kf.w};
+                *(float4*)(f + 2 * TILE_KEYS + 4 * lane) = {bf16_value(v4.x), bf16_value(v4.y), bf16_value(v4.z),
+                                                            bf16_value(v4.w)};
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&k_full[st]);
+            }
+        }
+    } else {
+        // the queries: codes into the K-major operand, theta
+        {
+            // staging over the weights' digits, which come later
+            int32_t* stage = (int32_t*)(sm + C::P) + warp * MAX_DIM;
+            for (int r = warp; r < n_rows && n_pass; r += 8) {
+                const int t = (row0 + r) / g, hq = head * g + (row0 + r) % g;
+                const int pos = len - n_new + t;
+                if (pos < 0) continue;
+                const long long row = (long long)begin + t;
+                const int2* cs = rope_row(a.rope, a.err, pos);
+                const double s = scale_value(a.scale[row * a.scale_stride], cs ? 30 : 0);
+                const float th = quantise_query<true>((int8_t*)sm + C::Q + r * 128, stage,
+                                                      a.q + row * a.ld_q + (long long)hq * dim, dim, a.vec, a.rope, cs,
+                                                      s, a.soft, r);
+                if (lane == 0) s_theta[r] = th;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        const int quad = warp & 3, half = warp >> 2;
+        const int r = quad * 32 + lane;  // row of the tile
+        const bool row_live = r < n_rows;
+        const int t = (row0 + min(r, n_rows - 1)) / g;
+        const int pos = row_live ? len - n_new + t : -1;
+        const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
+        uint32_t sc = 0, pc = 0, oc = 0;
+        bool ok = true;
+        float top = -INFINITY;
+        uint32_t sig = 0;
+        // whether every live row sees all of tile j0 .. j0 + 127 (the same for all warps)
+        auto whole = [&](int j0) {
+            if (j0 + TILE_KEYS - 1 > p0) return false;
+            return !a.window || j0 > p1 - a.window || j0 + TILE_KEYS <= a.sinks;
+        };
+        int32_t s32[2][32];
+        // this thread's 64 scores of the next tile; its key scales are ready then
+        auto next_scores = [&]() {
+            const uint32_t b = sc & 1;
+            ok = wait(&s_full[b], (sc >> 1) & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            dg::tmem_ld32(lane_addr + b * 128 + half * 64, s32[0]);
+            dg::tmem_ld32(lane_addr + b * 128 + half * 64 + 32, s32[1]);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[b]);
+            ok = wait(&k_full[sc % C::SCALES], (sc / C::SCALES) & 1u, a.err.word, dg::ERR_TIMEOUT_FULL);
+            ok = __all_sync(0xffffffffu, ok);
+        };
+        auto scales_read = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&k_free[sc % C::SCALES]);
+            ++sc;
+        };
+        // ── pass 0: the maxima ──
+        for (int i = 0; ok && n_pass && i < n; ++i) {
+            next_scores();
+            if (!ok) break;
+            const int j0 = kt_.at(i) * TILE_KEYS;
+            const float* f = (const float*)(sm + C::KEY_SCALES) + (sc % C::SCALES) * 3 * TILE_KEYS + half * 64;
+            if (whole(j0)) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        const ulonglong2 kf = *(const ulonglong2*)(f + c * 32 + k);
+                        const ulonglong2 kc = *(const ulonglong2*)(f + TILE_KEYS + c * 32 + k);
+                        const uint4 vf = *(const uint4*)(f + 2 * TILE_KEYS + c * 32 + k);
+                        float x0, x1, x2, x3;
+                        upk(scaled2(s32[c][k], s32[c][k + 1], kf.x, kc.x), x0, x1);
+                        upk(scaled2(s32[c][k + 2], s32[c][k + 3], kf.y, kc.y), x2, x3);
+                        top = fmaxf(fmaxf(top, x0), x1);
+                        top = fmaxf(fmaxf(top, x2), x3);
+                        sig = max(max(sig, vf.x), vf.y);
+                        sig = max(max(sig, vf.z), vf.w);
+                    }
+            } else {
+                const uint64_t seen = seen_bits(j0 + half * 64, pos, a.window, a.sinks);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t m = (uint32_t)(seen >> (32 * c));
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        const f2 kf = *(const f2*)(f + c * 32 + k), kc = *(const f2*)(f + TILE_KEYS + c * 32 + k);
+                        const uint2 vf = *(const uint2*)(f + 2 * TILE_KEYS + c * 32 + k);
+                        float x0, x1;
+                        upk(scaled2(s32[c][k], s32[c][k + 1], kf, kc), x0, x1);
+                        if (m >> k & 1) {
+                            top = fmaxf(top, x0);
+                            sig = max(sig, vf.x);
+                        }
+                        if (m >> k & 2) {
+                            top = fmaxf(top, x1);
+                            sig = max(sig, vf.y);
+                        }
+                    }
+                }
+            }
+            scales_read();
+        }
+        // the two halves of a row meet
+        s_top[half * TILE_ROWS + r] = top;
+        s_sig[half * TILE_ROWS + r] = sig;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        top = fmaxf(s_top[r], s_top[TILE_ROWS + r]);
+        sig = max(s_sig[r], s_sig[TILE_ROWS + r]);
+        const int e_row = sig ? scale_exp(sig >> 16) : 0;
+        const RowWeights rw = row_weights(top, row_live && pos >= 0 ? s_theta[r] : 0.0f, e_row);
+        uint64_t total = 0;
+        bool met = n_pass == 0;
+        int16_t* carry = (int16_t*)(sm + C::CARRY);
+        // ── the weights and the sums ──
+        for (int pass = 1; ok && pass < n_pass; ++pass) {
+            const int cols = min(128, dim - (pass - 1) * 128);
+            bool carried = false;
+            for (int i = 0; ok && i < n; ++i) {
+                next_scores();
+                if (!ok) break;
+                const int j0 = kt_.at(i) * TILE_KEYS;
+                const float* f = (const float*)(sm + C::KEY_SCALES) + (sc % C::SCALES) * 3 * TILE_KEYS + half * 64;
+                const uint32_t b = pc & 1;
+                ok = wait(&p_free[b], ((pc >> 1) & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_EMPTY);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                uint8_t* hi = sm + C::P + b * 2 * C::SLOT + r * 128;
+                uint8_t* lo = hi + C::SLOT;
+                uint32_t sum = 0;
+                auto digits = [&](auto mask_tag, uint64_t seen) {
+                    constexpr bool MASK = decltype(mask_tag)::value;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int k16 = 0; k16 < 32; k16 += 16) {
+                            uint32_t h4[4], l4[4];
+#pragma unroll
+                            for (int k4 = 0; k4 < 4; ++k4) {
+                                const int k = k16 + 4 * k4;
+                                const ulonglong2 kf = *(const ulonglong2*)(f + c * 32 + k);
+                                const ulonglong2 kc = *(const ulonglong2*)(f + TILE_KEYS + c * 32 + k);
+                                const ulonglong2 vf = *(const ulonglong2*)(f + 2 * TILE_KEYS + c * 32 + k);
+                                const uint32_t m = MASK ? (uint32_t)(seen >> (32 * c + k)) : 0u;
+                                const f2 w0 = weight2<MASK>(scaled2(s32[c][k], s32[c][k + 1], kf.x, kc.x), rw, m);
+                                const f2 w1 = weight2<MASK>(scaled2(s32[c][k + 2], s32[c][k + 3], kf.y, kc.y), rw, m >> 2);
+                                const f2 mg = pk(MAGIC, MAGIC), mg128 = pk(MAGIC + 128.0f, MAGIC + 128.0f);
+                                float a0, a1, a2, a3;
+                                upk(fma2(w0, rw.two_e, mg), a0, a1);
+                                upk(fma2(w1, rw.two_e, mg), a2, a3);
+                                sum += __float_as_uint(a0) + __float_as_uint(a1);
+                                sum += __float_as_uint(a2) + __float_as_uint(a3);
+                                upk(fma2(w0, vf.x, mg128), a0, a1);
+                                upk(fma2(w1, vf.y, mg128), a2, a3);
+                                // w + 128 in the low 16 bits: the upper byte is hi, the lower one lo + 128
+                                const uint32_t u = __byte_perm(__float_as_uint(a0), __float_as_uint(a1), 0x5140);
+                                const uint32_t v = __byte_perm(__float_as_uint(a2), __float_as_uint(a3), 0x5140);
+                                l4[k4] = __byte_perm(u, v, 0x5410) ^ 0x80808080u;
+                                h4[k4] = __byte_perm(u, v, 0x7632);
+                            }
+                            const int chunk = ((half * 4 + c * 2 + (k16 >> 4)) ^ (r & 7)) * 16;
+                            *(uint4*)(hi + chunk) = make_uint4(h4[0], h4[1], h4[2], h4[3]);
+                            *(uint4*)(lo + chunk) = make_uint4(l4[0], l4[1], l4[2], l4[3]);
+                        }
+                };
+                if (whole(j0))
+                    digits(Bool<false>{}, 0);
+                else
+                    digits(Bool<true>{}, seen_bits(j0 + half * 64, pos, a.window, a.sinks));
+                if (pass == 1) total += sum - 64u * MAGIC_BITS;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[b]);
+                ++pc;
+                scales_read();
+                if ((i + 1) % FLUSH_TILES == 0 && i + 1 < n) {
+                    ok = wait(o_full, oc & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                    for (int c = half * 64; c < min(cols, half * 64 + 64); c += 16) {
+                        int32_t h[16], l[16];
+                        dg::tmem_ld16(lane_addr + 256 + c, h);
+                        dg::tmem_ld16(lane_addr + 384 + c, l);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            // lo = 256 q + rest: q into hi; hi = 2^24 q + rest: q into the carry
+                            h[k] += l[k] >> 8;
+                            l[k] &= 255;
+                            int16_t* cw = carry + (c + k) * TILE_ROWS + r;
+                            *cw = (int16_t)((carried ? *cw : 0) + (h[k] >> 24));
+                            h[k] &= 0xffffff;
+                        }
+                        tmem_st16(lane_addr + 256 + c, h);
+                        tmem_st16(lane_addr + 384 + c, l);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(o_free);
+                    carried = true;
+                    ++oc;
+                }
+            }
+            if (pass == 1) {  // the row's total over both halves
+                s_total[half * TILE_ROWS + r] = total;
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                met = true;
+                total = s_total[r] + s_total[TILE_ROWS + r];
+            }
+            if (!ok) break;
+            ok = wait(o_full, oc & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            ++oc;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            const double inv = total ? __ddiv_rn(2097152.0, (double)total) : 0.0;
+            int32_t* out = a.o + ((long long)begin + t) * a.ld_o +
+                           (long long)(head * g + (row0 + min(r, n_rows - 1)) % g) * dim + (pass - 1) * 128;
+            for (int c = half * 64; c < min(cols, half * 64 + 64); c += 16) {
+                int32_t h[16], l[16];
+                dg::tmem_ld16(lane_addr + 256 + c, h);
+                dg::tmem_ld16(lane_addr + 384 + c, l);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (row_live) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        int64_t num = (int64_t)h[k] * 256 + l[k];
+                        if (carried) num += (int64_t)carry[(c + k) * TILE_ROWS + r] << 32;
+                        h[k] = total ? out_code(num, inv) : 0;
+                    }
+                    if (a.vec_o) {
+#pragma unroll
+                        for (int k = 0; k < 16; k += 4) *(int4*)(out + c + k) = make_int4(h[k], h[k + 1], h[k + 2], h[k + 3]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) out[c + k] = h[k];
+                    }
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free);
+        }
+        if (!met) asm volatile("bar.sync 1, 256;" ::: "memory");  // a wait failed: the other warps still meet here
+        if (n_pass == 0 && row_live && half == 0) {  // no row of the tile sees anything
+            int32_t* out = a.o + ((long long)begin + t) * a.ld_o + (long long)(head * g + (row0 + r) % g) * dim;
+            for (int k = 0; k < dim; ++k) out[k] = 0;
+        }
+        if (row_live && half == 0 && (row0 + r) % g == 0)
+            a.o_scale[((long long)begin + t) * a.c.heads + head] =
+                total ? make_longlong2(1, (long long)(uint32_t)(21 - e_row)) : make_longlong2(0, 0);
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;");
+    __syncthreads();
+    if (warp == 0) {
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+}  // namespace kv

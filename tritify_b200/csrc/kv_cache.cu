@@ -7,6 +7,7 @@
 
 #include "context.cuh"
 #include "kv_attend_simple.cuh"
+#include "kv_attend_tile.cuh"
 #include "kv_kernels.cuh"
 
 namespace {
@@ -20,8 +21,8 @@ kv::Error error_of(ktmoe_ctx* ctx) {
 // The cache and the batch of a call; KTMOE_OK, or the status of what is wrong with them.
 int check_cache(ktmoe_ctx* ctx, const ktmoe_kv_cache* c, const ktmoe_kv_batch* b, kv::Cache* kc, kv::Batch* kb) {
     if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(ctx, KTMOE_ERR_ARG, "a pool of the cache is null");
-    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 2) || !aligned(c->v_scale, 2))
-        return fail(ctx, KTMOE_ERR_ARG, "the cache's pools need 16-byte (codes) and 2-byte (scales) alignment");
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 16) || !aligned(c->v_scale, 16))
+        return fail(ctx, KTMOE_ERR_ARG, "the cache's pools need 16-byte alignment");
     if (c->head_dim < 16 || c->head_dim > kv::MAX_DIM || c->head_dim % 16 != 0)
         return fail(ctx, KTMOE_ERR_UNSUPPORTED, "head_dim must be a multiple of 16 from 16 to 256");
     int shift = 4;
@@ -53,6 +54,40 @@ int check_rope(ktmoe_ctx* ctx, const ktmoe_rope* r, int head_dim, kv::Rope* out)
 int check_scale(ktmoe_ctx* ctx, const ktmoe_scale* s, int32_t stride) {
     if (!aligned(s, 16) || (stride != 0 && stride != 1))
         return fail(ctx, KTMOE_ERR_ARG, "scales need 16-byte alignment and a stride of 0 (one scale) or 1 (one a row)");
+    return KTMOE_OK;
+}
+
+// The TMA map of a pool: boxes of one page of one KV head, 128 bytes of its rows. Bytes behind head_dim read as zero.
+int make_pool_map(ktmoe_ctx* ctx, CUtensorMap* map, const int8_t* pool, const kv::Cache& c) {
+    ktc::EncodeTiledFn enc = ktc::encode_fn();
+    if (!enc) return fail(ctx, KTMOE_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t ps = (cuuint64_t)1 << c.page_shift;
+    cuuint64_t gdim[4] = {(cuuint64_t)c.dim, ps, (cuuint64_t)c.heads, (cuuint64_t)c.n_pages};
+    cuuint64_t gstride[3] = {(cuuint64_t)c.dim, ps * c.dim, ps * c.dim * c.heads};
+    cuuint32_t box[4] = {128, (cuuint32_t)ps, 1, 1};
+    cuuint32_t estride[4] = {1, 1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(pool), gdim, gstride, box, estride,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ctx, KTMOE_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+    return KTMOE_OK;
+}
+
+template <int NK>
+int launch_tile(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
+    static bool attr_set[64] = {};
+    if (!attr_set[ctx->device & 63]) {
+        CK(cudaFuncSetAttribute(kv::attend_tile_kernel<NK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kv::TileCfg<NK>::BYTES));
+        attr_set[ctx->device & 63] = true;
+    }
+    CUtensorMap mk, mv;
+    if (int r = make_pool_map(ctx, &mk, a.c.k, a.c)) return r;
+    if (int r = make_pool_map(ctx, &mv, a.c.v, a.c)) return r;
+    const int64_t slots = a.b.rows * a.group / kv::TILE_ROWS + a.b.n_seqs;
+    if (slots * a.c.heads > INT32_MAX) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "too many query rows for one launch");
+    KLAUNCH(st, (unsigned)(slots * a.c.heads), kv::TILE_THREADS, kv::TileCfg<NK>::BYTES, (kv::attend_tile_kernel<NK>), mk,
+            mv, a, (long long)slots);
     return KTMOE_OK;
 }
 
@@ -157,7 +192,9 @@ int ktmoe_attention_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe
     a.o = o;
     a.ld_o = ld_o;
     a.o_scale = (longlong2*)o_scale;
+    a.vec_o = aligned(o, 16) && ld_o % 4 == 0;
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
+    if (a.group * batch->rows > 16 * batch->n_seqs) return a.c.dim <= 128 ? launch_tile<1>(ctx, st, a) : launch_tile<2>(ctx, st, a);
     dim3 grid((unsigned)batch->rows, (unsigned)a.c.heads, (unsigned)((a.group + kv::SIMPLE_HEADS - 1) / kv::SIMPLE_HEADS));
     KLAUNCH(st, grid, 128, 0, (kv::attend_simple_kernel), a);
     return KTMOE_OK;

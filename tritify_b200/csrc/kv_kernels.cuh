@@ -297,6 +297,7 @@ struct AttendArgs {
     int window, sinks;
     int32_t* o;
     long long ld_o;
+    int vec_o;  // rows of o are 16-byte aligned
     longlong2* o_scale;  // [rows][KV heads]
 };
 
@@ -323,9 +324,11 @@ __device__ __forceinline__ float weight(float x, float top, float theta) {
 __device__ __forceinline__ int scale_exp(uint32_t sigma) { return (int)(sigma >> 7) - 127 + ((sigma & 127) != 0); }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// A query row's codes (packed into its int8 row) and theta, by a whole warp. stage: head_dim int32 of shared memory.
+// A query row's codes and theta, by a whole warp. stage: head_dim int32 of shared memory. dst: the row's int8 codes; with
+// SW128, row r of a K-major operand in 128-byte blocks of 16384 bytes with the 128-byte swizzle.
+template <bool SW128>
 __device__ __forceinline__ float quantise_query(int8_t* dst, int32_t* stage, const int32_t* src, int dim, int vec,
-                                                const Rope& rope, const int2* cs, double s, double soft) {
+                                                const Rope& rope, const int2* cs, double s, double soft, int r = 0) {
     const int lane = threadIdx.x & 31;
     stage_row(stage, src, dim, vec);
     int64_t y[8];
@@ -351,7 +354,7 @@ __device__ __forceinline__ float quantise_query(int8_t* dst, int32_t* stage, con
             o.y = (signed char)code8(y[4 * i + 1], m);
             o.z = (signed char)code8(y[4 * i + 2], m);
             o.w = (signed char)code8(y[4 * i + 3], m);
-            *(char4*)(dst + e) = o;
+            *(char4*)(dst + (SW128 ? i * 16384 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3) : e)) = o;
         }
     }
     __syncwarp();
