@@ -11,8 +11,8 @@
 // in its pages, the MN-major operand). The int32 sums hold 132104 keys (127 * 128 each); every 131072 keys the carry of
 // lo goes into hi and that of hi into a 16-bit word of shared memory, which holds 2^25 keys.
 //
-// Roles (352 threads): warps 0-7 softmax (warp w: TMEM lanes 32 (w % 4) .., keys 64 (w / 4) .. of the tile), warp 8 TMA,
-// warp 9 MMA, warp 10 the keys' scales. Waits are bounded as in digit_gemm.cuh.
+// Roles (640 threads): warps 0-15 softmax, in two groups that take the tiles in turn; warp 16 TMA, warp 17 the products of
+// the scores, warp 18 the keys' scales, warp 19 the products of the values. Waits are bounded as in digit_gemm.cuh.
 #pragma once
 
 #include <cuda.h>
@@ -58,11 +58,21 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
-// Shared-memory descriptor of an MN-major operand one 128-byte block wide, with the 128-byte swizzle: rows are steps of
-// K, 8-row groups 1024 bytes apart (the other stride, between blocks, is not used).
-__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(1024 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// Low words of shared-memory descriptors with the 128-byte swizzle: the address in units of 16 bytes and a stride. K-major
+// operands do not use the stride; an MN-major operand one 128-byte block wide has rows that are steps of K, and neither
+// does it. The high word (8-row groups 1024 bytes apart, version, swizzle) is the same for all.
+constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | 1u << 16; }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return (addr >> 4) | (1024u >> 4) << 16; }
+
+// D += A B (or D = A B, accumulate = 0) of 8-bit operands given by their descriptors' low words.
+__device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(DESC_HI)
+        : "memory");
 }
 
 // kind::i8, s32 += s8 x s8, M = 128, N = n; `mn` bits 15 and 16: A, B MN-major.
@@ -102,13 +112,22 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const int32_t (&r)[16]
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 
+// 32 TMEM columns of 3 * 2^22, what the scores of a tile are summed onto (see scaled2).
+__device__ __forceinline__ void tmem_fill32(uint32_t taddr) {
+    const uint32_t v = 0x4B400000u;
+#pragma unroll
+    for (int c = 0; c < 32; c += 8)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1};" ::"r"(taddr + c), "r"(v));
+}
+
 constexpr float MAGIC = 12582912.0f;  // 3 * 2^22: adding it rounds to a whole number, left in the low bits
 constexpr uint32_t MAGIC_BITS = 0x4B400000u;
 
-// A dot product s (|s| <= 2^22) of two adjacent keys times their scales, RN24: s + 3 * 2^22 as a float is an integer
-// addition, and (3 * 2^22 + s) sigma - 3 * 2^22 sigma is one fused operation, whose constant is exact.
+// Dot products s (|s| <= 2^22) of two adjacent keys times their scales, RN24. The products are summed onto the bits of
+// 3 * 2^22, so what arrives is 3 * 2^22 + s as a float, and (3 * 2^22 + s) sigma - 3 * 2^22 sigma is one fused operation
+// whose constant is exact.
 __device__ __forceinline__ f2 scaled2(int32_t s0, int32_t s1, f2 sigma, f2 csigma) {
-    return fma2(pk(__int_as_float(s0 + (int)MAGIC_BITS), __int_as_float(s1 + (int)MAGIC_BITS)), sigma, csigma);
+    return fma2(pk(__int_as_float(s0), __int_as_float(s1)), sigma, csigma);
 }
 
 // What a row's weights need: the maximum, -theta, the cubic's coefficients times 2^-E, and 2^E.
@@ -168,14 +187,14 @@ struct KeyTiles {
     __device__ __forceinline__ int at(int i) const { return i < n_sink ? i : i - n_sink + first; }
 };
 
-// Bit k set: key j0 + k (k < 64) is visible to a row at position pos.
-__device__ __forceinline__ uint64_t seen_bits(int j0, int pos, int window, int sinks) {
-    auto below = [&](int end) -> uint64_t {  // keys j < end
+// Bit k set: key j0 + k (k < 32) is visible to a row at position pos.
+__device__ __forceinline__ uint32_t seen_bits(int j0, int pos, int window, int sinks) {
+    auto below = [&](int end) -> uint32_t {  // keys j < end
         const int k = end - j0;
-        return k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1;
+        return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1;
     };
     if (pos < 0) return 0;
-    uint64_t m = below(pos + 1);
+    uint32_t m = below(pos + 1);
     if (window && pos >= window) m &= ~below(pos + 1 - window) | below(sinks);
     return m;
 }
@@ -201,20 +220,24 @@ __device__ __forceinline__ int warp_search(int n, long long target, F f) {
 template <int NK>
 struct TileCfg {
     static constexpr int SLOT = TILE_KEYS * 128;  // bytes of one block of a key or value tile
-    static constexpr int SLOTS = NK == 1 ? 6 : 5;
+    static constexpr int K_SLOTS = 3, V_SLOTS = NK == 1 ? 3 : 2;  // rings of K and V blocks
+    static constexpr int SLOTS = K_SLOTS + V_SLOTS;
     static constexpr int SCALES = 4;  // tiles of key scales in flight
     static constexpr int Q = 0;
     static constexpr int P = Q + NK * SLOT;           // [2][hi, lo]
     static constexpr int RING = P + 4 * SLOT;
     static constexpr int CARRY = RING + SLOTS * SLOT;  // int16 [128 columns][128 rows]
-    static constexpr int KEY_SCALES = CARRY + TILE_ROWS * 128 * 2;  // [SCALES][sigma_k, -MAGIC sigma_k, sigma_v][128]
-    static constexpr int ROWS = KEY_SCALES + SCALES * 3 * TILE_KEYS * 4;  // theta, max [2], largest sigma [2], L [2]
-    static constexpr int BARS = ROWS + TILE_ROWS * (4 + 8 + 8 + 16);
+    // [SCALES]: sigma_k, -MAGIC sigma_k and sigma_v [128], the largest sigma_v
+    static constexpr int KEY_STAGE = 3 * TILE_KEYS + 4;
+    static constexpr int KEY_SCALES = CARRY + TILE_ROWS * 128 * 2;
+    static constexpr int ROWS = KEY_SCALES + SCALES * KEY_STAGE * 4;  // theta, max [4], largest sigma [4], L [4]
+    static constexpr int BARS = ROWS + TILE_ROWS * (4 + 16 + 16 + 32);
     static constexpr int BYTES = 1024 + BARS + 512;
     static_assert(BYTES <= 232448, "shared memory per block");
 };
 
-constexpr int TILE_THREADS = 352;
+constexpr int SOFTMAX_WARPS = 16;
+constexpr int TILE_THREADS = 32 * (SOFTMAX_WARPS + 4);
 constexpr int FLUSH_TILES = 1024;  // 131072 keys: |sum| <= 131072 * 127 * 128 < 2^31
 
 template <int NK>
@@ -227,9 +250,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     float* s_theta = (float*)(sm + C::ROWS);
     float* s_top = s_theta + TILE_ROWS;
-    uint32_t* s_sig = (uint32_t*)(s_top + 2 * TILE_ROWS);
-    unsigned long long* s_total = (unsigned long long*)(s_sig + 2 * TILE_ROWS);
-    uint64_t* full = (uint64_t*)(sm + C::BARS);  // [SLOTS] a block of K or V has landed
+    uint32_t* s_sig = (uint32_t*)(s_top + 4 * TILE_ROWS);
+    unsigned long long* s_total = (unsigned long long*)(s_sig + 4 * TILE_ROWS);
+    uint64_t* full = (uint64_t*)(sm + C::BARS);  // [SLOTS] a block of K or V has landed (K's slots, then V's)
     uint64_t* empty = full + C::SLOTS;           // [SLOTS] its products are done
     uint64_t* s_full = empty + C::SLOTS;         // [2] scores in TMEM
     uint64_t* s_free = s_full + 2;               // [2] scores read
@@ -240,8 +263,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     uint64_t* q_full = k_free + C::SCALES;
     uint64_t* o_full = q_full + 1;
     uint64_t* o_free = o_full + 1;
-    uint64_t* done = o_free + 1;
-    uint32_t* tmem_slot = (uint32_t*)(done + 1);
+    uint64_t* done = o_free + 1;  // [2] every product of an issuing warp is done
+    uint32_t* tmem_slot = (uint32_t*)(done + 2);
     int* s_job = (int*)(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -277,18 +300,19 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&s_free[i], 8);
-            mbar_init(&p_full[i], 8);
+            mbar_init(&s_free[i], SOFTMAX_WARPS / 2);
+            mbar_init(&p_full[i], SOFTMAX_WARPS / 2);
             mbar_init(&p_free[i], 1);
         }
         for (int i = 0; i < C::SCALES; ++i) {
             mbar_init(&k_full[i], 1);
-            mbar_init(&k_free[i], 8);
+            mbar_init(&k_free[i], SOFTMAX_WARPS / 2);
         }
-        mbar_init(q_full, 8);
+        mbar_init(q_full, SOFTMAX_WARPS);
         mbar_init(o_full, 1);
-        mbar_init(o_free, 8);
-        mbar_init(done, 1);
+        mbar_init(o_free, SOFTMAX_WARPS);
+        mbar_init(&done[0], 1);
+        mbar_init(&done[1], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
@@ -311,20 +335,28 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     const uint32_t tmem = *tmem_slot;
     const int ps = 1 << a.c.page_shift;
 
-    if (warp == 8) {
-        // K of pass 0; then, per value block, K of tile i + 1 ahead of V of tile i, as the products take them
-        const int per_tile = TILE_KEYS >> a.c.page_shift;
-        uint32_t q = 0;
+    if (warp == SOFTMAX_WARPS) {
+        // Step i takes K of tile i and, after pass 0, V of tile i - 1. A lane holds one page of a tile; page numbers are
+        // read three steps ahead.
+        const int per_tile = TILE_KEYS >> a.c.page_shift, last_page = p1 >> a.c.page_shift;
+        const int* pages = a.b.pages + (long long)seq * a.b.max_pages;
+        int ks = 0, vs = C::K_SLOTS;                // the next slots
+        uint32_t kph = 1, vph = 1, kq = 0, vq = 0;  // the parities of their release; blocks loaded so far
         bool alive = true;
-        auto load = [&](const CUtensorMap* map, int tile, int x) {
-            const int s = q % C::SLOTS;
+        auto page_of = [&](int i) -> int {
+            const int at = kt_.at(min(i, n - 1)) * per_tile + lane;
+            return lane < per_tile && at <= last_page ? pages[at] : 0;
+        };
+        auto load = [&](const CUtensorMap* map, int i, int x, int page, int s, uint32_t phase) {
             // pages that hold keys up to the last row's position; the others' keys are not visible
-            const int i0 = tile * per_tile, np = min(per_tile, (p1 >> a.c.page_shift) - i0 + 1);
-            int page = 0;
-            if (lane < np) page = (int)pool_page(a.b, a.c, a.err, seq, i0 + lane);
+            const int np = min(per_tile, last_page - kt_.at(i) * per_tile + 1);
+            if ((unsigned)page >= (unsigned long long)a.c.n_pages) {
+                a.err.raise(a.err.bad_page);
+                page = 0;
+            }
             bool ok = true;
             if (lane == 0) {
-                ok = wait(&empty[s], ((q / C::SLOTS) & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_EMPTY);
+                ok = wait(&empty[s], phase, a.err.word, dg::ERR_TIMEOUT_EMPTY);
                 if (ok) mbar_arrive_expect_tx(&full[s], (uint32_t)(np * ps * 128));
             }
             ok = __shfl_sync(0xffffffffu, (int)ok, 0);
@@ -334,145 +366,206 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             }
             if (lane < np)
                 tma_load_4d(smem_u32(sm + C::RING + s * C::SLOT + lane * ps * 128), map, x, 0, head, page, &full[s]);
-            ++q;
         };
         for (int pass = 0; alive && pass < n_pass; ++pass) {
-            for (int i = 0; alive && i < n; ++i) {
-                if (pass == 0 || i == 0)
-                    for (int x = 0; alive && x < NK; ++x) load(&map_k, kt_.at(i), x * 128);
-                if (pass > 0) {
-                    if (i + 1 < n)
-                        for (int x = 0; alive && x < NK; ++x) load(&map_k, kt_.at(i + 1), x * 128);
-                    if (alive) load(&map_v, kt_.at(i), (pass - 1) * 128);
+            int pg[4];
+#pragma unroll
+            for (int j = 0; j < 3; ++j) pg[j] = page_of(j);
+            for (int i0 = 0; alive && i0 <= n; i0 += 4) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = i0 + j;
+                    if (!alive || i > n) break;
+                    if (i < n) {
+#pragma unroll
+                        for (int x = 0; x < NK; ++x) {
+                            if (alive) load(&map_k, i, x * 128, pg[j], ks, kph);
+                            kq += alive;
+                            if (alive && ++ks == C::K_SLOTS) ks = 0, kph ^= 1;
+                        }
+                    }
+                    if (pass > 0 && i > 0 && alive) {
+                        load(&map_v, i - 1, (pass - 1) * 128, pg[(j + 3) & 3], vs, vph);
+                        vq += alive;
+                        if (alive && ++vs == C::SLOTS) vs = C::K_SLOTS, vph ^= 1;
+                    }
+                    pg[(j + 3) & 3] = page_of(i + 3);
                 }
             }
         }
-        if (lane == 0)  // copies still in flight land before the block leaves
-            for (uint32_t j = q > (uint32_t)C::SLOTS ? q - C::SLOTS : 0; j < q; ++j)
-                dg::mbar_wait_drain(&full[j % C::SLOTS], (j / C::SLOTS) & 1u, a.err.word, dg::ERR_TIMEOUT_FULL);
-    } else if (warp == 9) {
+        if (lane == 0) {  // copies still in flight land before the block leaves
+            for (uint32_t j = kq > (uint32_t)C::K_SLOTS ? kq - C::K_SLOTS : 0; j < kq; ++j)
+                dg::mbar_wait_drain(&full[j % C::K_SLOTS], (j / C::K_SLOTS) & 1u, a.err.word, dg::ERR_TIMEOUT_FULL);
+            for (uint32_t j = vq > (uint32_t)C::V_SLOTS ? vq - C::V_SLOTS : 0; j < vq; ++j)
+                dg::mbar_wait_drain(&full[C::K_SLOTS + j % C::V_SLOTS], (j / C::V_SLOTS) & 1u, a.err.word,
+                                    dg::ERR_TIMEOUT_FULL);
+        }
+    } else if (warp == SOFTMAX_WARPS + 1) {
+        // scores: S of tile after tile, as soon as K has landed and the buffer has been read
         if (lane == 0) {
             const int ksteps = (dim + 31) / 32;
-            uint32_t q = 0, sc = 0, pc = 0, oc = 0;
             const uint32_t id_s = idesc_i8(TILE_KEYS, 0);
-            auto scores = [&]() -> bool {
-                const uint32_t b = sc & 1;
-                if (!wait(&s_free[b], ((sc >> 1) & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM)) return false;
+            const uint32_t qd = desc_k(smem_u32(sm + C::Q)), kd = desc_k(smem_u32(sm + C::RING));
+            int ks = 0;
+            uint32_t kph = 0, b = 0, sph = 1;
+            bool ok = n_pass == 0 || wait(q_full, 0, a.err.word, dg::ERR_TIMEOUT_FULL);
+            for (int u = n_pass * n; ok && u > 0; --u) {
+                ok = wait(&s_free[b], sph, a.err.word, dg::ERR_TIMEOUT_ACCUM);
 #pragma unroll
                 for (int x = 0; x < NK; ++x) {
-                    const int s = q % C::SLOTS;
-                    if (!wait(&full[s], (q / C::SLOTS) & 1u, a.err.word, dg::ERR_TIMEOUT_FULL)) return false;
+                    ok = ok && wait(&full[ks], kph, a.err.word, dg::ERR_TIMEOUT_FULL);
+                    if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;");
-                    const uint32_t qa = smem_u32(sm + C::Q + x * C::SLOT), kb = smem_u32(sm + C::RING + s * C::SLOT);
-                    for (int kk = 0; kk < min(4, ksteps - 4 * x); ++kk)
-                        dg::umma_i8(tmem + b * 128, dg::smem_desc_sw128(qa + kk * 32), dg::smem_desc_sw128(kb + kk * 32), id_s,
-                                    x + kk > 0);
-                    umma_commit(&empty[s]);
-                    ++q;
-                }
-                umma_commit(&s_full[b]);
-                ++sc;
-                return true;
-            };
-            auto values = [&](int i, int cols) -> bool {
-                const uint32_t b = pc & 1;
-                const int s = q % C::SLOTS;
-                if (!wait(&p_full[b], (pc >> 1) & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM)) return false;
-                if (!wait(&full[s], (q / C::SLOTS) & 1u, a.err.word, dg::ERR_TIMEOUT_FULL)) return false;
-                asm volatile("tcgen05.fence::after_thread_sync;");
-                const uint32_t id_o = idesc_i8(cols, 1u << 16);
-                const uint32_t pa = smem_u32(sm + C::P + b * 2 * C::SLOT), vb = smem_u32(sm + C::RING + s * C::SLOT);
+                    // descriptors hold addresses in units of 16 bytes
+                    const uint32_t qx = qd + x * (C::SLOT >> 4), kx = kd + ks * (C::SLOT >> 4);
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    const uint64_t dv = desc_mn_sw128(vb + kk * 32 * 128);
-                    dg::umma_i8(tmem + 256, dg::smem_desc_sw128(pa + kk * 32), dv, id_o, i + kk > 0);
-                    dg::umma_i8(tmem + 384, dg::smem_desc_sw128(pa + C::SLOT + kk * 32), dv, id_o, i + kk > 0);
+                    for (int kk = 0; kk < 4; ++kk)
+                        if (4 * x + kk < ksteps) umma(tmem + b * 128, qx + 2 * kk, kx + 2 * kk, id_s, 1u);
+                    umma_commit(&empty[ks]);
+                    if (++ks == C::K_SLOTS) ks = 0, kph ^= 1;
                 }
-                umma_commit(&empty[s]);
-                umma_commit(&p_free[b]);
-                ++q;
-                ++pc;
-                return true;
-            };
-            bool ok = n_pass == 0 || wait(q_full, 0, a.err.word, dg::ERR_TIMEOUT_FULL);
-            for (int pass = 0; ok && pass < n_pass; ++pass) {
-                const int cols = min(128, dim - (pass - 1) * 128);
-                for (int i = 0; ok && i < n; ++i) {
-                    if (pass == 0 || i == 0) ok = ok && scores();
-                    if (pass > 0) {
-                        if (i + 1 < n) ok = ok && scores();
-                        ok = ok && values(i, cols);
-                        // the sums are read at the end of the block, and carried on every FLUSH_TILES tiles
-                        if (ok && (i + 1 == n || (i + 1) % FLUSH_TILES == 0)) {
-                            umma_commit(o_full);
-                            if (i + 1 < n || pass + 1 < n_pass) {
-                                ok = wait(o_free, oc & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
-                                asm volatile("tcgen05.fence::after_thread_sync;");
-                            }
-                            ++oc;
+                if (!ok) break;
+                umma_commit(&s_full[b]);
+                b ^= 1;
+                if (b == 0) sph ^= 1;
+            }
+            umma_commit(&done[0]);
+            dg::mbar_wait_drain(&done[0], 0u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+        }
+    } else if (warp == SOFTMAX_WARPS + 3) {
+        // the values: O += P V with both digits, as soon as a tile's weights are there
+        if (lane == 0) {
+            const uint32_t pd = desc_k(smem_u32(sm + C::P)), vd = desc_mn(smem_u32(sm + C::RING));
+            int vs = C::K_SLOTS;
+            uint32_t vph = 0, b = (uint32_t)n & 1, pph = 0, oc = 0;  // pass 1 begins with scores number n
+            bool ok = true, second = false;
+            for (int pass = 1; ok && pass < n_pass; ++pass) {
+                const uint32_t id_o = idesc_i8(min(128, dim - (pass - 1) * 128), 1u << 16);
+                for (int i = 0; i < n; ++i) {
+                    ok = wait(&p_full[b], pph, a.err.word, dg::ERR_TIMEOUT_ACCUM) &&
+                         wait(&full[vs], vph, a.err.word, dg::ERR_TIMEOUT_FULL);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                    const uint32_t px = pd + b * (2 * C::SLOT >> 4), vx = vd + vs * (C::SLOT >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        umma(tmem + 256, px + 2 * kk, vx + kk * (32 * 128 >> 4), id_o, i + kk > 0);
+                        umma(tmem + 384, px + (C::SLOT >> 4) + 2 * kk, vx + kk * (32 * 128 >> 4), id_o, i + kk > 0);
+                    }
+                    umma_commit(&empty[vs]);
+                    umma_commit(&p_free[b]);
+                    if (++vs == C::SLOTS) vs = C::K_SLOTS, vph ^= 1;
+                    b ^= 1;
+                    if (second) pph ^= 1;
+                    second = !second;
+                    // the sums are read at the end of the block, and carried on every FLUSH_TILES tiles
+                    if (i + 1 == n || (i + 1) % FLUSH_TILES == 0) {
+                        umma_commit(o_full);
+                        if (i + 1 < n || pass + 1 < n_pass) {
+                            ok = wait(o_free, oc & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+                            if (!ok) break;
+                            asm volatile("tcgen05.fence::after_thread_sync;");
                         }
+                        ++oc;
                     }
                 }
             }
-            umma_commit(done);
-            dg::mbar_wait_drain(done, 0u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+            umma_commit(&done[1]);
+            dg::mbar_wait_drain(&done[1], 0u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
         }
-    } else if (warp == 10) {
-        // the scales of each tile's keys, four keys a lane
-        uint32_t kc = 0;
-        bool alive = true;
-        for (int pass = 0; alive && pass < n_pass; ++pass) {
-            for (int i = 0; alive && i < n; ++i, ++kc) {
-                const int st = kc % C::SCALES;
-                const int j = kt_.at(i) * TILE_KEYS + 4 * lane;
-                ushort4 k4 = {0, 0, 0, 0}, v4 = {0, 0, 0, 0};
-                if (j <= p1) {
-                    const long long page = pool_page(a.b, a.c, a.err, seq, j >> a.c.page_shift);
-                    const long long row = ((page * a.c.heads + head) << a.c.page_shift) + (j & (ps - 1));
-                    k4 = *(const ushort4*)(a.c.ks + row);
-                    v4 = *(const ushort4*)(a.c.vs + row);
+    } else if (warp == SOFTMAX_WARPS + 2) {
+        // The scales of each tile's keys, four keys a lane: read four tiles ahead, their page numbers eight.
+        const int* pages = a.b.pages + (long long)seq * a.b.max_pages;
+        const int total = n_pass * n;
+        auto key_of = [&](int u) {
+            for (; u >= n; u -= n) {}  // at most two passes back
+            return kt_.at(u) * TILE_KEYS + 4 * lane;
+        };
+        auto page_of = [&](int u) -> int {
+            const int j = u < total ? key_of(u) : p1 + 1;
+            return j <= p1 ? pages[j >> a.c.page_shift] : 0;
+        };
+        auto scales_of = [&](int u, int page) -> uint4 {  // four bfloat16 of K, four of V
+            uint4 r = {0, 0, 0, 0};
+            const int j = u < total ? key_of(u) : p1 + 1;
+            if (j <= p1) {
+                if ((unsigned)page >= (unsigned long long)a.c.n_pages) {
+                    a.err.raise(a.err.bad_page);
+                    page = 0;
                 }
-                alive = wait(&k_free[st], ((kc / C::SCALES) & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_EMPTY);
-                alive = __all_sync(0xffffffffu, alive);
-                if (!alive) break;
-                float* f = (float*)(sm + C::KEY_SCALES) + st * 3 * TILE_KEYS;
-                const float4 kf = {bf16_value(k4.x), bf16_value(k4.y), bf16_value(k4.z), bf16_value(k4.w)};
-                *(float4*)(f + 4 * lane) = kf;
-                *(float4*)(f + TILE_KEYS + 4 * lane) = {-MAGIC * kf.x, -MAGIC * kf.y, -MAGIC * kf.z, -MAGIC * kf.w};
-                *(float4*)(f + 2 * TILE_KEYS + 4 * lane) = {bf16_value(v4.x), bf16_value(v4.y), bf16_value(v4.z),
-                                                            bf16_value(v4.w)};
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&k_full[st]);
+                const long long row = (((long long)page * a.c.heads + head) << a.c.page_shift) + (j & (ps - 1));
+                const uint2 k = __ldg((const uint2*)(a.c.ks + row)), v = __ldg((const uint2*)(a.c.vs + row));
+                r = make_uint4(k.x, k.y, v.x, v.y);
+            }
+            return r;
+        };
+        if (total > 0) {
+            int pg[4];
+            uint4 val[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pg[j] = page_of(j);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                val[j] = scales_of(j, pg[j]);
+                pg[j] = page_of(j + 4);
+            }
+            bool alive = true;
+            for (int u0 = 0; alive && u0 < total; u0 += 4) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {  // stage j: C::SCALES is 4
+                    const int u = u0 + j;
+                    if (u >= total || !alive) break;
+                    alive = wait(&k_free[j], ((u >> 2) & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_EMPTY);
+                    alive = __all_sync(0xffffffffu, alive);
+                    if (!alive) break;
+                    float* f = (float*)(sm + C::KEY_SCALES) + j * C::KEY_STAGE;
+                    const uint4 w = val[j];
+                    const uint32_t hi16 = 0xffff0000u;
+                    const float4 kf = {__uint_as_float(w.x << 16), __uint_as_float(w.x & hi16),
+                                       __uint_as_float(w.y << 16), __uint_as_float(w.y & hi16)};
+                    const uint4 vf = {w.z << 16, w.z & hi16, w.w << 16, w.w & hi16};
+                    *(float4*)(f + 4 * lane) = kf;
+                    *(float4*)(f + TILE_KEYS + 4 * lane) = {-MAGIC * kf.x, -MAGIC * kf.y, -MAGIC * kf.z, -MAGIC * kf.w};
+                    *(uint4*)(f + 2 * TILE_KEYS + 4 * lane) = vf;
+                    const unsigned big = max(max(vf.x, vf.y), max(vf.z, vf.w));
+                    const unsigned tile_big = __reduce_max_sync(0xffffffffu, big);
+                    if (lane == 0) ((uint32_t*)f)[3 * TILE_KEYS] = tile_big;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&k_full[j]);
+                    val[j] = scales_of(u + 4, pg[j]);
+                    pg[j] = page_of(u + 8);
+                }
             }
         }
     } else {
-        // the queries: codes into the K-major operand, theta
-        {
-            // staging over the weights' digits, which come later
-            int32_t* stage = (int32_t*)(sm + C::P) + warp * MAX_DIM;
-            for (int r = warp; r < n_rows && n_pass; r += 8) {
-                const int t = (row0 + r) / g, hq = head * g + (row0 + r) % g;
-                const int pos = len - n_new + t;
-                if (pos < 0) continue;
-                const long long row = (long long)begin + t;
-                const int2* cs = rope_row(a.rope, a.err, pos);
-                const double s = scale_value(a.scale[row * a.scale_stride], cs ? 30 : 0);
-                const float th = quantise_query<true>((int8_t*)sm + C::Q + r * 128, stage,
-                                                      a.q + row * a.ld_q + (long long)hq * dim, dim, a.vec, a.rope, cs,
-                                                      s, a.soft, r);
-                if (lane == 0) s_theta[r] = th;
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
-        }
-        const int quad = warp & 3, half = warp >> 2;
+        // Two groups of eight warps take the tiles in turn, each with its own buffer of scores and of digits, so that
+        // one group's waits pass under the other's arithmetic. A warp has the rows of TMEM lanes 32 quad .. and the
+        // keys 64 part .. of its group's tiles.
+        const int quad = warp & 3, part = (warp >> 2) & 1, grp = warp >> 3;
+        const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
+        const uint32_t s_addr = lane_addr + grp * 128 + part * 64;
+        tmem_fill32(s_addr);
+        tmem_fill32(s_addr + 32);
+        // the queries: codes into the K-major operand, theta; 8 rows a warp
+        constexpr int Q_WARP = TILE_ROWS / SOFTMAX_WARPS;
+        if (n_pass > 0 && Q_WARP * warp < n_rows)
+            quantise_rows<Q_WARP, NK>(
+                a, [&](int r) -> QueryRow {
+                    if (r >= n_rows) return {-1, -1, 0};
+                    const int t = (row0 + r) / g;
+                    return {len - n_new + t, (long long)begin + t, head * g + (row0 + r) % g};
+                },
+                Q_WARP * warp, (int8_t*)sm + C::Q, s_theta);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
         const int r = quad * 32 + lane;  // row of the tile
         const bool row_live = r < n_rows;
         const int t = (row0 + min(r, n_rows - 1)) / g;
         const int pos = row_live ? len - n_new + t : -1;
-        const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
-        uint32_t sc = 0, pc = 0, oc = 0;
+        uint32_t sc = 0, oc = 0;  // sc: number of the scores at hand, over all passes
         bool ok = true;
         float top = -INFINITY;
         uint32_t sig = 0;
@@ -481,61 +574,63 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             if (j0 + TILE_KEYS - 1 > p0) return false;
             return !a.window || j0 > p1 - a.window || j0 + TILE_KEYS <= a.sinks;
         };
-        int32_t s32[2][32];
-        // this thread's 64 scores of the next tile; its key scales are ready then
+        // the first tile of a pass that this group takes: scores number sc with sc % 2 == grp
+        auto first_of = [&](int pass) { return (grp ^ (pass * n)) & 1; };
+        int32_t s32[32];
+        // wait for scores number sc and their key scales
         auto next_scores = [&]() {
-            const uint32_t b = sc & 1;
-            ok = wait(&s_full[b], (sc >> 1) & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+            ok = wait(&s_full[grp], (sc >> 1) & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM) &&
+                 wait(&k_full[sc % C::SCALES], (sc / C::SCALES) & 1u, a.err.word, dg::ERR_TIMEOUT_FULL);
             ok = __all_sync(0xffffffffu, ok);
-            if (!ok) return;
             asm volatile("tcgen05.fence::after_thread_sync;");
-            dg::tmem_ld32(lane_addr + b * 128 + half * 64, s32[0]);
-            dg::tmem_ld32(lane_addr + b * 128 + half * 64 + 32, s32[1]);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            asm volatile("tcgen05.fence::before_thread_sync;");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free[b]);
-            ok = wait(&k_full[sc % C::SCALES], (sc / C::SCALES) & 1u, a.err.word, dg::ERR_TIMEOUT_FULL);
-            ok = __all_sync(0xffffffffu, ok);
         };
+        // 32 of this thread's 64 scores; after the second half the buffer goes back to the products
+        auto load_scores = [&](int c) {
+            dg::tmem_ld32(s_addr + c * 32, s32);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            tmem_fill32(s_addr + c * 32);
+            if (c == 1) {
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_free[grp]);
+            }
+        };
+        auto key_scales = [&]() { return (const float*)(sm + C::KEY_SCALES) + (sc % C::SCALES) * C::KEY_STAGE + part * 64; };
         auto scales_read = [&]() {
             __syncwarp();
             if (lane == 0) mbar_arrive(&k_free[sc % C::SCALES]);
-            ++sc;
         };
         // ── pass 0: the maxima ──
-        for (int i = 0; ok && n_pass && i < n; ++i) {
+        for (int i = first_of(0); ok && n_pass && i < n; i += 2) {
+            sc = i;
             next_scores();
             if (!ok) break;
             const int j0 = kt_.at(i) * TILE_KEYS;
-            const float* f = (const float*)(sm + C::KEY_SCALES) + (sc % C::SCALES) * 3 * TILE_KEYS + half * 64;
-            if (whole(j0)) {
+            const bool all = whole(j0);
+            if (all) sig = max(sig, ((const uint32_t*)key_scales())[3 * TILE_KEYS - part * 64]);
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 2; ++c) {
+                const float* f = key_scales() + c * 32;
+                load_scores(c);
+                if (all) {
 #pragma unroll
                     for (int k = 0; k < 32; k += 4) {
-                        const ulonglong2 kf = *(const ulonglong2*)(f + c * 32 + k);
-                        const ulonglong2 kc = *(const ulonglong2*)(f + TILE_KEYS + c * 32 + k);
-                        const uint4 vf = *(const uint4*)(f + 2 * TILE_KEYS + c * 32 + k);
+                        const ulonglong2 kf = *(const ulonglong2*)(f + k), kc = *(const ulonglong2*)(f + TILE_KEYS + k);
                         float x0, x1, x2, x3;
-                        upk(scaled2(s32[c][k], s32[c][k + 1], kf.x, kc.x), x0, x1);
-                        upk(scaled2(s32[c][k + 2], s32[c][k + 3], kf.y, kc.y), x2, x3);
+                        upk(scaled2(s32[k], s32[k + 1], kf.x, kc.x), x0, x1);
+                        upk(scaled2(s32[k + 2], s32[k + 3], kf.y, kc.y), x2, x3);
                         top = fmaxf(fmaxf(top, x0), x1);
                         top = fmaxf(fmaxf(top, x2), x3);
-                        sig = max(max(sig, vf.x), vf.y);
-                        sig = max(max(sig, vf.z), vf.w);
                     }
-            } else {
-                const uint64_t seen = seen_bits(j0 + half * 64, pos, a.window, a.sinks);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const uint32_t m = (uint32_t)(seen >> (32 * c));
+                } else {
+                    const uint32_t m = seen_bits(j0 + part * 64 + c * 32, pos, a.window, a.sinks);
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
-                        const f2 kf = *(const f2*)(f + c * 32 + k), kc = *(const f2*)(f + TILE_KEYS + c * 32 + k);
-                        const uint2 vf = *(const uint2*)(f + 2 * TILE_KEYS + c * 32 + k);
+                        const f2 kf = *(const f2*)(f + k), kc = *(const f2*)(f + TILE_KEYS + k);
+                        const uint2 vf = *(const uint2*)(f + 2 * TILE_KEYS + k);
                         float x0, x1;
-                        upk(scaled2(s32[c][k], s32[c][k + 1], kf, kc), x0, x1);
+                        upk(scaled2(s32[k], s32[k + 1], kf, kc), x0, x1);
                         if (m >> k & 1) {
                             top = fmaxf(top, x0);
                             sig = max(sig, vf.x);
@@ -549,49 +644,88 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             }
             scales_read();
         }
-        // the two halves of a row meet
-        s_top[half * TILE_ROWS + r] = top;
-        s_sig[half * TILE_ROWS + r] = sig;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        top = fmaxf(s_top[r], s_top[TILE_ROWS + r]);
-        sig = max(s_sig[r], s_sig[TILE_ROWS + r]);
+        // the four parts of a row (two groups, two halves of a tile) meet
+        const int mine = (grp * 2 + part) * TILE_ROWS + r;
+        s_top[mine] = top;
+        s_sig[mine] = sig;
+        asm volatile("bar.sync 1, 512;" ::: "memory");
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            top = fmaxf(top, s_top[p * TILE_ROWS + r]);
+            sig = max(sig, s_sig[p * TILE_ROWS + r]);
+        }
         const int e_row = sig ? scale_exp(sig >> 16) : 0;
         const RowWeights rw = row_weights(top, row_live && pos >= 0 ? s_theta[r] : 0.0f, e_row);
         uint64_t total = 0;
         bool met = n_pass == 0;
         int16_t* carry = (int16_t*)(sm + C::CARRY);
+        const int col0 = (grp * 2 + part) * 32;  // the columns of the sums that this warp reads
         // ── the weights and the sums ──
+        uint32_t used = 0;  // times this group's digit buffer has been filled
         for (int pass = 1; ok && pass < n_pass; ++pass) {
             const int cols = min(128, dim - (pass - 1) * 128);
-            bool carried = false;
-            for (int i = 0; ok && i < n; ++i) {
+            int flushed = 0;
+            auto flush = [&]() {
+                ok = wait(o_full, oc & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                asm volatile("tcgen05.fence::after_thread_sync;");
+                for (int c = col0; c < min(cols, col0 + 32); c += 16) {
+                    int32_t h[16], l[16];
+                    dg::tmem_ld16(lane_addr + 256 + c, h);
+                    dg::tmem_ld16(lane_addr + 384 + c, l);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        // lo = 256 q + rest: q into hi; hi = 2^24 q + rest: q into the carry
+                        h[k] += l[k] >> 8;
+                        l[k] &= 255;
+                        int16_t* cw = carry + (c + k) * TILE_ROWS + r;
+                        *cw = (int16_t)((flushed ? *cw : 0) + (h[k] >> 24));
+                        h[k] &= 0xffffff;
+                    }
+                    tmem_st16(lane_addr + 256 + c, h);
+                    tmem_st16(lane_addr + 384 + c, l);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_free);
+                ++flushed;
+                ++oc;
+            };
+            for (int i = first_of(pass); ok && i < n; i += 2) {
+                while (ok && flushed < i / FLUSH_TILES) flush();
+                if (!ok) break;
+                sc = pass * n + i;
                 next_scores();
                 if (!ok) break;
                 const int j0 = kt_.at(i) * TILE_KEYS;
-                const float* f = (const float*)(sm + C::KEY_SCALES) + (sc % C::SCALES) * 3 * TILE_KEYS + half * 64;
-                const uint32_t b = pc & 1;
-                ok = wait(&p_free[b], ((pc >> 1) & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_EMPTY);
+                const bool all = whole(j0);
+                ok = wait(&p_free[grp], (used & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_EMPTY);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                uint8_t* hi = sm + C::P + b * 2 * C::SLOT + r * 128;
+                uint8_t* hi = sm + C::P + grp * 2 * C::SLOT + r * 128;
                 uint8_t* lo = hi + C::SLOT;
                 uint32_t sum = 0;
-                auto digits = [&](auto mask_tag, uint64_t seen) {
-                    constexpr bool MASK = decltype(mask_tag)::value;
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    const float* f = key_scales() + c * 32;
+                    load_scores(c);
+                    auto digits = [&](auto mask_tag, uint32_t seen) {
+                        constexpr bool MASK = decltype(mask_tag)::value;
 #pragma unroll
                         for (int k16 = 0; k16 < 32; k16 += 16) {
                             uint32_t h4[4], l4[4];
 #pragma unroll
                             for (int k4 = 0; k4 < 4; ++k4) {
                                 const int k = k16 + 4 * k4;
-                                const ulonglong2 kf = *(const ulonglong2*)(f + c * 32 + k);
-                                const ulonglong2 kc = *(const ulonglong2*)(f + TILE_KEYS + c * 32 + k);
-                                const ulonglong2 vf = *(const ulonglong2*)(f + 2 * TILE_KEYS + c * 32 + k);
-                                const uint32_t m = MASK ? (uint32_t)(seen >> (32 * c + k)) : 0u;
-                                const f2 w0 = weight2<MASK>(scaled2(s32[c][k], s32[c][k + 1], kf.x, kc.x), rw, m);
-                                const f2 w1 = weight2<MASK>(scaled2(s32[c][k + 2], s32[c][k + 3], kf.y, kc.y), rw, m >> 2);
+                                const ulonglong2 kf = *(const ulonglong2*)(f + k);
+                                const ulonglong2 kc = *(const ulonglong2*)(f + TILE_KEYS + k);
+                                const ulonglong2 vf = *(const ulonglong2*)(f + 2 * TILE_KEYS + k);
+                                const uint32_t m = MASK ? seen >> k : 0u;
+                                const f2 w0 = weight2<MASK>(scaled2(s32[k], s32[k + 1], kf.x, kc.x), rw, m);
+                                const f2 w1 = weight2<MASK>(scaled2(s32[k + 2], s32[k + 3], kf.y, kc.y), rw, m >> 2);
                                 const f2 mg = pk(MAGIC, MAGIC), mg128 = pk(MAGIC + 128.0f, MAGIC + 128.0f);
                                 float a0, a1, a2, a3;
                                 upk(fma2(w0, rw.two_e, mg), a0, a1);
@@ -606,56 +740,31 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                                 l4[k4] = __byte_perm(u, v, 0x5410) ^ 0x80808080u;
                                 h4[k4] = __byte_perm(u, v, 0x7632);
                             }
-                            const int chunk = ((half * 4 + c * 2 + (k16 >> 4)) ^ (r & 7)) * 16;
+                            const int chunk = ((part * 4 + c * 2 + (k16 >> 4)) ^ (r & 7)) * 16;
                             *(uint4*)(hi + chunk) = make_uint4(h4[0], h4[1], h4[2], h4[3]);
                             *(uint4*)(lo + chunk) = make_uint4(l4[0], l4[1], l4[2], l4[3]);
                         }
-                };
-                if (whole(j0))
-                    digits(Bool<false>{}, 0);
-                else
-                    digits(Bool<true>{}, seen_bits(j0 + half * 64, pos, a.window, a.sinks));
+                    };
+                    if (all)
+                        digits(Bool<false>{}, 0);
+                    else
+                        digits(Bool<true>{}, seen_bits(j0 + part * 64 + c * 32, pos, a.window, a.sinks));
+                }
                 if (pass == 1) total += sum - 64u * MAGIC_BITS;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[b]);
-                ++pc;
+                if (lane == 0) mbar_arrive(&p_full[grp]);
+                ++used;
                 scales_read();
-                if ((i + 1) % FLUSH_TILES == 0 && i + 1 < n) {
-                    ok = wait(o_full, oc & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;");
-                    for (int c = half * 64; c < min(cols, half * 64 + 64); c += 16) {
-                        int32_t h[16], l[16];
-                        dg::tmem_ld16(lane_addr + 256 + c, h);
-                        dg::tmem_ld16(lane_addr + 384 + c, l);
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            // lo = 256 q + rest: q into hi; hi = 2^24 q + rest: q into the carry
-                            h[k] += l[k] >> 8;
-                            l[k] &= 255;
-                            int16_t* cw = carry + (c + k) * TILE_ROWS + r;
-                            *cw = (int16_t)((carried ? *cw : 0) + (h[k] >> 24));
-                            h[k] &= 0xffffff;
-                        }
-                        tmem_st16(lane_addr + 256 + c, h);
-                        tmem_st16(lane_addr + 384 + c, l);
-                    }
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                    asm volatile("tcgen05.fence::before_thread_sync;");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(o_free);
-                    carried = true;
-                    ++oc;
-                }
             }
-            if (pass == 1) {  // the row's total over both halves
-                s_total[half * TILE_ROWS + r] = total;
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+            while (ok && flushed < (n - 1) / FLUSH_TILES) flush();
+            if (pass == 1) {  // the row's total over its parts
+                s_total[mine] = total;
+                asm volatile("bar.sync 1, 512;" ::: "memory");
                 met = true;
-                total = s_total[r] + s_total[TILE_ROWS + r];
+                total = 0;
+#pragma unroll
+                for (int p = 0; p < 4; ++p) total += s_total[p * TILE_ROWS + r];
             }
             if (!ok) break;
             ok = wait(o_full, oc & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
@@ -666,7 +775,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             const double inv = total ? __ddiv_rn(2097152.0, (double)total) : 0.0;
             int32_t* out = a.o + ((long long)begin + t) * a.ld_o +
                            (long long)(head * g + (row0 + min(r, n_rows - 1)) % g) * dim + (pass - 1) * 128;
-            for (int c = half * 64; c < min(cols, half * 64 + 64); c += 16) {
+            for (int c = col0; c < min(cols, col0 + 32); c += 16) {
                 int32_t h[16], l[16];
                 dg::tmem_ld16(lane_addr + 256 + c, h);
                 dg::tmem_ld16(lane_addr + 384 + c, l);
@@ -675,7 +784,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         int64_t num = (int64_t)h[k] * 256 + l[k];
-                        if (carried) num += (int64_t)carry[(c + k) * TILE_ROWS + r] << 32;
+                        if (flushed) num += (int64_t)carry[(c + k) * TILE_ROWS + r] << 32;
                         h[k] = total ? out_code(num, inv) : 0;
                     }
                     if (a.vec_o) {
@@ -691,12 +800,12 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(o_free);
         }
-        if (!met) asm volatile("bar.sync 1, 256;" ::: "memory");  // a wait failed: the other warps still meet here
-        if (n_pass == 0 && row_live && half == 0) {  // no row of the tile sees anything
+        if (!met) asm volatile("bar.sync 1, 512;" ::: "memory");  // a wait failed: the other warps still meet here
+        if (n_pass == 0 && row_live && grp == 0 && part == 0) {  // no row of the tile sees anything
             int32_t* out = a.o + ((long long)begin + t) * a.ld_o + (long long)(head * g + (row0 + r) % g) * dim;
             for (int k = 0; k < dim; ++k) out[k] = 0;
         }
-        if (row_live && half == 0 && (row0 + r) % g == 0)
+        if (row_live && grp == 0 && part == 0 && (row0 + r) % g == 0)
             a.o_scale[((long long)begin + t) * a.c.heads + head] =
                 total ? make_longlong2(1, (long long)(uint32_t)(21 - e_row)) : make_longlong2(0, 0);
     }

@@ -362,8 +362,125 @@ __device__ __forceinline__ float quantise_query(int8_t* dst, int32_t* stage, con
     return __double2float_rn(fmin(__dmul_rn(__ddiv_rn(__dmul_rn(td, s), 127.0), soft), 0x1p60));
 }
 
+// RN64 of a 64-bit integer and the nearest whole number to a double (ties to even, |v| < 2^31) on the FP64 pipe: the
+// conversion instructions run at a quarter of its rate. 2^52 + 2^31 + hi and 2^52 + lo are doubles whose low words are
+// the integer's halves.
+__device__ __forceinline__ double to_double(int64_t v) {
+    const double hi = __dsub_rn(__hiloint2double(0x43300000, (int)(v >> 32) ^ (int)0x80000000), 4503601774854144.0);
+    const double lo = __dsub_rn(__hiloint2double(0x43300000, (int)v), 4503599627370496.0);
+    return __fma_rn(hi, 4294967296.0, lo);
+}
+__device__ __forceinline__ double to_double(int32_t v) {
+    return __dsub_rn(__hiloint2double(0x43300000, v ^ (int)0x80000000), 4503601774854144.0);
+}
+__device__ __forceinline__ int to_int(double v) { return __double2loint(__dadd_rn(v, 6755399441055744.0)); }
+
+// Where a query row stands: its position, its row of the caller's buffers and its query head. pos < 0: no row.
+struct QueryRow {
+    int pos;
+    long long row;
+    int head;
+};
+
+// Four elements e .. e + 3 of a query row after the rotation. x: the row; cs: its row of the rotation table.
+__device__ __forceinline__ void rotated4(int64_t (&y)[4], const AttendArgs& a, const int32_t* x, const int2* cs, int e) {
+    int4 v;
+    if (a.vec) {
+        v = __ldg((const int4*)(x + e));
+    } else {
+        v = make_int4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+    }
+    const int half = a.rope.half;
+    if (!a.rope.table) {
+        y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
+    } else if (e >= 2 * half) {
+        y[0] = (int64_t)v.x << 30, y[1] = (int64_t)v.y << 30, y[2] = (int64_t)v.z << 30, y[3] = (int64_t)v.w << 30;
+    } else if (a.rope.interleaved && e + 4 <= 2 * half) {
+        const int2 c0 = __ldg(cs + e / 2), c1 = __ldg(cs + e / 2 + 1);
+        y[0] = (int64_t)v.x * c0.x - (int64_t)v.y * c0.y;
+        y[1] = (int64_t)v.y * c0.x + (int64_t)v.x * c0.y;
+        y[2] = (int64_t)v.z * c1.x - (int64_t)v.w * c1.y;
+        y[3] = (int64_t)v.w * c1.x + (int64_t)v.z * c1.y;
+    } else if (!a.rope.interleaved && half % 4 == 0 && a.vec) {
+        const bool first = e < half;
+        const int4 o = __ldg((const int4*)(x + (first ? e + half : e - half)));
+        const int2* c = cs + (first ? e : e - half);
+        const int2 c0 = __ldg(c), c1 = __ldg(c + 1), c2 = __ldg(c + 2), c3 = __ldg(c + 3);
+        const int sg = first ? -1 : 1;
+        y[0] = (int64_t)v.x * c0.x + (int64_t)o.x * (sg * c0.y);
+        y[1] = (int64_t)v.y * c1.x + (int64_t)o.y * (sg * c1.y);
+        y[2] = (int64_t)v.z * c2.x + (int64_t)o.z * (sg * c2.y);
+        y[3] = (int64_t)v.w * c3.x + (int64_t)o.w * (sg * c3.y);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = rotated(x, e + k, a.rope, cs);
+    }
+}
+
+// N query rows by one warp: codes of row r, r0 <= r < r0 + N, into row r of a K-major operand in 128-byte blocks with the
+// 128-byte swizzle (16384 bytes a block), theta into theta[r]. NB: blocks of a row. The rows are rotated twice, for
+// their largest element and for their codes (from L1 then), so that one division serves all rows and the loads of
+// many rows overlap: what this costs is latency, not work.
+template <int N, int NB, class RowOf>
+__device__ __forceinline__ void quantise_rows(const AttendArgs& a, RowOf row_of, int r0, int8_t* dst, float* theta) {
+    const int lane = threadIdx.x & 31, dim = a.c.dim;
+    uint64_t mine = 0;  // lane i: the largest element of row r0 + i
+#pragma unroll 4
+    for (int i = 0; i < N; ++i) {
+        const QueryRow at = row_of(r0 + i);
+        uint64_t top = 0;
+        if (at.pos >= 0) {
+            const int32_t* x = a.q + at.row * a.ld_q + (long long)at.head * dim;
+            const int2* cs = rope_row(a.rope, a.err, at.pos);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const int e = 4 * lane + 128 * b;
+                if (e >= dim) continue;
+                int64_t y[4];
+                rotated4(y, a, x, cs, e);
+                top = max(max(top, max(uabs(y[0]), uabs(y[1]))), max(uabs(y[2]), uabs(y[3])));
+            }
+        }
+        top = warp_umax(top);
+        if (lane == i) mine = top;
+    }
+    const double td = to_double((int64_t)mine);
+    const double m = __ddiv_rn(127.0, fmax(td, 1.0));
+    if (lane < N) {
+        const QueryRow me = row_of(r0 + lane);
+        if (me.pos >= 0) {
+            const double s = scale_value(a.scale[me.row * a.scale_stride], a.rope.table ? 30 : 0);
+            theta[r0 + lane] =
+                mine ? __double2float_rn(fmin(__dmul_rn(__ddiv_rn(__dmul_rn(td, s), 127.0), a.soft), 0x1p60)) : 0.0f;
+        }
+    }
+#pragma unroll 4
+    for (int i = 0; i < N; ++i) {
+        const QueryRow at = row_of(r0 + i);
+        const double mi = __shfl_sync(0xffffffffu, m, i);
+        if (at.pos < 0) continue;
+        const int32_t* x = a.q + at.row * a.ld_q + (long long)at.head * dim;
+        const int2* cs = rope_row(a.rope, a.err, at.pos);
+        const int r = r0 + i;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int e = 4 * lane + 128 * b;
+            if (e >= dim) continue;
+            int64_t y[4];
+            rotated4(y, a, x, cs, e);
+            // |y m| <= 127 (1 + 2^-52): the codes stay within +-127
+            char4 o;
+            o.x = (signed char)to_int(__dmul_rn(to_double(y[0]), mi));
+            o.y = (signed char)to_int(__dmul_rn(to_double(y[1]), mi));
+            o.z = (signed char)to_int(__dmul_rn(to_double(y[2]), mi));
+            o.w = (signed char)to_int(__dmul_rn(to_double(y[3]), mi));
+            *(char4*)(dst + b * 16384 + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)) = o;
+        }
+    }
+}
+
 __device__ __forceinline__ int32_t out_code(int64_t num, double inv) {
-    return __double2int_rn(__dmul_rn((double)num, inv));
+    return to_int(__dmul_rn(to_double(num), inv));
 }
 
 }  // namespace kv
