@@ -11,7 +11,6 @@ constexpr int SIMPLE_HEADS = 8;
 __global__ void __launch_bounds__(128) attend_simple_kernel(const AttendArgs a) {
     kt::pdl_enter();
     __shared__ __align__(16) int8_t q8[SIMPLE_HEADS][MAX_DIM];
-    __shared__ __align__(16) int32_t stage[4][MAX_DIM];
     __shared__ float theta[SIMPLE_HEADS];
     __shared__ float top[SIMPLE_HEADS];
     __shared__ float red[4][SIMPLE_HEADS];
@@ -34,10 +33,13 @@ __global__ void __launch_bounds__(128) attend_simple_kernel(const AttendArgs a) 
     const int2* cs = rope_row(a.rope, a.err, p.pos);
     const double s = scale_value(a.scale[(long long)t * a.scale_stride], cs ? 30 : 0);
     for (int i = warp; i < ng; i += 4) {
-        const float th = quantise_query<false>(q8[i], stage[warp],
-                                        a.q + (long long)t * a.ld_q + (long long)(h * a.group + g0 + i) * dim, dim,
-                                        a.vec, a.rope, cs, s, a.soft);
-        if (lane == 0) theta[i] = th;
+        RowBatch<2> rows;
+        const int32_t* x = a.q + (long long)t * a.ld_q + (long long)(h * a.group + g0 + i) * dim;
+        turn_rows<2>(rows, fetch_rows<2>(x, 1, dim, a.vec, a.rope), x, 1, dim, a.rope, cs);
+        const double m = __shfl_sync(0xffffffffu, __ddiv_rn(127.0, fmax(rows.top, 1.0)), 0);
+        for (int b = 0; b < 2; ++b)
+            if (4 * lane + 128 * b < dim) *(uint32_t*)(q8[i] + 4 * lane + 128 * b) = codes4<false>(rows.y[0][b], m);
+        if (lane == 0) theta[i] = row_theta(rows.top, s, a.soft);
     }
     for (int i = tid; i < SIMPLE_HEADS; i += 128) total[i] = 0;
     __syncthreads();

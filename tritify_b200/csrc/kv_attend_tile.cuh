@@ -256,7 +256,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     uint64_t* empty = full + C::SLOTS;           // [SLOTS] its products are done
     uint64_t* s_full = empty + C::SLOTS;         // [2] scores in TMEM
     uint64_t* s_free = s_full + 2;               // [2] scores read
-    uint64_t* p_full = s_free + 2;               // [2] digits of the weights in shared memory
+    uint64_t* m_full = s_free + 2;               // [4] the same in pass 0, which has no sums in TMEM and uses it all
+    uint64_t* m_free = m_full + 4;               // [4]
+    uint64_t* p_full = m_free + 4;               // [2] digits of the weights in shared memory
     uint64_t* p_free = p_full + 2;               // [2] their products are done
     uint64_t* k_full = p_free + 2;               // [SCALES]
     uint64_t* k_free = k_full + C::SCALES;       // [SCALES]
@@ -303,6 +305,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             mbar_init(&s_free[i], SOFTMAX_WARPS / 2);
             mbar_init(&p_full[i], SOFTMAX_WARPS / 2);
             mbar_init(&p_free[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&m_full[i], 1);
+            mbar_init(&m_free[i], SOFTMAX_WARPS / 2);
         }
         for (int i = 0; i < C::SCALES; ++i) {
             mbar_init(&k_full[i], 1);
@@ -407,10 +413,19 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             const uint32_t id_s = idesc_i8(TILE_KEYS, 0);
             const uint32_t qd = desc_k(smem_u32(sm + C::Q)), kd = desc_k(smem_u32(sm + C::RING));
             int ks = 0;
-            uint32_t kph = 0, b = 0, sph = 1;
+            uint32_t kph = 0;
             bool ok = n_pass == 0 || wait(q_full, 0, a.err.word, dg::ERR_TIMEOUT_FULL);
-            for (int u = n_pass * n; ok && u > 0; --u) {
-                ok = wait(&s_free[b], sph, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+            const int total = n_pass * n;
+            for (int u = 0; ok && u < total; ++u) {
+                // scores number u go to buffer u % 4 in pass 0 and to buffer u % 2 later, first when pass 0 has read it
+                const bool maxima = u < n;
+                const uint32_t b = maxima ? u & 3 : u & 1;
+                const uint32_t use = (uint32_t)(maxima ? u >> 2 : (u - n) >> 1);
+                if (!maxima && use == 0) {
+                    const uint32_t uses = (uint32_t)(n - (int)b + 3) / 4;
+                    ok = uses == 0 || wait(&m_free[b], (uses - 1) & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+                }
+                ok = ok && wait(maxima ? &m_free[b] : &s_free[b], (use & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
 #pragma unroll
                 for (int x = 0; x < NK; ++x) {
                     ok = ok && wait(&full[ks], kph, a.err.word, dg::ERR_TIMEOUT_FULL);
@@ -425,9 +440,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     if (++ks == C::K_SLOTS) ks = 0, kph ^= 1;
                 }
                 if (!ok) break;
-                umma_commit(&s_full[b]);
-                b ^= 1;
-                if (b == 0) sph ^= 1;
+                umma_commit(maxima ? &m_full[b] : &s_full[b]);
             }
             umma_commit(&done[0]);
             dg::mbar_wait_drain(&done[0], 0u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
@@ -544,18 +557,19 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         const int quad = warp & 3, part = (warp >> 2) & 1, grp = warp >> 3;
         const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
         const uint32_t s_addr = lane_addr + grp * 128 + part * 64;
-        tmem_fill32(s_addr);
-        tmem_fill32(s_addr + 32);
-        // the queries: codes into the K-major operand, theta; 8 rows a warp
-        constexpr int Q_WARP = TILE_ROWS / SOFTMAX_WARPS;
-        if (n_pass > 0 && Q_WARP * warp < n_rows)
-            quantise_rows<Q_WARP, NK>(
-                a, [&](int r) -> QueryRow {
-                    if (r >= n_rows) return {-1, -1, 0};
-                    const int t = (row0 + r) / g;
-                    return {len - n_new + t, (long long)begin + t, head * g + (row0 + r) % g};
-                },
-                Q_WARP * warp, (int8_t*)sm + C::Q, s_theta);
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) tmem_fill32(s_addr + (c >> 1) * 256 + (c & 1) * 32);
+        // the queries' codes, from where query_kernel left them, into the K-major operand
+        if (n_pass > 0) {
+            const int per_row = dim / 16;
+            for (int i = threadIdx.x; i < n_rows * per_row; i += 32 * SOFTMAX_WARPS) {
+                const int r = i / per_row, c = i - r * per_row, rr = row0 + r;
+                const int32_t* x = a.o + ((long long)begin + rr / g) * a.ld_o + (long long)(head * g + rr % g) * dim;
+                const int4 v = a.vec_o ? *(const int4*)(x + 4 * c) : make_int4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+                *(int4*)(sm + C::Q + (c >> 3) * C::SLOT + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+                if (c == 0) s_theta[r] = __int_as_float(x[dim / 4]);
+            }
+        }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -577,23 +591,23 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         // the first tile of a pass that this group takes: scores number sc with sc % 2 == grp
         auto first_of = [&](int pass) { return (grp ^ (pass * n)) & 1; };
         int32_t s32[32];
-        // wait for scores number sc and their key scales
-        auto next_scores = [&]() {
-            ok = wait(&s_full[grp], (sc >> 1) & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM) &&
+        // wait for scores number sc, the `use`th in their buffer, and their key scales
+        auto next_scores = [&](uint64_t* bar, uint32_t use) {
+            ok = wait(bar, use & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM) &&
                  wait(&k_full[sc % C::SCALES], (sc / C::SCALES) & 1u, a.err.word, dg::ERR_TIMEOUT_FULL);
             ok = __all_sync(0xffffffffu, ok);
             asm volatile("tcgen05.fence::after_thread_sync;");
         };
         // 32 of this thread's 64 scores; after the second half the buffer goes back to the products
-        auto load_scores = [&](int c) {
-            dg::tmem_ld32(s_addr + c * 32, s32);
+        auto load_scores = [&](uint32_t addr, int c, uint64_t* bar) {
+            dg::tmem_ld32(addr + c * 32, s32);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            tmem_fill32(s_addr + c * 32);
+            tmem_fill32(addr + c * 32);
             if (c == 1) {
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&s_free[grp]);
+                if (lane == 0) mbar_arrive(bar);
             }
         };
         auto key_scales = [&]() { return (const float*)(sm + C::KEY_SCALES) + (sc % C::SCALES) * C::KEY_STAGE + part * 64; };
@@ -604,7 +618,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         // ── pass 0: the maxima ──
         for (int i = first_of(0); ok && n_pass && i < n; i += 2) {
             sc = i;
-            next_scores();
+            next_scores(&m_full[i & 3], i >> 2);
             if (!ok) break;
             const int j0 = kt_.at(i) * TILE_KEYS;
             const bool all = whole(j0);
@@ -612,7 +626,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const float* f = key_scales() + c * 32;
-                load_scores(c);
+                load_scores(s_addr + (i & 2) * 128, c, &m_free[i & 3]);
                 if (all) {
 #pragma unroll
                     for (int k = 0; k < 32; k += 4) {
@@ -698,7 +712,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 while (ok && flushed < i / FLUSH_TILES) flush();
                 if (!ok) break;
                 sc = pass * n + i;
-                next_scores();
+                next_scores(&s_full[grp], (sc - n) >> 1);
                 if (!ok) break;
                 const int j0 = kt_.at(i) * TILE_KEYS;
                 const bool all = whole(j0);
@@ -711,7 +725,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 #pragma unroll 1
                 for (int c = 0; c < 2; ++c) {
                     const float* f = key_scales() + c * 32;
-                    load_scores(c);
+                    load_scores(s_addr, c, &s_free[grp]);
                     auto digits = [&](auto mask_tag, uint32_t seen) {
                         constexpr bool MASK = decltype(mask_tag)::value;
 #pragma unroll

@@ -73,6 +73,15 @@ int make_pool_map(ktmoe_ctx* ctx, CUtensorMap* map, const int8_t* pool, const kv
     return KTMOE_OK;
 }
 
+unsigned row_blocks(int64_t warps) { return (unsigned)((warps + kv::ROW_WARPS - 1) / kv::ROW_WARPS); }
+
+template <int NB>
+int launch_append(ktmoe_ctx* ctx, cudaStream_t st, const kv::AppendArgs& a) {
+    const int chunks = (a.c.heads + kv::RowBatch<NB>::B - 1) / kv::RowBatch<NB>::B;
+    KLAUNCH(st, row_blocks(a.b.rows * 2 * chunks), 32 * kv::ROW_WARPS, 0, (kv::append_kernel<NB>), a, chunks);
+    return KTMOE_OK;
+}
+
 template <int NK>
 int launch_tile(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
     static bool attr_set[64] = {};
@@ -81,11 +90,13 @@ int launch_tile(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
                                 kv::TileCfg<NK>::BYTES));
         attr_set[ctx->device & 63] = true;
     }
+    const int64_t slots = a.b.rows * a.group / kv::TILE_ROWS + a.b.n_seqs;
+    if (slots * a.c.heads > INT32_MAX) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "too many query rows for one launch");
     CUtensorMap mk, mv;
     if (int r = make_pool_map(ctx, &mk, a.c.k, a.c)) return r;
     if (int r = make_pool_map(ctx, &mv, a.c.v, a.c)) return r;
-    const int64_t slots = a.b.rows * a.group / kv::TILE_ROWS + a.b.n_seqs;
-    if (slots * a.c.heads > INT32_MAX) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "too many query rows for one launch");
+    const int chunks = (a.c.heads * a.group + kv::RowBatch<NK>::B - 1) / kv::RowBatch<NK>::B;
+    KLAUNCH(st, row_blocks(a.b.rows * chunks), 32 * kv::ROW_WARPS, 0, (kv::query_kernel<NK>), a, chunks);
     KLAUNCH(st, (unsigned)(slots * a.c.heads), kv::TILE_THREADS, kv::TileCfg<NK>::BYTES, (kv::attend_tile_kernel<NK>), mk,
             mv, a, (long long)slots);
     return KTMOE_OK;
@@ -133,8 +144,7 @@ int ktmoe_kv_append_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe
     a.scale_stride = scale_stride;
     a.vec = aligned(k, 16) && aligned(v, 16) && ld_k % 4 == 0 && ld_v % 4 == 0;
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
-    KLAUNCH(st, (unsigned)batch->rows, 32 * kv::APPEND_WARPS, 0, (kv::append_kernel), a);
-    return KTMOE_OK;
+    return a.c.dim <= 128 ? launch_append<1>(ctx, st, a) : launch_append<2>(ctx, st, a);
 }
 
 int ktmoe_kv_read_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, float* k, int64_t ld_k,
@@ -155,7 +165,7 @@ int ktmoe_kv_read_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_k
     a.ld_v = ld_v;
     a.vec = aligned(k, 16) && aligned(v, 16) && ld_k % 4 == 0 && ld_v % 4 == 0;
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
-    KLAUNCH(st, (unsigned)batch->rows, 32 * kv::APPEND_WARPS, 0, (kv::read_kernel), a);
+    KLAUNCH(st, (unsigned)batch->rows, 32 * kv::READ_WARPS, 0, (kv::read_kernel), a);
     return KTMOE_OK;
 }
 

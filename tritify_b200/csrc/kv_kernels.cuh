@@ -112,11 +112,9 @@ __device__ __forceinline__ double scale_value(longlong2 s, int extra_shift) {
     return s.x <= 0 ? 0.0 : ldexp((double)s.x, -shift);
 }
 
-// A row's codes after the rotation, four per lane and step: element e = 4 * lane + 128 * step.
-// x: the row's int32 codes (all of head_dim readable).
+// Element e of a row after the rotation. x: the row; cs: its row of the rotation table.
 __device__ __forceinline__ int64_t rotated(const int32_t* x, int e, const Rope& r, const int2* cs) {
     const int64_t v = x[e];
-    if (!cs) return v;
     if (e >= 2 * r.half) return v * (1 << 30);
     int j, mate;
     bool first;
@@ -131,7 +129,7 @@ __device__ __forceinline__ int64_t rotated(const int32_t* x, int e, const Rope& 
     }
     const int2 t = cs[j];
     const int64_t o = x[mate];
-    return first ? v * t.x - o * t.y : v * t.x + o * t.y;  // |.| <= 2^31 (2^30 + 2^30) = 2^62
+    return first ? v * t.x - o * t.y : v * t.x + o * t.y;
 }
 
 // The rotation table's row for a position, or null without rotation. A position beyond the table raises the error
@@ -155,14 +153,147 @@ __device__ __forceinline__ uint32_t sigma_bits(double t) {
 
 __device__ __forceinline__ float bf16_value(uint32_t bits) { return __uint_as_float(bits << 16); }
 
-// rne(RN64(y m)) held within +-127.
-__device__ __forceinline__ int code8(int64_t y, double m) {
-    return max(-127, min(127, __double2int_rn(__dmul_rn((double)y, m))));
+// RN64 of a 64-bit integer and the nearest whole number to a double (ties to even, |v| < 2^31) on the FP64 pipe: the
+// conversion instructions run at a quarter of its rate. 2^52 + 2^31 + hi and 2^52 + lo are doubles whose low words are
+// the integer's halves.
+__device__ __forceinline__ double to_double(int64_t v) {
+    const double hi = __dsub_rn(__hiloint2double(0x43300000, (int)(v >> 32) ^ (int)0x80000000), 4503601774854144.0);
+    const double lo = __dsub_rn(__hiloint2double(0x43300000, (int)v), 4503599627370496.0);
+    return __fma_rn(hi, 4294967296.0, lo);
+}
+__device__ __forceinline__ double to_double(int32_t v) {
+    return __dsub_rn(__hiloint2double(0x43300000, v ^ (int)0x80000000), 4503601774854144.0);
+}
+__device__ __forceinline__ int to_int(double v) { return __double2loint(__dadd_rn(v, 6755399441055744.0)); }
+
+// ── rows of codes: rotation, largest element, quantisation ──
+// A warp takes up to B heads of one token, which share the rotation's entries, the scale and one division; lane l has
+// the elements 4 l .. 4 l + 3 of each 128 (NB of them). Elements are turned into RN64 of their codes at once, which is
+// all that what follows needs: RN64 keeps the order, so the largest element's is the largest.
+template <int NB>
+struct RowBatch {
+    static constexpr int B = NB == 1 ? 4 : 2;
+    double y[B][NB][4];
+    double top;  // lane i: of head i
+};
+
+// The rotation's entries of elements e .. e + 3, the sine with the sign it takes. by_four: a four and its mates lie in
+// aligned fours (else element by element).
+__device__ __forceinline__ bool turns_by_four(const Rope& r) { return (r.interleaved ? 2 * r.half : r.half) % 4 == 0; }
+__device__ __forceinline__ void fetch_turn(int2 (&c)[4], const Rope& r, const int2* cs, int e) {
+    const int j = r.interleaved ? e / 2 : e < r.half ? e : e - r.half;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        c[k] = e < 2 * r.half ? __ldg(cs + j + (r.interleaved ? k >> 1 : k)) : make_int2(1 << 30, 0);
+        if (r.interleaved ? !(k & 1) : e < r.half) c[k].y = -c[k].y;
+    }
+}
+
+// The elements as they lie and those that the rotation mixes them with: asked for before anything is known of the row's
+// place, so that both arrive together. x: the first head's row, `heads` of them (the others count as zeros).
+template <int NB>
+struct RawBatch {
+    int4 v[RowBatch<NB>::B][NB], o[RowBatch<NB>::B][NB];
+};
+template <int NB>
+__device__ __forceinline__ RawBatch<NB> fetch_rows(const int32_t* __restrict__ x, int heads, int dim, int vec, const Rope& r) {
+    const int lane = threadIdx.x & 31;
+    const bool far = r.table && turns_by_four(r) && !r.interleaved;
+    auto four = [&](const int32_t* p) {
+        return vec ? __ldg((const int4*)p) : make_int4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+    };
+    RawBatch<NB> w;
+#pragma unroll
+    for (int i = 0; i < RowBatch<NB>::B; ++i)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int e = 4 * lane + 128 * b;
+            w.v[i][b] = w.o[i][b] = make_int4(0, 0, 0, 0);
+            if (i < heads && e < dim) w.v[i][b] = four(x + i * dim + e);
+            if (far && i < heads && e < 2 * r.half) w.o[i][b] = four(x + i * dim + (e < r.half ? e + r.half : e - r.half));
+        }
+    return w;
+}
+
+// cs: the rotation table's row (null: none).
+template <int NB>
+__device__ __forceinline__ void turn_rows(RowBatch<NB>& out, const RawBatch<NB>& w, const int32_t* __restrict__ x, int heads,
+                                          int dim, const Rope& r, const int2* cs) {
+    constexpr int B = RowBatch<NB>::B;
+    const int lane = threadIdx.x & 31;
+    const bool by_four = cs && turns_by_four(r);
+    const auto& v = w.v;
+    if (by_four) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            int2 c[4];
+            fetch_turn(c, r, cs, 4 * lane + 128 * b);
+#pragma unroll
+            for (int i = 0; i < B; ++i) {  // |.| <= 2^31 (2^30 + 2^30) = 2^62
+                const int4 p = v[i][b], q = r.interleaved ? make_int4(p.y, p.x, p.w, p.z) : w.o[i][b];
+                out.y[i][b][0] = to_double((int64_t)p.x * c[0].x + (int64_t)q.x * c[0].y);
+                out.y[i][b][1] = to_double((int64_t)p.y * c[1].x + (int64_t)q.y * c[1].y);
+                out.y[i][b][2] = to_double((int64_t)p.z * c[2].x + (int64_t)q.z * c[2].y);
+                out.y[i][b][3] = to_double((int64_t)p.w * c[3].x + (int64_t)q.w * c[3].y);
+            }
+        }
+    } else if (!cs) {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                out.y[i][b][0] = to_double(v[i][b].x);
+                out.y[i][b][1] = to_double(v[i][b].y);
+                out.y[i][b][2] = to_double(v[i][b].z);
+                out.y[i][b][3] = to_double(v[i][b].w);
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int e = 4 * lane + 128 * b + k;
+                    out.y[i][b][k] = i < heads && e < dim ? to_double(rotated(x + i * dim, e, r, cs)) : 0.0;
+                }
+    }
+    // the largest: the upper words of |y| first, then the lower words of those that have it
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        uint32_t hi = 0, lo = 0;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) hi = max(hi, (uint32_t)__double2hiint(out.y[i][b][k]) & 0x7fffffffu);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (((uint32_t)__double2hiint(out.y[i][b][k]) & 0x7fffffffu) == hi)
+                    lo = max(lo, (uint32_t)__double2loint(out.y[i][b][k]));
+        lo = __reduce_max_sync(0xffffffffu, lo);
+        if (lane == i || i == 0) out.top = __hiloint2double((int)hi, (int)lo);
+    }
+}
+
+// rne(RN64(y m)) of four elements, as the bytes of a word; CLAMP: held within +-127.
+template <bool CLAMP>
+__device__ __forceinline__ uint32_t codes4(const double (&y)[4], double m) {
+    int c[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const double v = __dmul_rn(y[k], m);
+        // beyond 2^31 to_int does not hold
+        c[k] = CLAMP ? to_int(fmin(fmax(v, -127.0), 127.0)) : to_int(v);
+    }
+    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
 // ── writing ──
-// One block per row of the batch, one warp per (key or value, KV head) row of head_dim codes in turn. Bound by memory:
-// 4 bytes read and 1 written per element.
+// A warp per (token, keys or values, up to four KV heads). Bound by memory at large sizes: 4 bytes read and 1 written
+// per element.
 struct AppendArgs {
     Cache c;
     Batch b;
@@ -175,71 +306,48 @@ struct AppendArgs {
     int vec;  // rows are 16-byte aligned: 16-byte loads
 };
 
-constexpr int APPEND_WARPS = 8;
+constexpr int ROW_WARPS = 4;
 
-__device__ __forceinline__ void stage_row(int32_t* dst, const int32_t* __restrict__ src, int dim, int vec) {
-    const int lane = threadIdx.x & 31;
-    if (vec) {
-        for (int e = 4 * lane; e < dim; e += 128) *(int4*)(dst + e) = __ldg((const int4*)(src + e));
-    } else {
-        for (int e = lane; e < dim; e += 32) dst[e] = src[e];
-    }
-    __syncwarp();
-}
-
-__global__ void __launch_bounds__(32 * APPEND_WARPS) append_kernel(const AppendArgs a) {
+template <int NB>
+__global__ void __launch_bounds__(32 * ROW_WARPS) append_kernel(const AppendArgs a, int chunks) {
     kt::pdl_enter();
-    __shared__ __align__(16) int32_t stage[APPEND_WARPS][MAX_DIM];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int t = blockIdx.x;
+    constexpr int B = RowBatch<NB>::B;
+    const int lane = threadIdx.x & 31, dim = a.c.dim;
+    const long long u = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    const int t = (int)(u / (2 * chunks)), c = (int)(u % (2 * chunks));
+    if (t >= a.b.rows) return;
+    const bool is_v = c >= chunks;
+    const int h0 = (is_v ? c - chunks : c) * B, heads = min(B, a.c.heads - h0);
+    const int32_t* x = (is_v ? a.v + (long long)t * a.ld_v : a.k + (long long)t * a.ld_k) + (long long)h0 * dim;
+    Rope rope = a.rope;
+    if (is_v) rope.table = nullptr;
+    const RawBatch<NB> raw = fetch_rows<NB>(x, heads, dim, a.vec, rope);
     Place p;
     if (!locate(a.b, a.err, t, a.c.page_shift, p) || p.pos < 0) return;
-    const long long page = pool_page(a.b, a.c, a.err, p.seq, p.pos >> a.c.page_shift);
-    const int in_page = p.pos & ((1 << a.c.page_shift) - 1);
     const longlong2 sc = a.scale[(long long)t * a.scale_stride];
-    const int2* cs = rope_row(a.rope, a.err, p.pos);
-    const int dim = a.c.dim;
-    for (int r = warp; r < 2 * a.c.heads; r += APPEND_WARPS) {
-        const bool is_v = r >= a.c.heads;
-        const int h = is_v ? r - a.c.heads : r;
-        const int32_t* src = (is_v ? a.v + (long long)t * a.ld_v : a.k + (long long)t * a.ld_k) + (long long)h * dim;
-        stage_row(stage[warp], src, dim, a.vec);
-        const int2* rot = is_v ? nullptr : cs;
-        int64_t y[8];
-        uint64_t top = 0;
+    const long long page = pool_page(a.b, a.c, a.err, p.seq, p.pos >> a.c.page_shift);
+    const int2* cs = rope_row(rope, a.err, p.pos);
+    RowBatch<NB> rows;
+    turn_rows<NB>(rows, raw, x, heads, dim, rope, cs);
+    const double s = scale_value(sc, cs ? 30 : 0);
+    const uint32_t sg = sigma_bits(__ddiv_rn(__dmul_rn(rows.top, s), 127.0));
+    const double m = __ddiv_rn(s, (double)bf16_value(sg));
+    const long long row0 = ((page * a.c.heads + h0) << a.c.page_shift) + (p.pos & ((1 << a.c.page_shift) - 1));
+    if (lane < heads) (is_v ? a.c.vs : a.c.ks)[row0 + ((long long)lane << a.c.page_shift)] = (uint16_t)sg;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int e = 4 * lane + 128 * i;
+    for (int i = 0; i < B; ++i) {
+        const double mi = __shfl_sync(0xffffffffu, m, i);
+        int8_t* dst = (is_v ? a.c.v : a.c.k) + (row0 + ((long long)i << a.c.page_shift)) * dim;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                y[4 * i + q] = e < dim ? rotated(stage[warp], e + q, a.rope, rot) : 0;
-                top = max(top, uabs(y[4 * i + q]));
-            }
-        }
-        top = warp_umax(top);
-        const double s = scale_value(sc, rot ? 30 : 0);
-        const uint32_t sg = sigma_bits(__ddiv_rn(__dmul_rn((double)(int64_t)top, s), 127.0));
-        const double m = __ddiv_rn(s, (double)bf16_value(sg));
-        const long long row = ((page * a.c.heads + h) << a.c.page_shift) + in_page;
-        int8_t* dst = (is_v ? a.c.v : a.c.k) + row * dim;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int e = 4 * lane + 128 * i;
-            if (e < dim) {
-                char4 o;
-                o.x = (signed char)code8(y[4 * i], m);
-                o.y = (signed char)code8(y[4 * i + 1], m);
-                o.z = (signed char)code8(y[4 * i + 2], m);
-                o.w = (signed char)code8(y[4 * i + 3], m);
-                *(char4*)(dst + e) = o;
-            }
-        }
-        if (lane == 0) (is_v ? a.c.vs : a.c.ks)[row] = (uint16_t)sg;
-        __syncwarp();
+        for (int b = 0; b < NB; ++b)
+            if (i < heads && 4 * lane + 128 * b < dim)
+                *(uint32_t*)(dst + 4 * lane + 128 * b) = codes4<true>(rows.y[i][b], mi);
     }
 }
 
 // ── reading back ──
+constexpr int READ_WARPS = 8;
+
 struct ReadArgs {
     Cache c;
     Batch b;
@@ -249,7 +357,7 @@ struct ReadArgs {
     int vec;
 };
 
-__global__ void __launch_bounds__(32 * APPEND_WARPS) read_kernel(const ReadArgs a) {
+__global__ void __launch_bounds__(32 * READ_WARPS) read_kernel(const ReadArgs a) {
     kt::pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t = blockIdx.x;
@@ -258,7 +366,7 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS) read_kernel(const ReadArgs 
     const long long page = pool_page(a.b, a.c, a.err, p.seq, p.pos >> a.c.page_shift);
     const int in_page = p.pos & ((1 << a.c.page_shift) - 1);
     const int dim = a.c.dim;
-    for (int r = warp; r < 2 * a.c.heads; r += APPEND_WARPS) {
+    for (int r = warp; r < 2 * a.c.heads; r += READ_WARPS) {
         const bool is_v = r >= a.c.heads;
         const int h = is_v ? r - a.c.heads : r;
         const long long row = ((page * a.c.heads + h) << a.c.page_shift) + in_page;
@@ -324,158 +432,41 @@ __device__ __forceinline__ float weight(float x, float top, float theta) {
 __device__ __forceinline__ int scale_exp(uint32_t sigma) { return (int)(sigma >> 7) - 127 + ((sigma & 127) != 0); }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// A query row's codes and theta, by a whole warp. stage: head_dim int32 of shared memory. dst: the row's int8 codes; with
-// SW128, row r of a K-major operand in 128-byte blocks of 16384 bytes with the 128-byte swizzle.
-template <bool SW128>
-__device__ __forceinline__ float quantise_query(int8_t* dst, int32_t* stage, const int32_t* src, int dim, int vec,
-                                                const Rope& rope, const int2* cs, double s, double soft, int r = 0) {
-    const int lane = threadIdx.x & 31;
-    stage_row(stage, src, dim, vec);
-    int64_t y[8];
-    uint64_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int e = 4 * lane + 128 * i;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            y[4 * i + q] = e < dim ? rotated(stage, e + q, rope, cs) : 0;
-            top = max(top, uabs(y[4 * i + q]));
-        }
-    }
-    top = warp_umax(top);
-    const double td = (double)(int64_t)top;
-    const double m = __ddiv_rn(127.0, fmax(td, 1.0));
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int e = 4 * lane + 128 * i;
-        if (e < dim) {
-            char4 o;
-            o.x = (signed char)code8(y[4 * i], m);
-            o.y = (signed char)code8(y[4 * i + 1], m);
-            o.z = (signed char)code8(y[4 * i + 2], m);
-            o.w = (signed char)code8(y[4 * i + 3], m);
-            *(char4*)(dst + (SW128 ? i * 16384 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3) : e)) = o;
-        }
-    }
-    __syncwarp();
-    if (top == 0) return 0.0f;
-    return __double2float_rn(fmin(__dmul_rn(__ddiv_rn(__dmul_rn(td, s), 127.0), soft), 0x1p60));
+// theta of a row from its largest element, its scale and softmax_scale * log2(e).
+__device__ __forceinline__ float row_theta(double top, double s, double soft) {
+    return top > 0.0 ? __double2float_rn(fmin(__dmul_rn(__ddiv_rn(__dmul_rn(top, s), 127.0), soft), 0x1p60)) : 0.0f;
 }
 
-// RN64 of a 64-bit integer and the nearest whole number to a double (ties to even, |v| < 2^31) on the FP64 pipe: the
-// conversion instructions run at a quarter of its rate. 2^52 + 2^31 + hi and 2^52 + lo are doubles whose low words are
-// the integer's halves.
-__device__ __forceinline__ double to_double(int64_t v) {
-    const double hi = __dsub_rn(__hiloint2double(0x43300000, (int)(v >> 32) ^ (int)0x80000000), 4503601774854144.0);
-    const double lo = __dsub_rn(__hiloint2double(0x43300000, (int)v), 4503599627370496.0);
-    return __fma_rn(hi, 4294967296.0, lo);
-}
-__device__ __forceinline__ double to_double(int32_t v) {
-    return __dsub_rn(__hiloint2double(0x43300000, v ^ (int)0x80000000), 4503601774854144.0);
-}
-__device__ __forceinline__ int to_int(double v) { return __double2loint(__dadd_rn(v, 6755399441055744.0)); }
-
-// Where a query row stands: its position, its row of the caller's buffers and its query head. pos < 0: no row.
-struct QueryRow {
-    int pos;
-    long long row;
-    int head;
-};
-
-// Four elements e .. e + 3 of a query row after the rotation. x: the row; cs: its row of the rotation table.
-__device__ __forceinline__ void rotated4(int64_t (&y)[4], const AttendArgs& a, const int32_t* x, const int2* cs, int e) {
-    int4 v;
-    if (a.vec) {
-        v = __ldg((const int4*)(x + e));
-    } else {
-        v = make_int4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-    }
-    const int half = a.rope.half;
-    if (!a.rope.table) {
-        y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
-    } else if (e >= 2 * half) {
-        y[0] = (int64_t)v.x << 30, y[1] = (int64_t)v.y << 30, y[2] = (int64_t)v.z << 30, y[3] = (int64_t)v.w << 30;
-    } else if (a.rope.interleaved && e + 4 <= 2 * half) {
-        const int2 c0 = __ldg(cs + e / 2), c1 = __ldg(cs + e / 2 + 1);
-        y[0] = (int64_t)v.x * c0.x - (int64_t)v.y * c0.y;
-        y[1] = (int64_t)v.y * c0.x + (int64_t)v.x * c0.y;
-        y[2] = (int64_t)v.z * c1.x - (int64_t)v.w * c1.y;
-        y[3] = (int64_t)v.w * c1.x + (int64_t)v.z * c1.y;
-    } else if (!a.rope.interleaved && half % 4 == 0 && a.vec) {
-        const bool first = e < half;
-        const int4 o = __ldg((const int4*)(x + (first ? e + half : e - half)));
-        const int2* c = cs + (first ? e : e - half);
-        const int2 c0 = __ldg(c), c1 = __ldg(c + 1), c2 = __ldg(c + 2), c3 = __ldg(c + 3);
-        const int sg = first ? -1 : 1;
-        y[0] = (int64_t)v.x * c0.x + (int64_t)o.x * (sg * c0.y);
-        y[1] = (int64_t)v.y * c1.x + (int64_t)o.y * (sg * c1.y);
-        y[2] = (int64_t)v.z * c2.x + (int64_t)o.z * (sg * c2.y);
-        y[3] = (int64_t)v.w * c3.x + (int64_t)o.w * (sg * c3.y);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) y[k] = rotated(x, e + k, a.rope, cs);
-    }
-}
-
-// N query rows by one warp: codes of row r, r0 <= r < r0 + N, into row r of a K-major operand in 128-byte blocks with the
-// 128-byte swizzle (16384 bytes a block), theta into theta[r]. NB: blocks of a row. The rows are rotated twice, for
-// their largest element and for their codes (from L1 then), so that one division serves all rows and the loads of
-// many rows overlap: what this costs is latency, not work.
-template <int N, int NB, class RowOf>
-__device__ __forceinline__ void quantise_rows(const AttendArgs& a, RowOf row_of, int r0, int8_t* dst, float* theta) {
+// Quantised queries wait for the tile kernel where its output will be: the head_dim int32 words of a row and head first
+// hold the head_dim codes, then theta; whoever reads them writes the output over them. No other memory is needed. Bound
+// by memory at large sizes: 4 bytes read and 1 written per element.
+template <int NB>
+__global__ void __launch_bounds__(32 * ROW_WARPS) query_kernel(const AttendArgs a, int chunks) {
+    kt::pdl_enter();
+    constexpr int B = RowBatch<NB>::B;
     const int lane = threadIdx.x & 31, dim = a.c.dim;
-    uint64_t mine = 0;  // lane i: the largest element of row r0 + i
-#pragma unroll 4
-    for (int i = 0; i < N; ++i) {
-        const QueryRow at = row_of(r0 + i);
-        uint64_t top = 0;
-        if (at.pos >= 0) {
-            const int32_t* x = a.q + at.row * a.ld_q + (long long)at.head * dim;
-            const int2* cs = rope_row(a.rope, a.err, at.pos);
+    const long long u = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    const int t = (int)(u / chunks), h0 = (int)(u % chunks) * B, heads = min(B, a.c.heads * a.group - h0);
+    if (t >= a.b.rows) return;
+    const int32_t* x = a.q + (long long)t * a.ld_q + (long long)h0 * dim;
+    const RawBatch<NB> raw = fetch_rows<NB>(x, heads, dim, a.vec, a.rope);
+    Place p;
+    if (!locate(a.b, a.err, t, a.c.page_shift, p) || p.pos < 0) return;
+    const longlong2 sc = a.scale[(long long)t * a.scale_stride];
+    const int2* cs = rope_row(a.rope, a.err, p.pos);
+    RowBatch<NB> rows;
+    turn_rows<NB>(rows, raw, x, heads, dim, a.rope, cs);
+    const double m = __ddiv_rn(127.0, fmax(rows.top, 1.0));
+    int32_t* out = a.o + (long long)t * a.ld_o + (long long)h0 * dim;
+    const float theta = row_theta(rows.top, scale_value(sc, cs ? 30 : 0), a.soft);
+    __syncwarp();  // o may be q: every lane has read its elements
+    if (lane < heads) out[lane * dim + dim / 4] = __float_as_int(theta);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const int e = 4 * lane + 128 * b;
-                if (e >= dim) continue;
-                int64_t y[4];
-                rotated4(y, a, x, cs, e);
-                top = max(max(top, max(uabs(y[0]), uabs(y[1]))), max(uabs(y[2]), uabs(y[3])));
-            }
-        }
-        top = warp_umax(top);
-        if (lane == i) mine = top;
-    }
-    const double td = to_double((int64_t)mine);
-    const double m = __ddiv_rn(127.0, fmax(td, 1.0));
-    if (lane < N) {
-        const QueryRow me = row_of(r0 + lane);
-        if (me.pos >= 0) {
-            const double s = scale_value(a.scale[me.row * a.scale_stride], a.rope.table ? 30 : 0);
-            theta[r0 + lane] =
-                mine ? __double2float_rn(fmin(__dmul_rn(__ddiv_rn(__dmul_rn(td, s), 127.0), a.soft), 0x1p60)) : 0.0f;
-        }
-    }
-#pragma unroll 4
-    for (int i = 0; i < N; ++i) {
-        const QueryRow at = row_of(r0 + i);
+    for (int i = 0; i < B; ++i) {
         const double mi = __shfl_sync(0xffffffffu, m, i);
-        if (at.pos < 0) continue;
-        const int32_t* x = a.q + at.row * a.ld_q + (long long)at.head * dim;
-        const int2* cs = rope_row(a.rope, a.err, at.pos);
-        const int r = r0 + i;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int e = 4 * lane + 128 * b;
-            if (e >= dim) continue;
-            int64_t y[4];
-            rotated4(y, a, x, cs, e);
-            // |y m| <= 127 (1 + 2^-52): the codes stay within +-127
-            char4 o;
-            o.x = (signed char)to_int(__dmul_rn(to_double(y[0]), mi));
-            o.y = (signed char)to_int(__dmul_rn(to_double(y[1]), mi));
-            o.z = (signed char)to_int(__dmul_rn(to_double(y[2]), mi));
-            o.w = (signed char)to_int(__dmul_rn(to_double(y[3]), mi));
-            *(char4*)(dst + b * 16384 + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + 4 * (lane & 3)) = o;
-        }
+        for (int b = 0; b < NB; ++b)  // |y m| <= 127 (1 + 2^-52): the codes stay within +-127
+            if (i < heads && 4 * lane + 128 * b < dim) out[i * dim + lane + 32 * b] = (int)codes4<false>(rows.y[i][b], mi);
     }
 }
 
