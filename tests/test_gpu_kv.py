@@ -288,6 +288,15 @@ def test_attention_beyond_131072_keys(ctx):
     s2.check(s2.codes(16), s2.scales())
 
 
+def test_attention_of_millions_of_keys(ctx):
+    """So many keys that each block of a decode cluster takes its 32-bit sums out on the way."""
+    n = 2300000
+    s = Setup(ctx, [(1, n)], 1, 1, 16, 128)
+    s.pool["k"][:], s.pool["v"][:], s.pool["ks"][:], s.pool["vs"][:] = 1, 127, 1.0, 255 / 256
+    s.push()
+    s.check(s.codes(16), s.scales())
+
+
 def test_attention_takes_strided_and_unaligned_queries(ctx):
     torch = _torch()
     s = Setup(ctx, [(5, 90), (30, 200)], 4, 2, 48, 16)

@@ -20,7 +20,7 @@ LIB = os.path.join(PKG, "libktmoe.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES_CU = ["ktmoe.cu", "kv_cache.cu", "noalloc.cu"]
 SOURCES_CPP = ["host_prep.cpp", "wire.cpp"]
-KV_HEADERS = ["kv_kernels.cuh", "kv_attend_simple.cuh", "kv_attend_tile.cuh"]  # of kv_cache.cu alone
+KV_HEADERS = ["kv_kernels.cuh", "kv_attend_few.cuh", "kv_attend_tile.cuh"]  # of kv_cache.cu alone
 HEADERS = ["context.cuh", "fixed_point.cuh", "digit_gemm.cuh", "digit_gemm_pair.cuh", "moe_kernels.cuh", "ep_peer.cuh", "synth.cuh",
            "host_prep.h"]
 

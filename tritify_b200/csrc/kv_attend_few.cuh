@@ -1,0 +1,636 @@
+// Attention over the paged cache for few query rows of a sequence (decode, short chunks): a cluster of blocks takes up to
+// 16 rows (token, query head) of one sequence and KV head, and each block an even share of the keys they see. Bound by
+// memory: every key and value byte once; everything else has to pass under that stream.
+//
+// Operands are swapped against the tile kernel, so that few rows still fill the tensor cores and K and V go from their
+// pages to the products by TMA alone: S^T = K Q^T (128 keys by 16 rows) and O^T = V^T P^T (128 columns by 16 rows, both
+// digits of the weights in one product of 32 columns). A thread has one key of a tile.
+//
+// The row maxima must be known before the first weight is rounded, so there are two phases; K is read once all the same,
+// because the scores wait in TMEM: 16 columns a tile, 28 tiles a block (26 of rows longer than 128). Only tiles beyond
+// that are formed again. While the cluster exchanges its maxima, V is already on its way. Sums over the keys are
+// integers, so the shares of a cluster add up to the same bits in any order.
+//
+// Roles (224 threads): warps 0-3 softmax, warp 4 TMA, warp 5 the products, warp 6 the keys' scales.
+#pragma once
+
+#include "kv_attend_tile.cuh"
+
+namespace kv {
+
+constexpr int FEW_ROWS = 16;
+constexpr int FEW_THREADS = 224;
+
+template <int NK>
+struct FewCfg {
+    static constexpr int SLOT = TILE_KEYS * 128;
+    static constexpr int SLOTS = 8;
+    static constexpr int SCALES = 4;
+    static constexpr int KEEP = NK == 1 ? 28 : 26;  // tiles whose scores stay in TMEM
+    static constexpr int AGAIN = 16 * KEEP;         // two more score buffers, for the others
+    static constexpr int SUMS = 512 - 32 * NK;      // O^T of each 128 columns: 16 hi, 16 lo
+    static constexpr int RING = 0;
+    static constexpr int Q = RING + SLOTS * SLOT;               // [NK][16 rows][128]
+    static constexpr int P = Q + NK * 16 * 128;                 // [2][16 hi, 16 lo][128 keys]
+    static constexpr int RED = P + 2 * 32 * 128;                // int64 [16 rows][NK * 128]
+    static constexpr int KEY_SCALES = RED + 16 * NK * 128 * 8;  // [SCALES][sigma_k, sigma_v][128]
+    static constexpr int ROWS = KEY_SCALES + SCALES * 2 * TILE_KEYS * 4;
+    // per row: theta; position; max and largest sigma of each warp and of each block of the cluster; total of the block and
+    // of each warp; the row's (max, -theta, 2^-E, 2^E); 2^21 / L
+    static constexpr int BARS = ROWS + FEW_ROWS * (4 + 4 + 32 + 128 + 8 + 32 + 16 + 8);
+    static constexpr int BYTES = 1024 + BARS + 512;
+    static_assert(AGAIN + 32 <= SUMS, "TMEM columns");
+    static_assert(BYTES <= 232448, "shared memory per block");
+};
+
+__device__ __forceinline__ uint32_t cluster_ctarank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_nctarank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+// Every thread of every block of the cluster meets; what was written to shared memory before the arrival is seen after
+// the wait.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t peer_addr(const void* local, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(local)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void peer_store(uint32_t a, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+// One arrival at a barrier of another block of the cluster; what this thread wrote before is seen after the wait.
+__device__ __forceinline__ void peer_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// wait() for arrivals from other blocks.
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* err, int code) {
+    const uint64_t t0 = dg::globaltimer();
+    for (uint32_t it = 1;; ++it) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if ((it & 255u) == 0) {
+            const int e = *(volatile int*)err;
+            if (e > 0 && e < 100) return false;
+            if (dg::globaltimer() - t0 > 2000000000ull) {
+                atomicCAS(err, 0, code);
+                return false;
+            }
+        }
+    }
+}
+__device__ __forceinline__ uint64_t peer_u64(uint32_t a) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+    return v;
+}
+
+template <int NK>
+__global__ void __launch_bounds__(FEW_THREADS, 1)
+    attend_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                      const AttendArgs a) {
+    kt::pdl_enter();
+    using C = FewCfg<NK>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float4* s_row = (float4*)(sm + C::ROWS);                  // max, -theta, 2^-E, 2^E
+    unsigned long long* s_total4 = (unsigned long long*)(s_row + FEW_ROWS);  // [4][16]
+    unsigned long long* s_total = s_total4 + 4 * FEW_ROWS;
+    double* s_inv = (double*)(s_total + FEW_ROWS);
+    float* s_top4 = (float*)(s_inv + FEW_ROWS);               // [4][16]
+    uint32_t* s_sig4 = (uint32_t*)(s_top4 + 4 * FEW_ROWS);    // [4][16]
+    uint32_t* s_top = s_sig4 + 4 * FEW_ROWS;                  // [16 ranks][16], written by the ranks
+    uint32_t* s_sig = s_top + 16 * FEW_ROWS;                  // [16 ranks][16]
+    float* s_theta = (float*)(s_sig + 16 * FEW_ROWS);
+    int* s_pos = (int*)(s_theta + FEW_ROWS);
+    uint64_t* full = (uint64_t*)(sm + C::BARS);  // [SLOTS]
+    uint64_t* empty = full + C::SLOTS;           // [SLOTS]
+    uint64_t* s_full = empty + C::SLOTS;         // [4] scores that stay
+    uint64_t* s_free = s_full + 4;               // [4]
+    uint64_t* r_full = s_free + 4;               // [2] scores formed twice
+    uint64_t* r_free = r_full + 2;               // [2]
+    uint64_t* p_full = r_free + 2;               // [2]
+    uint64_t* p_free = p_full + 2;               // [2]
+    uint64_t* k_full = p_free + 2;               // [SCALES]
+    uint64_t* k_free = k_full + C::SCALES;       // [SCALES]
+    uint64_t* q_full = k_free + C::SCALES;
+    uint64_t* o_full = q_full + 1;
+    uint64_t* o_free = o_full + 1;
+    uint64_t* x_full = o_free + 1;  // every block's maxima have arrived
+    uint64_t* done = x_full + 1;
+    uint32_t* tmem_slot = (uint32_t*)(done + 1);
+    int* s_job = (int*)(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = a.group, dim = a.c.dim;
+    const uint32_t rank = cluster_ctarank(), ranks = cluster_nctarank();
+    const unsigned job = blockIdx.x / ranks;
+    const int head = (int)(job % (unsigned)a.c.heads);
+    const long long slot = job / (unsigned)a.c.heads;
+    // Sequence b's groups of 16 rows stand at slots begin_b g / 16 + b and on; slots without rows leave, whole clusters.
+    if (warp == 0) {
+        auto first_slot = [&](int b) { return (long long)a.b.begin[b] * g / FEW_ROWS + b; };
+        const int b = warp_search(a.b.n_seqs, slot, first_slot);
+        const int begin = a.b.begin[b], end = a.b.begin[b + 1], len = a.b.kv_len[b];
+        const long long row0 = (slot - first_slot(b)) * FEW_ROWS;
+        bool live = row0 >= 0 && row0 < (long long)(end - begin) * g;
+        if (begin < 0 || begin > end || end > a.b.begin[a.b.n_seqs] || end > a.b.rows || len < 0 ||
+            ((len + (1 << a.c.page_shift) - 1) >> a.c.page_shift) > a.b.max_pages) {
+            if (lane == 0) a.err.raise(a.err.bad_length);
+            live = false;
+        }
+        if (lane == 0) {
+            s_job[0] = live ? b : -1;
+            s_job[1] = begin;
+            s_job[2] = end - begin;
+            s_job[3] = len;
+            s_job[4] = (int)row0;
+        }
+    }
+    if (threadIdx.x == 32) {
+        for (int i = 0; i < C::SLOTS; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&s_free[i], 4);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&r_full[i], 1);
+            mbar_init(&r_free[i], 4);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&p_free[i], 1);
+        }
+        for (int i = 0; i < C::SCALES; ++i) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_free[i], 4);
+        }
+        mbar_init(q_full, 4);
+        mbar_init(o_full, 1);
+        mbar_init(o_free, 4);
+        mbar_init(x_full, FEW_ROWS * ranks);
+        mbar_init(done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    const int seq = s_job[0];
+    if (seq < 0) return;
+    const int begin = s_job[1], n_new = s_job[2], len = s_job[3], row0 = s_job[4];
+    const int n_rows = min(FEW_ROWS, n_new * g - row0);
+    const int p0 = len - n_new + row0 / g, p1 = len - n_new + (row0 + n_rows - 1) / g;
+    const KeyTiles all_tiles(p0, p1, a.window, a.sinks);
+    // this block's share of the tiles
+    const int i_first = (int)((long long)all_tiles.n * rank / ranks), i_last = (int)((long long)all_tiles.n * (rank + 1) / ranks);
+    const int n = i_last - i_first, n_again = max(0, n - C::KEEP);
+    auto tile_at = [&](int i) { return all_tiles.at(i_first + i); };
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.fence::before_thread_sync;");
+    }
+    // the blocks of the cluster are there and their barriers stand
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    const uint32_t tmem = *tmem_slot;
+    const int ps = 1 << a.c.page_shift;
+    const int* pages = a.b.pages + (long long)seq * a.b.max_pages;
+    int* err = a.err.word;
+    const bool soft = warp < 4;
+
+    if (warp == 4) {
+        // K of every tile; then V of tile after tile, and K of tile i + 1 ahead of V of tile i where its scores did not
+        // stay. A lane holds one page of a tile; page numbers are read two tiles ahead.
+        const int per_tile = TILE_KEYS >> a.c.page_shift, last_page = p1 >> a.c.page_shift;
+        uint32_t q = 0;
+        int s = 0;
+        uint32_t phase = 1;
+        bool alive = true;
+        auto page_of = [&](int i) -> int {
+            const int at = tile_at(min(i, n - 1)) * per_tile + lane;
+            return lane < per_tile && at <= last_page ? __ldg(pages + at) : 0;
+        };
+        auto load = [&](const CUtensorMap* map, int i, int page) {
+            const int np = min(per_tile, last_page - tile_at(i) * per_tile + 1);
+            if ((unsigned)page >= (unsigned long long)a.c.n_pages) {
+                a.err.raise(a.err.bad_page);
+                page = 0;
+            }
+#pragma unroll
+            for (int x = 0; x < NK; ++x) {
+                bool ok = alive;
+                if (ok && lane == 0) {
+                    ok = wait(&empty[s], phase, err, dg::ERR_TIMEOUT_EMPTY);
+                    if (ok) mbar_arrive_expect_tx(&full[s], (uint32_t)(np * ps * 128));
+                }
+                alive = __shfl_sync(0xffffffffu, (int)ok, 0);
+                if (!alive) return;
+                if (lane < np)
+                    tma_load_4d(smem_u32(sm + C::RING + s * C::SLOT + lane * ps * 128), map, x * 128, 0, head, page, &full[s]);
+                ++q;
+                if (++s == C::SLOTS) s = 0, phase ^= 1;
+            }
+        };
+        for (int ph = 0; alive && n > 0 && ph < 2; ++ph) {
+            int pa = page_of(0), pb = page_of(1);
+            for (int i = 0; alive && i < n; ++i) {
+                const int pc = page_of(i + 2);
+                if (ph == 0) {
+                    load(&map_k, i, pa);
+                } else {
+                    if (i + 1 >= C::KEEP && i + 1 < n) load(&map_k, i + 1, pb);
+                    if (alive) load(&map_v, i, pa);
+                }
+                pa = pb;
+                pb = pc;
+            }
+        }
+        if (lane == 0)  // copies still in flight land before the block leaves
+            for (uint32_t j = q > (uint32_t)C::SLOTS ? q - C::SLOTS : 0; j < q; ++j)
+                dg::mbar_wait_drain(&full[j % C::SLOTS], (j / C::SLOTS) & 1u, err, dg::ERR_TIMEOUT_FULL);
+        __syncwarp();
+    } else if (warp == 5) {
+        if (lane == 0 && n > 0) {
+            const int ksteps = (dim + 31) / 32;
+            const uint32_t id_s = idesc_i8(FEW_ROWS, 0), id_o = idesc_i8(2 * FEW_ROWS, 1u << 15);
+            const uint32_t qd = desc_k(smem_u32(sm + C::Q)), kd = desc_k(smem_u32(sm + C::RING)),
+                           pd = desc_k(smem_u32(sm + C::P)), vd = desc_mn(smem_u32(sm + C::RING));
+            int s = 0;
+            uint32_t phase = 0, again = 0, oc = 0;
+            bool ok = wait(q_full, 0, err, dg::ERR_TIMEOUT_FULL);
+            auto next = [&]() {
+                if (++s == C::SLOTS) s = 0, phase ^= 1;
+            };
+            auto scores = [&](int i, bool stays) {
+                const uint32_t b = stays ? i & 3 : again & 1, use = stays ? i >> 2 : again >> 1;
+                ok = ok && wait(stays ? &s_free[b] : &r_free[b], (use & 1u) ^ 1u, err, dg::ERR_TIMEOUT_ACCUM);
+                const uint32_t d = tmem + (stays ? 16 * i : C::AGAIN + 16 * b);
+#pragma unroll
+                for (int x = 0; x < NK; ++x) {
+                    ok = ok && wait(&full[s], phase, err, dg::ERR_TIMEOUT_FULL);
+                    if (!ok) return;
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                    const uint32_t kx = kd + s * (C::SLOT >> 4), qx = qd + x * (16 * 128 >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        if (4 * x + kk < ksteps) umma(d, kx + 2 * kk, qx + 2 * kk, id_s, x + kk > 0);
+                    umma_commit(&empty[s]);
+                    next();
+                }
+                umma_commit(stays ? &s_full[b] : &r_full[b]);
+                if (!stays) ++again;
+            };
+            for (int i = 0; ok && i < n; ++i) scores(i, i < C::KEEP);
+            for (int i = 0; ok && i < n; ++i) {
+                if (i + 1 >= C::KEEP && i + 1 < n) scores(i + 1, false);
+                ok = ok && wait(&p_full[i & 1], (i >> 1) & 1u, err, dg::ERR_TIMEOUT_ACCUM);
+#pragma unroll
+                for (int x = 0; x < NK; ++x) {
+                    ok = ok && wait(&full[s], phase, err, dg::ERR_TIMEOUT_FULL);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;");
+                    const uint32_t vx = vd + s * (C::SLOT >> 4), px = pd + (i & 1) * (32 * 128 >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        umma(tmem + C::SUMS + 32 * x, vx + kk * (32 * 128 >> 4), px + 2 * kk, id_o, i % FLUSH_TILES + kk > 0);
+                    umma_commit(&empty[s]);
+                    next();
+                }
+                if (!ok) break;
+                umma_commit(&p_free[i & 1]);
+                if (i + 1 == n || (i + 1) % FLUSH_TILES == 0) {
+                    umma_commit(o_full);
+                    if (i + 1 < n) {  // the sums are taken out and begin anew
+                        ok = wait(o_free, oc & 1u, err, dg::ERR_TIMEOUT_ACCUM);
+                        asm volatile("tcgen05.fence::after_thread_sync;");
+                    }
+                    ++oc;
+                }
+            }
+            umma_commit(done);
+            dg::mbar_wait_drain(done, 0u, err, dg::ERR_TIMEOUT_ACCUM);
+        }
+        __syncwarp();
+    } else if (warp == 6) {
+        // The scales of each tile's keys, four keys a lane, for both phases: read four tiles ahead, their pages eight.
+        const int total = 2 * n;
+        auto key_of = [&](int u) { return tile_at(u >= n ? u - n : u) * TILE_KEYS + 4 * lane; };
+        auto page_of = [&](int u) -> int {
+            const int j = u < total ? key_of(u) : p1 + 1;
+            return j <= p1 ? __ldg(pages + (j >> a.c.page_shift)) : 0;
+        };
+        auto scales_of = [&](int u, int page) -> uint4 {  // four bfloat16 of K, four of V
+            uint4 r = {0, 0, 0, 0};
+            const int j = u < total ? key_of(u) : p1 + 1;
+            if (j <= p1) {
+                if ((unsigned)page >= (unsigned long long)a.c.n_pages) {
+                    a.err.raise(a.err.bad_page);
+                    page = 0;
+                }
+                const long long row = (((long long)page * a.c.heads + head) << a.c.page_shift) + (j & (ps - 1));
+                const uint2 k = __ldg((const uint2*)(a.c.ks + row)), v = __ldg((const uint2*)(a.c.vs + row));
+                r = make_uint4(k.x, k.y, v.x, v.y);
+            }
+            return r;
+        };
+        if (total > 0) {
+            int pg[4];
+            uint4 val[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pg[j] = page_of(j);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                val[j] = scales_of(j, pg[j]);
+                pg[j] = page_of(j + 4);
+            }
+            bool alive = true;
+            for (int u0 = 0; alive && u0 < total; u0 += 4) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {  // stage j: C::SCALES is 4
+                    const int u = u0 + j;
+                    if (u >= total || !alive) break;
+                    alive = wait(&k_free[j], ((u >> 2) & 1u) ^ 1u, err, dg::ERR_TIMEOUT_EMPTY);
+                    alive = __all_sync(0xffffffffu, alive);
+                    if (!alive) break;
+                    uint32_t* f = (uint32_t*)(sm + C::KEY_SCALES) + j * 2 * TILE_KEYS;
+                    const uint4 w = val[j];
+                    const uint32_t hi16 = 0xffff0000u;
+                    *(uint4*)(f + 4 * lane) = make_uint4(w.x << 16, w.x & hi16, w.y << 16, w.y & hi16);
+                    *(uint4*)(f + TILE_KEYS + 4 * lane) = make_uint4(w.z << 16, w.z & hi16, w.w << 16, w.w & hi16);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&k_full[j]);
+                    val[j] = scales_of(u + 4, pg[j]);
+                    pg[j] = page_of(u + 8);
+                }
+            }
+        }
+        __syncwarp();
+    }
+
+    // ── the softmax warps; the others go on to where the cluster meets ──
+    const int key = 32 * (warp & 3) + lane;  // of a tile
+    const uint32_t lane_addr = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    bool ok = true;
+    uint32_t again = 0;
+    int32_t s16[16];
+    float kf = 0.0f;
+    uint32_t vf = 0;
+    // the scores of tile i and its keys' scales; `stays` tiles of phase 1 are in TMEM already
+    auto next_scores = [&](int i, int u) {
+        const bool stays = i < C::KEEP;
+        const uint32_t b = again & 1;
+        if (!stays) {
+            ok = wait(&r_full[b], (again >> 1) & 1u, err, dg::ERR_TIMEOUT_ACCUM);
+        } else if (u < n) {
+            ok = wait(&s_full[i & 3], (i >> 2) & 1u, err, dg::ERR_TIMEOUT_ACCUM);
+        }
+        ok = ok && wait(&k_full[u & 3], (u >> 2) & 1u, err, dg::ERR_TIMEOUT_FULL);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        dg::tmem_ld16(lane_addr + (stays ? 16 * i : C::AGAIN + 16 * b), s16);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;");
+        const uint32_t* f = (const uint32_t*)(sm + C::KEY_SCALES) + (u & 3) * 2 * TILE_KEYS;
+        kf = __uint_as_float(f[key]);
+        vf = f[TILE_KEYS + key];
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(&k_free[u & 3]);
+            if (!stays) {
+                mbar_arrive(&r_free[b]);
+            } else if (u < n) {
+                mbar_arrive(&s_free[i & 3]);
+            }
+        }
+        if (!stays) ++again;
+    };
+    // bit r: row r sees this thread's key of the tile
+    auto seen_rows = [&](int j0) -> uint32_t {
+        if (j0 + TILE_KEYS - 1 <= p0 && (!a.window || j0 > p1 - a.window || j0 + TILE_KEYS <= a.sinks)) return 0xffffu;
+        const int j = j0 + key;
+        uint32_t m = 0;
+        for (int r = 0; r < n_rows; ++r) {
+            const int pos = s_pos[r];
+            m |= (uint32_t)(j <= pos && (!a.window || j > pos - a.window || j < a.sinks)) << r;
+        }
+        return m;
+    };
+    const float kc_of = -MAGIC;
+    if (soft) {
+        // the queries, up to B rows of one token at a time
+        if (threadIdx.x < FEW_ROWS) s_pos[threadIdx.x] = threadIdx.x < n_rows ? len - n_new + (row0 + (int)threadIdx.x) / g : -1;
+        constexpr int B = RowBatch<NK>::B;
+#pragma unroll 1
+        for (int rb = B * warp; rb < n_rows; rb += 4 * B) {
+            int count = 0;
+#pragma unroll 1
+            for (int r = rb; r < min(rb + B, n_rows); r += count) {
+                const int t = (row0 + r) / g, hq = (row0 + r) % g, pos = len - n_new + t;
+                count = min(min(rb + B, n_rows) - r, g - hq);
+                if (pos < 0) continue;
+                const int32_t* x = a.q + ((long long)begin + t) * a.ld_q + (long long)(head * g + hq) * dim;
+                const RawBatch<NK> raw = fetch_rows<NK>(x, count, dim, a.vec, a.rope);
+                const longlong2 sc = a.scale[((long long)begin + t) * a.scale_stride];
+                const int2* cs = rope_row(a.rope, a.err, pos);
+                RowBatch<NK> rows;
+                turn_rows<NK>(rows, raw, x, count, dim, a.rope, cs);
+                const double m = __ddiv_rn(127.0, fmax(rows.top, 1.0));
+                if (lane < count) s_theta[r + lane] = row_theta(rows.top, scale_value(sc, cs ? 30 : 0), a.soft);
+#pragma unroll
+                for (int i = 0; i < B; ++i) {
+                    const double mi = __shfl_sync(0xffffffffu, m, i);
+                    const int ri = r + i;
+#pragma unroll
+                    for (int b = 0; b < NK; ++b)
+                        if (i < count && 4 * lane + 128 * b < dim)
+                            *(uint32_t*)(sm + C::Q + b * 2048 + ri * 128 + (((lane >> 2) ^ (ri & 7)) << 4) + 4 * (lane & 3)) =
+                                codes4<false>(rows.y[i][b], mi);
+                }
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // s_pos, s_theta
+        // ── phase 0: the maxima ──
+        float top[FEW_ROWS];
+        uint32_t sig[FEW_ROWS];
+#pragma unroll
+        for (int r = 0; r < FEW_ROWS; ++r) top[r] = -INFINITY, sig[r] = 0;
+        for (int i = 0; i < n; ++i) {
+            next_scores(i, i);
+            if (!ok) break;
+            const uint32_t m = seen_rows(tile_at(i) * TILE_KEYS);
+            const float kc = kc_of * kf;
+#pragma unroll
+            for (int r = 0; r < FEW_ROWS; ++r) {
+                if (r >= n_rows) break;
+                const float x = __fmaf_rn(__int_as_float(s16[r] + (int)MAGIC_BITS), kf, kc);
+                if (m >> r & 1) {
+                    top[r] = fmaxf(top[r], x);
+                    sig[r] = max(sig[r], vf);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < FEW_ROWS; ++r) {
+            float t = top[r];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            const uint32_t sg = __reduce_max_sync(0xffffffffu, sig[r]);
+            if (lane == 0) {
+                s_top4[warp * FEW_ROWS + r] = t;
+                s_sig4[warp * FEW_ROWS + r] = sg;
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (threadIdx.x < FEW_ROWS) {
+            float t = -INFINITY;
+            uint32_t sg = 0;
+            for (int w = 0; w < 4; ++w) {
+                t = fmaxf(t, s_top4[w * FEW_ROWS + threadIdx.x]);
+                sg = max(sg, s_sig4[w * FEW_ROWS + threadIdx.x]);
+            }
+            for (uint32_t c = 0; c < ranks; ++c) {  // to every block of the cluster
+                peer_store(peer_addr(s_top + rank * FEW_ROWS + threadIdx.x, c), __float_as_uint(t));
+                peer_store(peer_addr(s_sig + rank * FEW_ROWS + threadIdx.x, c), sg);
+                peer_arrive(peer_addr(x_full, c));
+            }
+        }
+        __syncwarp();
+    }
+    uint32_t row_sig = 0;  // threads 0 .. 15: of their row
+    if (soft) {
+        bool met = wait_cluster(x_full, 0, err, dg::ERR_TIMEOUT_ACCUM);
+        ok = __all_sync(0xffffffffu, met && ok);
+        if (threadIdx.x < FEW_ROWS) {
+            float t = -INFINITY;
+            for (uint32_t c = 0; c < ranks; ++c) {
+                t = fmaxf(t, __uint_as_float(s_top[c * FEW_ROWS + threadIdx.x]));
+                row_sig = max(row_sig, s_sig[c * FEW_ROWS + threadIdx.x]);
+            }
+            const int e = row_sig ? scale_exp(row_sig >> 16) : 0;
+            s_row[threadIdx.x] = make_float4(t, s_pos[threadIdx.x] >= 0 ? -s_theta[threadIdx.x] : 0.0f, pow2f(-e), pow2f(e));
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        // ── phase 1: the weights and the sums ──
+        uint32_t total[FEW_ROWS];  // at most 131072 tiles of one key a thread: below 2^32
+#pragma unroll
+        for (int r = 0; r < FEW_ROWS; ++r) total[r] = 0;
+        long long* red = (long long*)(sm + C::RED);
+        uint32_t oc = 0;
+        auto take_sums = [&]() {  // thread `key` has column 128 x + key of O
+            ok = ok && wait(o_full, oc & 1u, err, dg::ERR_TIMEOUT_ACCUM);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+#pragma unroll
+            for (int x = 0; x < NK; ++x) {
+                int32_t h[32];
+                dg::tmem_ld32(lane_addr + C::SUMS + 32 * x, h);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int r = 0; r < FEW_ROWS; ++r) {
+                    long long* w = red + r * (NK * 128) + x * 128 + key;
+                    *w = (oc ? *w : 0) + (long long)h[r] * 256 + h[16 + r];
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free);
+            ++oc;
+        };
+        for (int i = 0; ok && i < n; ++i) {
+            next_scores(i, n + i);
+            if (!ok) break;
+            ok = wait(&p_free[i & 1], ((i >> 1) & 1u) ^ 1u, err, dg::ERR_TIMEOUT_EMPTY);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint32_t m = seen_rows(tile_at(i) * TILE_KEYS);
+            const float kc = kc_of * kf, sv = __uint_as_float(vf);
+            uint8_t* pp = sm + C::P + (i & 1) * 4096 + (key & 15);
+            const int chunk = key >> 4;
+#pragma unroll
+            for (int r = 0; r < FEW_ROWS; ++r) {
+                if (r >= n_rows) break;
+                const float4 row = s_row[r];
+                const float x = __fmaf_rn(__int_as_float(s16[r] + (int)MAGIC_BITS), kf, kc);
+                float w = weight(x, row.x, -row.y);
+                if (!(m >> r & 1)) w = 0.0f;
+                total[r] += __float_as_uint(__fadd_rn(w, MAGIC)) - MAGIC_BITS;
+                const uint32_t d = __float_as_uint(__fmaf_rn(w, __fmul_rn(sv, row.z), MAGIC + 128.0f));
+                uint8_t* at = pp + r * 128 + ((chunk ^ (r & 7)) << 4);
+                at[0] = (uint8_t)(d >> 8);
+                at[16 * 128] = (uint8_t)(d ^ 0x80u);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[i & 1]);
+            if ((i + 1) % FLUSH_TILES == 0 || i + 1 == n) take_sums();
+        }
+        if (n == 0 || !ok)
+            for (int i = threadIdx.x; i < FEW_ROWS * NK * 128; i += 128) red[i] = 0;
+#pragma unroll
+        for (int r = 0; r < FEW_ROWS; ++r) {
+            const unsigned long long lo = __reduce_add_sync(0xffffffffu, total[r] & 0xffffu),
+                                     hi = __reduce_add_sync(0xffffffffu, total[r] >> 16);
+            if (lane == 0) s_total4[warp * FEW_ROWS + r] = lo + (hi << 16);
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (threadIdx.x < FEW_ROWS) {
+            unsigned long long t = 0;
+            for (int w = 0; w < 4; ++w) t += s_total4[w * FEW_ROWS + threadIdx.x];
+            s_total[threadIdx.x] = t;
+        }
+        __syncwarp();
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (soft) {
+        // the cluster's sums: each block writes its share of the outputs
+        if (threadIdx.x < FEW_ROWS) {
+            unsigned long long t = 0;
+            for (uint32_t c = 0; c < ranks; ++c) t += peer_u64(peer_addr(s_total + threadIdx.x, c));
+            s_inv[threadIdx.x] = t ? __ddiv_rn(2097152.0, (double)t) : 0.0;
+            const int r = threadIdx.x;
+            if (rank == 0 && r < n_rows && (row0 + r) % g == 0)
+                a.o_scale[((long long)begin + (row0 + r) / g) * a.c.heads + head] =
+                    t ? make_longlong2(1, (long long)(uint32_t)(21 - scale_exp(row_sig >> 16))) : make_longlong2(0, 0);
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const long long* red = (const long long*)(sm + C::RED);
+        for (int e = (int)(rank * 128 + threadIdx.x); e < n_rows * dim; e += 128 * (int)ranks) {
+            const int r = e / dim, d = e - r * dim;
+            long long v = 0;
+            for (uint32_t c = 0; c < ranks; ++c) v += (long long)peer_u64(peer_addr(red + r * (NK * 128) + d, c));
+            a.o[((long long)begin + (row0 + r) / g) * a.ld_o + (long long)(head * g + (row0 + r) % g) * dim + d] =
+                out_code(v, s_inv[r]);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;");
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();  // nobody leaves while its sums are being read
+    if (warp == 0) {
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+}  // namespace kv

@@ -2,11 +2,12 @@
 // over the cache. All on device buffers, ordered on the caller's stream, nothing allocated and no workspace kept, so
 // calls on several streams and captured graphs share nothing but the caller's own buffers.
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
 #include "context.cuh"
-#include "kv_attend_simple.cuh"
+#include "kv_attend_few.cuh"
 #include "kv_attend_tile.cuh"
 #include "kv_kernels.cuh"
 
@@ -31,8 +32,8 @@ int check_cache(ktmoe_ctx* ctx, const ktmoe_kv_cache* c, const ktmoe_kv_batch* b
     if (c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->n_pages < 1 || c->n_pages > INT32_MAX)
         return fail(ctx, KTMOE_ERR_ARG, "the cache needs 1 to 1024 KV heads and 1 to 2^31 - 1 pages");
     if (b->n_seqs < 0 || b->rows < 0 || b->rows > (int64_t)1 << 30 || b->max_pages < 0 ||
-        (int64_t)b->max_pages * c->page_tokens > (int64_t)1 << 30)
-        return fail(ctx, KTMOE_ERR_ARG, "a batch holds at most 2^30 rows and 2^30 tokens a sequence, none of them negative");
+        (int64_t)b->max_pages * c->page_tokens > (int64_t)1 << 24)
+        return fail(ctx, KTMOE_ERR_ARG, "a batch holds at most 2^30 rows and a page table at most 2^24 tokens a sequence, none of them negative");
     if (b->n_seqs > 0 && (!b->q_begin || !b->kv_len || (b->max_pages > 0 && !b->page_table)))
         return fail(ctx, KTMOE_ERR_ARG, "the batch's offsets, lengths or page table are null");
     *kc = kv::Cache{c->k, c->v, c->k_scale, c->v_scale, c->n_pages, shift, c->n_kv_heads, c->head_dim};
@@ -99,6 +100,53 @@ int launch_tile(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
     KLAUNCH(st, row_blocks(a.b.rows * chunks), 32 * kv::ROW_WARPS, 0, (kv::query_kernel<NK>), a, chunks);
     KLAUNCH(st, (unsigned)(slots * a.c.heads), kv::TILE_THREADS, kv::TileCfg<NK>::BYTES, (kv::attend_tile_kernel<NK>), mk,
             mv, a, (long long)slots);
+    return KTMOE_OK;
+}
+
+// Blocks of a cluster: twice as many while the blocks do not fill the GPU and each would keep two tiles or more, and until
+// a block's tiles fit the scores that stay in TMEM (as far as the page table tells: the lengths are on the device).
+int few_cluster(const ktmoe_ctx* ctx, const kv::AttendArgs& a, int64_t jobs) {
+    const int64_t tiles = ((int64_t)a.b.max_pages << a.c.page_shift) / kv::TILE_KEYS;
+    int c = 1;
+    while (c < 16 && tiles >= 4 * c && (jobs * c < ctx->num_sms || tiles > 26 * c)) c *= 2;
+    return c;
+}
+
+template <int NK>
+int launch_few(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
+    static bool attr_set[64] = {};
+    if (!attr_set[ctx->device & 63]) {
+        CK(cudaFuncSetAttribute(kv::attend_few_kernel<NK>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kv::FewCfg<NK>::BYTES));
+        CK(cudaFuncSetAttribute(kv::attend_few_kernel<NK>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        attr_set[ctx->device & 63] = true;
+    }
+    const int64_t jobs = (a.b.rows * a.group / kv::FEW_ROWS + a.b.n_seqs) * a.c.heads;
+    int c = few_cluster(ctx, a, jobs);
+    static int most[64] = {};  // the largest cluster that fits this device at this kernel's shared memory
+    int& top = most[ctx->device & 63];
+    for (int t = 16; top == 0; t /= 2) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)t);
+        cfg.blockDim = dim3(kv::FEW_THREADS);
+        cfg.dynamicSmemBytes = kv::FewCfg<NK>::BYTES;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = (unsigned)t;
+        at[0].val.clusterDim.y = 1;
+        at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (t == 1 || (cudaOccupancyMaxActiveClusters(&n, kv::attend_few_kernel<NK>, &cfg) == cudaSuccess && n > 0)) top = t;
+        cudaGetLastError();
+    }
+    c = std::min(c, top);
+    if (jobs * c > INT32_MAX) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "too many query rows for one launch");
+    CUtensorMap mk, mv;
+    if (int r = make_pool_map(ctx, &mk, a.c.k, a.c)) return r;
+    if (int r = make_pool_map(ctx, &mv, a.c.v, a.c)) return r;
+    KLAUNCHC(st, (unsigned)(jobs * c), kv::FEW_THREADS, kv::FewCfg<NK>::BYTES, (unsigned)c, (kv::attend_few_kernel<NK>), mk, mv, a);
     return KTMOE_OK;
 }
 
@@ -204,10 +252,10 @@ int ktmoe_attention_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe
     a.o_scale = (longlong2*)o_scale;
     a.vec_o = aligned(o, 16) && ld_o % 4 == 0;
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
-    if (a.group * batch->rows > 16 * batch->n_seqs) return a.c.dim <= 128 ? launch_tile<1>(ctx, st, a) : launch_tile<2>(ctx, st, a);
-    dim3 grid((unsigned)batch->rows, (unsigned)a.c.heads, (unsigned)((a.group + kv::SIMPLE_HEADS - 1) / kv::SIMPLE_HEADS));
-    KLAUNCH(st, grid, 128, 0, (kv::attend_simple_kernel), a);
-    return KTMOE_OK;
+    // few rows a sequence: bound by the keys' and values' bytes; many: by the arithmetic on the scores
+    if ((int64_t)a.group * batch->rows > (int64_t)2 * kv::FEW_ROWS * batch->n_seqs)
+        return a.c.dim <= 128 ? launch_tile<1>(ctx, st, a) : launch_tile<2>(ctx, st, a);
+    return a.c.dim <= 128 ? launch_few<1>(ctx, st, a) : launch_few<2>(ctx, st, a);
 }
 
 }  // extern "C"
