@@ -11,7 +11,8 @@
 // that are formed again. While the cluster exchanges its maxima, V is already on its way. Sums over the keys are
 // integers, so the shares of a cluster add up to the same bits in any order.
 //
-// Roles (224 threads): warps 0-3 softmax, warp 4 TMA, warp 5 the products, warp 6 the keys' scales.
+// Roles (352 threads): warps 0-7 softmax, in two groups that take the tiles in turn, so that one group's waits pass under
+// the other's arithmetic; warp 8 TMA, warp 9 the products, warp 10 the keys' scales.
 #pragma once
 
 #include "kv_attend_tile.cuh"
@@ -19,7 +20,8 @@
 namespace kv {
 
 constexpr int FEW_ROWS = 16;
-constexpr int FEW_THREADS = 224;
+constexpr int FEW_SOFT = 8;  // softmax warps
+constexpr int FEW_THREADS = 32 * (FEW_SOFT + 3);
 
 template <int NK>
 struct FewCfg {
@@ -37,7 +39,7 @@ struct FewCfg {
     static constexpr int ROWS = KEY_SCALES + SCALES * 2 * TILE_KEYS * 4;
     // per row: theta; position; max and largest sigma of each warp and of each block of the cluster; total of the block and
     // of each warp; the row's (max, -theta, 2^-E, 2^E); 2^21 / L
-    static constexpr int BARS = ROWS + FEW_ROWS * (4 + 4 + 32 + 128 + 8 + 32 + 16 + 8);
+    static constexpr int BARS = ROWS + FEW_ROWS * (4 + 4 + 64 + 128 + 8 + 64 + 16 + 8);
     static constexpr int BYTES = 1024 + BARS + 512;
     static_assert(AGAIN + 32 <= SUMS, "TMEM columns");
     static_assert(BYTES <= 232448, "shared memory per block");
@@ -107,12 +109,12 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     float4* s_row = (float4*)(sm + C::ROWS);                  // max, -theta, 2^-E, 2^E
-    unsigned long long* s_total4 = (unsigned long long*)(s_row + FEW_ROWS);  // [4][16]
-    unsigned long long* s_total = s_total4 + 4 * FEW_ROWS;
+    unsigned long long* s_totals = (unsigned long long*)(s_row + FEW_ROWS);  // [8][16]
+    unsigned long long* s_total = s_totals + FEW_SOFT * FEW_ROWS;
     double* s_inv = (double*)(s_total + FEW_ROWS);
-    float* s_top4 = (float*)(s_inv + FEW_ROWS);               // [4][16]
-    uint32_t* s_sig4 = (uint32_t*)(s_top4 + 4 * FEW_ROWS);    // [4][16]
-    uint32_t* s_top = s_sig4 + 4 * FEW_ROWS;                  // [16 ranks][16], written by the ranks
+    float* s_tops = (float*)(s_inv + FEW_ROWS);               // [8][16]
+    uint32_t* s_sigs = (uint32_t*)(s_tops + FEW_SOFT * FEW_ROWS);  // [8][16]
+    uint32_t* s_top = s_sigs + FEW_SOFT * FEW_ROWS;           // [16 ranks][16], written by the ranks
     uint32_t* s_sig = s_top + 16 * FEW_ROWS;                  // [16 ranks][16]
     float* s_theta = (float*)(s_sig + 16 * FEW_ROWS);
     int* s_pos = (int*)(s_theta + FEW_ROWS);
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             mbar_init(&k_full[i], 1);
             mbar_init(&k_free[i], 4);
         }
-        mbar_init(q_full, 4);
+        mbar_init(q_full, FEW_SOFT);
         mbar_init(o_full, 1);
         mbar_init(o_free, 4);
         mbar_init(x_full, FEW_ROWS * ranks);
@@ -211,9 +213,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     const int ps = 1 << a.c.page_shift;
     const int* pages = a.b.pages + (long long)seq * a.b.max_pages;
     int* err = a.err.word;
-    const bool soft = warp < 4;
+    const bool soft = warp < FEW_SOFT;
 
-    if (warp == 4) {
+    if (warp == FEW_SOFT) {
         // K of every tile; then V of tile after tile, and K of tile i + 1 ahead of V of tile i where its scores did not
         // stay. A lane holds one page of a tile; page numbers are read two tiles ahead.
         const int per_tile = TILE_KEYS >> a.c.page_shift, last_page = p1 >> a.c.page_shift;
@@ -264,69 +266,70 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             for (uint32_t j = q > (uint32_t)C::SLOTS ? q - C::SLOTS : 0; j < q; ++j)
                 dg::mbar_wait_drain(&full[j % C::SLOTS], (j / C::SLOTS) & 1u, err, dg::ERR_TIMEOUT_FULL);
         __syncwarp();
-    } else if (warp == 5) {
-        if (lane == 0 && n > 0) {
+    } else if (warp == FEW_SOFT + 1) {
+        if (n > 0) {
+            const bool issue = lane == 0;
             const int ksteps = (dim + 31) / 32;
             const uint32_t id_s = idesc_i8(FEW_ROWS, 0), id_o = idesc_i8(2 * FEW_ROWS, 1u << 15);
             const uint32_t qd = desc_k(smem_u32(sm + C::Q)), kd = desc_k(smem_u32(sm + C::RING)),
                            pd = desc_k(smem_u32(sm + C::P)), vd = desc_mn(smem_u32(sm + C::RING));
             int s = 0;
             uint32_t phase = 0, again = 0, oc = 0;
-            bool ok = wait(q_full, 0, err, dg::ERR_TIMEOUT_FULL);
+            bool ok = warp_wait(q_full, 0, err, dg::ERR_TIMEOUT_FULL);
             auto next = [&]() {
                 if (++s == C::SLOTS) s = 0, phase ^= 1;
             };
             auto scores = [&](int i, bool stays) {
                 const uint32_t b = stays ? i & 3 : again & 1, use = stays ? i >> 2 : again >> 1;
-                ok = ok && wait(stays ? &s_free[b] : &r_free[b], (use & 1u) ^ 1u, err, dg::ERR_TIMEOUT_ACCUM);
+                ok = ok && warp_wait(stays ? &s_free[b] : &r_free[b], (use & 1u) ^ 1u, err, dg::ERR_TIMEOUT_ACCUM);
                 const uint32_t d = tmem + (stays ? 16 * i : C::AGAIN + 16 * b);
 #pragma unroll
                 for (int x = 0; x < NK; ++x) {
-                    ok = ok && wait(&full[s], phase, err, dg::ERR_TIMEOUT_FULL);
+                    ok = ok && warp_wait(&full[s], phase, err, dg::ERR_TIMEOUT_FULL);
                     if (!ok) return;
                     asm volatile("tcgen05.fence::after_thread_sync;");
                     const uint32_t kx = kd + s * (C::SLOT >> 4), qx = qd + x * (16 * 128 >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        if (4 * x + kk < ksteps) umma(d, kx + 2 * kk, qx + 2 * kk, id_s, x + kk > 0);
-                    umma_commit(&empty[s]);
+                        if (4 * x + kk < ksteps) umma(issue, d, kx + 2 * kk, qx + 2 * kk, id_s, x + kk > 0);
+                    umma_arrive(issue, &empty[s]);
                     next();
                 }
-                umma_commit(stays ? &s_full[b] : &r_full[b]);
+                umma_arrive(issue, stays ? &s_full[b] : &r_full[b]);
                 if (!stays) ++again;
             };
             for (int i = 0; ok && i < n; ++i) scores(i, i < C::KEEP);
             for (int i = 0; ok && i < n; ++i) {
                 if (i + 1 >= C::KEEP && i + 1 < n) scores(i + 1, false);
-                ok = ok && wait(&p_full[i & 1], (i >> 1) & 1u, err, dg::ERR_TIMEOUT_ACCUM);
+                ok = ok && warp_wait(&p_full[i & 1], (i >> 1) & 1u, err, dg::ERR_TIMEOUT_ACCUM);
 #pragma unroll
                 for (int x = 0; x < NK; ++x) {
-                    ok = ok && wait(&full[s], phase, err, dg::ERR_TIMEOUT_FULL);
+                    ok = ok && warp_wait(&full[s], phase, err, dg::ERR_TIMEOUT_FULL);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;");
                     const uint32_t vx = vd + s * (C::SLOT >> 4), px = pd + (i & 1) * (32 * 128 >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        umma(tmem + C::SUMS + 32 * x, vx + kk * (32 * 128 >> 4), px + 2 * kk, id_o, i % FLUSH_TILES + kk > 0);
-                    umma_commit(&empty[s]);
+                        umma(issue, tmem + C::SUMS + 32 * x, vx + kk * (32 * 128 >> 4), px + 2 * kk, id_o, i % FLUSH_TILES + kk > 0);
+                    umma_arrive(issue, &empty[s]);
                     next();
                 }
                 if (!ok) break;
-                umma_commit(&p_free[i & 1]);
+                umma_arrive(issue, &p_free[i & 1]);
                 if (i + 1 == n || (i + 1) % FLUSH_TILES == 0) {
-                    umma_commit(o_full);
+                    umma_arrive(issue, o_full);
                     if (i + 1 < n) {  // the sums are taken out and begin anew
-                        ok = wait(o_free, oc & 1u, err, dg::ERR_TIMEOUT_ACCUM);
+                        ok = warp_wait(o_free, oc & 1u, err, dg::ERR_TIMEOUT_ACCUM);
                         asm volatile("tcgen05.fence::after_thread_sync;");
                     }
                     ++oc;
                 }
             }
-            umma_commit(done);
-            dg::mbar_wait_drain(done, 0u, err, dg::ERR_TIMEOUT_ACCUM);
+            umma_arrive(issue, done);
+            if (issue) dg::mbar_wait_drain(done, 0u, err, dg::ERR_TIMEOUT_ACCUM);
         }
         __syncwarp();
-    } else if (warp == 6) {
+    } else if (warp == FEW_SOFT + 2) {
         // The scales of each tile's keys, four keys a lane, for both phases: read four tiles ahead, their pages eight.
         const int total = 2 * n;
         auto key_of = [&](int u) { return tile_at(u >= n ? u - n : u) * TILE_KEYS + 4 * lane; };
@@ -383,17 +386,17 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     }
 
     // ── the softmax warps; the others go on to where the cluster meets ──
-    const int key = 32 * (warp & 3) + lane;  // of a tile
+    const int key = 32 * (warp & 3) + lane, grp = (warp >> 2) & 1;  // of a tile; this group takes tiles grp, grp + 2, ..
     const uint32_t lane_addr = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     bool ok = true;
-    uint32_t again = 0;
     int32_t s16[16];
     float kf = 0.0f;
     uint32_t vf = 0;
     // the scores of tile i and its keys' scales; `stays` tiles of phase 1 are in TMEM already
     auto next_scores = [&](int i, int u) {
         const bool stays = i < C::KEEP;
-        const uint32_t b = again & 1;
+        // the scores that do not stay are numbered over both phases
+        const uint32_t again = (uint32_t)(i - C::KEEP + (u < n ? 0 : n_again)), b = again & 1;
         if (!stays) {
             ok = wait(&r_full[b], (again >> 1) & 1u, err, dg::ERR_TIMEOUT_ACCUM);
         } else if (u < n) {
@@ -418,7 +421,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
                 mbar_arrive(&s_free[i & 3]);
             }
         }
-        if (!stays) ++again;
     };
     // bit r: row r sees this thread's key of the tile
     auto seen_rows = [&](int j0) -> uint32_t {
@@ -437,7 +439,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         if (threadIdx.x < FEW_ROWS) s_pos[threadIdx.x] = threadIdx.x < n_rows ? len - n_new + (row0 + (int)threadIdx.x) / g : -1;
         constexpr int B = RowBatch<NK>::B;
 #pragma unroll 1
-        for (int rb = B * warp; rb < n_rows; rb += 4 * B) {
+        for (int rb = B * warp; rb < n_rows; rb += FEW_SOFT * B) {
             int count = 0;
 #pragma unroll 1
             for (int r = rb; r < min(rb + B, n_rows); r += count) {
@@ -467,13 +469,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // s_pos, s_theta
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // s_pos, s_theta
         // ── phase 0: the maxima ──
         float top[FEW_ROWS];
         uint32_t sig[FEW_ROWS];
 #pragma unroll
         for (int r = 0; r < FEW_ROWS; ++r) top[r] = -INFINITY, sig[r] = 0;
-        for (int i = 0; i < n; ++i) {
+        for (int i = grp; i < n; i += 2) {
             next_scores(i, i);
             if (!ok) break;
             const uint32_t m = seen_rows(tile_at(i) * TILE_KEYS);
@@ -495,17 +497,17 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             for (int o = 16; o; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
             const uint32_t sg = __reduce_max_sync(0xffffffffu, sig[r]);
             if (lane == 0) {
-                s_top4[warp * FEW_ROWS + r] = t;
-                s_sig4[warp * FEW_ROWS + r] = sg;
+                s_tops[warp * FEW_ROWS + r] = t;
+                s_sigs[warp * FEW_ROWS + r] = sg;
             }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         if (threadIdx.x < FEW_ROWS) {
             float t = -INFINITY;
             uint32_t sg = 0;
-            for (int w = 0; w < 4; ++w) {
-                t = fmaxf(t, s_top4[w * FEW_ROWS + threadIdx.x]);
-                sg = max(sg, s_sig4[w * FEW_ROWS + threadIdx.x]);
+            for (int w = 0; w < FEW_SOFT; ++w) {
+                t = fmaxf(t, s_tops[w * FEW_ROWS + threadIdx.x]);
+                sg = max(sg, s_sigs[w * FEW_ROWS + threadIdx.x]);
             }
             for (uint32_t c = 0; c < ranks; ++c) {  // to every block of the cluster
                 peer_store(peer_addr(s_top + rank * FEW_ROWS + threadIdx.x, c), __float_as_uint(t));
@@ -528,14 +530,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             const int e = row_sig ? scale_exp(row_sig >> 16) : 0;
             s_row[threadIdx.x] = make_float4(t, s_pos[threadIdx.x] >= 0 ? -s_theta[threadIdx.x] : 0.0f, pow2f(-e), pow2f(e));
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         // ── phase 1: the weights and the sums ──
         uint32_t total[FEW_ROWS];  // at most 131072 tiles of one key a thread: below 2^32
 #pragma unroll
         for (int r = 0; r < FEW_ROWS; ++r) total[r] = 0;
         long long* red = (long long*)(sm + C::RED);
-        uint32_t oc = 0;
-        auto take_sums = [&]() {  // thread `key` has column 128 x + key of O
+        // Sums number oc are taken by the group whose tile was the last; thread `key` has column 128 x + key of O.
+        auto take_sums = [&](uint32_t oc) {
             ok = ok && wait(o_full, oc & 1u, err, dg::ERR_TIMEOUT_ACCUM);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) return;
@@ -554,9 +556,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             asm volatile("tcgen05.fence::before_thread_sync;");
             __syncwarp();
             if (lane == 0) mbar_arrive(o_free);
-            ++oc;
         };
-        for (int i = 0; ok && i < n; ++i) {
+        for (int i = grp; ok && i < n; i += 2) {
             next_scores(i, n + i);
             if (!ok) break;
             ok = wait(&p_free[i & 1], ((i >> 1) & 1u) ^ 1u, err, dg::ERR_TIMEOUT_EMPTY);
@@ -582,20 +583,20 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[i & 1]);
-            if ((i + 1) % FLUSH_TILES == 0 || i + 1 == n) take_sums();
+            if ((i + 1) % FLUSH_TILES == 0 || i + 1 == n) take_sums((uint32_t)i / FLUSH_TILES);
         }
-        if (n == 0 || !ok)
-            for (int i = threadIdx.x; i < FEW_ROWS * NK * 128; i += 128) red[i] = 0;
+        if (n == 0)
+            for (int i = threadIdx.x; i < FEW_ROWS * NK * 128; i += 32 * FEW_SOFT) red[i] = 0;
 #pragma unroll
         for (int r = 0; r < FEW_ROWS; ++r) {
             const unsigned long long lo = __reduce_add_sync(0xffffffffu, total[r] & 0xffffu),
                                      hi = __reduce_add_sync(0xffffffffu, total[r] >> 16);
-            if (lane == 0) s_total4[warp * FEW_ROWS + r] = lo + (hi << 16);
+            if (lane == 0) s_totals[warp * FEW_ROWS + r] = lo + (hi << 16);
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         if (threadIdx.x < FEW_ROWS) {
             unsigned long long t = 0;
-            for (int w = 0; w < 4; ++w) t += s_total4[w * FEW_ROWS + threadIdx.x];
+            for (int w = 0; w < FEW_SOFT; ++w) t += s_totals[w * FEW_ROWS + threadIdx.x];
             s_total[threadIdx.x] = t;
         }
         __syncwarp();
@@ -613,9 +614,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
                 a.o_scale[((long long)begin + (row0 + r) / g) * a.c.heads + head] =
                     t ? make_longlong2(1, (long long)(uint32_t)(21 - scale_exp(row_sig >> 16))) : make_longlong2(0, 0);
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         const long long* red = (const long long*)(sm + C::RED);
-        for (int e = (int)(rank * 128 + threadIdx.x); e < n_rows * dim; e += 128 * (int)ranks) {
+        for (int e = (int)(rank * 32 * FEW_SOFT + threadIdx.x); e < n_rows * dim; e += 32 * FEW_SOFT * (int)ranks) {
             const int r = e / dim, d = e - r * dim;
             long long v = 0;
             for (uint32_t c = 0; c < ranks; ++c) v += (long long)peer_u64(peer_addr(red + r * (NK * 128) + d, c));

@@ -26,7 +26,6 @@ using dg::mbar_arrive;
 using dg::mbar_arrive_expect_tx;
 using dg::mbar_init;
 using dg::smem_u32;
-using dg::umma_commit;
 
 constexpr int TILE_KEYS = 128;
 constexpr int TILE_ROWS = 128;
@@ -49,6 +48,11 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, i
     }
 }
 
+// wait() by a whole warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+    return __all_sync(0xffffffffu, wait(bar, parity, err, code));
+}
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
                                             uint64_t* bar) {
     asm volatile(
@@ -65,13 +69,23 @@ constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
 __device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | 1u << 16; }
 __device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return (addr >> 4) | (1024u >> 4) << 16; }
 
-// D += A B (or D = A B, accumulate = 0) of 8-bit operands given by their descriptors' low words.
-__device__ __forceinline__ void umma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+// D += A B (or D = A B, accumulate = 0) of 8-bit operands given by their descriptors' low words, and the arrival of a
+// barrier when every product issued so far is done. A whole warp comes here and the one lane with `issue` set acts: with
+// the loop around them uniform the operands stay in uniform registers (issuing the four products of a tile from a branch
+// of one lane took 850 clocks, moving operands over).
+__device__ __forceinline__ void umma(bool issue, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(DESC_HI)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(DESC_HI), "r"((int)issue)
+        : "memory");
+}
+__device__ __forceinline__ void umma_arrive(bool issue, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"((int)issue)
         : "memory");
 }
 
@@ -408,13 +422,14 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         }
     } else if (warp == SOFTMAX_WARPS + 1) {
         // scores: S of tile after tile, as soon as K has landed and the buffer has been read
-        if (lane == 0) {
+        {
+            const bool issue = lane == 0;
             const int ksteps = (dim + 31) / 32;
             const uint32_t id_s = idesc_i8(TILE_KEYS, 0);
             const uint32_t qd = desc_k(smem_u32(sm + C::Q)), kd = desc_k(smem_u32(sm + C::RING));
             int ks = 0;
             uint32_t kph = 0;
-            bool ok = n_pass == 0 || wait(q_full, 0, a.err.word, dg::ERR_TIMEOUT_FULL);
+            bool ok = n_pass == 0 || warp_wait(q_full, 0, a.err.word, dg::ERR_TIMEOUT_FULL);
             const int total = n_pass * n;
             for (int u = 0; ok && u < total; ++u) {
                 // scores number u go to buffer u % 4 in pass 0 and to buffer u % 2 later, first when pass 0 has read it
@@ -423,31 +438,32 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 const uint32_t use = (uint32_t)(maxima ? u >> 2 : (u - n) >> 1);
                 if (!maxima && use == 0) {
                     const uint32_t uses = (uint32_t)(n - (int)b + 3) / 4;
-                    ok = uses == 0 || wait(&m_free[b], (uses - 1) & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+                    ok = uses == 0 || warp_wait(&m_free[b], (uses - 1) & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
                 }
-                ok = ok && wait(maxima ? &m_free[b] : &s_free[b], (use & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+                ok = ok && warp_wait(maxima ? &m_free[b] : &s_free[b], (use & 1u) ^ 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
 #pragma unroll
                 for (int x = 0; x < NK; ++x) {
-                    ok = ok && wait(&full[ks], kph, a.err.word, dg::ERR_TIMEOUT_FULL);
+                    ok = ok && warp_wait(&full[ks], kph, a.err.word, dg::ERR_TIMEOUT_FULL);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;");
                     // descriptors hold addresses in units of 16 bytes
                     const uint32_t qx = qd + x * (C::SLOT >> 4), kx = kd + ks * (C::SLOT >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        if (4 * x + kk < ksteps) umma(tmem + b * 128, qx + 2 * kk, kx + 2 * kk, id_s, 1u);
-                    umma_commit(&empty[ks]);
+                        if (4 * x + kk < ksteps) umma(issue, tmem + b * 128, qx + 2 * kk, kx + 2 * kk, id_s, 1u);
+                    umma_arrive(issue, &empty[ks]);
                     if (++ks == C::K_SLOTS) ks = 0, kph ^= 1;
                 }
                 if (!ok) break;
-                umma_commit(maxima ? &m_full[b] : &s_full[b]);
+                umma_arrive(issue, maxima ? &m_full[b] : &s_full[b]);
             }
-            umma_commit(&done[0]);
-            dg::mbar_wait_drain(&done[0], 0u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+            umma_arrive(issue, &done[0]);
+            if (issue) dg::mbar_wait_drain(&done[0], 0u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
         }
     } else if (warp == SOFTMAX_WARPS + 3) {
         // the values: O += P V with both digits, as soon as a tile's weights are there
-        if (lane == 0) {
+        {
+            const bool issue = lane == 0;
             const uint32_t pd = desc_k(smem_u32(sm + C::P)), vd = desc_mn(smem_u32(sm + C::RING));
             int vs = C::K_SLOTS;
             uint32_t vph = 0, b = (uint32_t)n & 1, pph = 0, oc = 0;  // pass 1 begins with scores number n
@@ -455,27 +471,27 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             for (int pass = 1; ok && pass < n_pass; ++pass) {
                 const uint32_t id_o = idesc_i8(min(128, dim - (pass - 1) * 128), 1u << 16);
                 for (int i = 0; i < n; ++i) {
-                    ok = wait(&p_full[b], pph, a.err.word, dg::ERR_TIMEOUT_ACCUM) &&
-                         wait(&full[vs], vph, a.err.word, dg::ERR_TIMEOUT_FULL);
+                    ok = warp_wait(&p_full[b], pph, a.err.word, dg::ERR_TIMEOUT_ACCUM) &&
+                         warp_wait(&full[vs], vph, a.err.word, dg::ERR_TIMEOUT_FULL);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;");
                     const uint32_t px = pd + b * (2 * C::SLOT >> 4), vx = vd + vs * (C::SLOT >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
-                        umma(tmem + 256, px + 2 * kk, vx + kk * (32 * 128 >> 4), id_o, i + kk > 0);
-                        umma(tmem + 384, px + (C::SLOT >> 4) + 2 * kk, vx + kk * (32 * 128 >> 4), id_o, i + kk > 0);
+                        umma(issue, tmem + 256, px + 2 * kk, vx + kk * (32 * 128 >> 4), id_o, i + kk > 0);
+                        umma(issue, tmem + 384, px + (C::SLOT >> 4) + 2 * kk, vx + kk * (32 * 128 >> 4), id_o, i + kk > 0);
                     }
-                    umma_commit(&empty[vs]);
-                    umma_commit(&p_free[b]);
+                    umma_arrive(issue, &empty[vs]);
+                    umma_arrive(issue, &p_free[b]);
                     if (++vs == C::SLOTS) vs = C::K_SLOTS, vph ^= 1;
                     b ^= 1;
                     if (second) pph ^= 1;
                     second = !second;
                     // the sums are read at the end of the block, and carried on every FLUSH_TILES tiles
                     if (i + 1 == n || (i + 1) % FLUSH_TILES == 0) {
-                        umma_commit(o_full);
+                        umma_arrive(issue, o_full);
                         if (i + 1 < n || pass + 1 < n_pass) {
-                            ok = wait(o_free, oc & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+                            ok = warp_wait(o_free, oc & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
                             if (!ok) break;
                             asm volatile("tcgen05.fence::after_thread_sync;");
                         }
@@ -483,8 +499,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     }
                 }
             }
-            umma_commit(&done[1]);
-            dg::mbar_wait_drain(&done[1], 0u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
+            umma_arrive(issue, &done[1]);
+            if (issue) dg::mbar_wait_drain(&done[1], 0u, a.err.word, dg::ERR_TIMEOUT_ACCUM);
         }
     } else if (warp == SOFTMAX_WARPS + 2) {
         // The scales of each tile's keys, four keys a lane: read four tiles ahead, their page numbers eight.
