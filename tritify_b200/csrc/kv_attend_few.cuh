@@ -7,12 +7,15 @@
 // digits of the weights in one product of 32 columns). A thread has one key of a tile.
 //
 // The row maxima must be known before the first weight is rounded, so there are two phases; K is read once all the same,
-// because the scores wait in TMEM: 16 columns a tile, 28 tiles a block (26 of rows longer than 128). Only tiles beyond
-// that are formed again. While the cluster exchanges its maxima, V is already on its way. Sums over the keys are
-// integers, so the shares of a cluster add up to the same bits in any order.
+// because the scores wait in TMEM, 16 columns a tile. Only tiles beyond what a block has room for are formed again. While
+// the cluster exchanges its maxima, V is already on its way. Sums over the keys are integers, so the shares of a cluster
+// add up to the same bits in any order: each block adds its own into the shared memory of the block that writes them out.
 //
-// Roles (352 threads): warps 0-7 softmax, in two groups that take the tiles in turn, so that one group's waits pass under
-// the other's arithmetic; warp 8 TMA, warp 9 the products, warp 10 the keys' scales.
+// A block's start, exchange and end are latency (10 us of a block's 26 at 12 tiles), so where the sequences are not so
+// long that the scores of a block need all of TMEM, two blocks share an SM, one's waits under the other's stream.
+//
+// Roles: softmax warps, in one or two groups of four that take the tiles in turn; then one warp each for TMA, the
+// products and the keys' scales.
 #pragma once
 
 #include "kv_attend_tile.cuh"
@@ -20,29 +23,31 @@
 namespace kv {
 
 constexpr int FEW_ROWS = 16;
-constexpr int FEW_SOFT = 8;  // softmax warps
-constexpr int FEW_THREADS = 32 * (FEW_SOFT + 3);
 
-template <int NK>
+// NK: 128-byte blocks of a key row; PER_SM: blocks that share an SM.
+template <int NK, int PER_SM>
 struct FewCfg {
     static constexpr int SLOT = TILE_KEYS * 128;
-    static constexpr int SLOTS = 8;
+    static constexpr int SLOTS = 8 / PER_SM;
+    static constexpr int SOFT = 8 / PER_SM;  // softmax warps
+    static constexpr int THREADS = 32 * (SOFT + 3);
+    static constexpr int COLS = 512 / PER_SM;  // of TMEM
     static constexpr int SCALES = 4;
-    static constexpr int KEEP = NK == 1 ? 28 : 26;  // tiles whose scores stay in TMEM
-    static constexpr int AGAIN = 16 * KEEP;         // two more score buffers, for the others
-    static constexpr int SUMS = 512 - 32 * NK;      // O^T of each 128 columns: 16 hi, 16 lo
+    static constexpr int SUMS = COLS - 32 * NK;        // O^T of each 128 columns: 16 hi, 16 lo
+    static constexpr int KEEP = (SUMS - 32) / 16;      // tiles whose scores stay in TMEM: 28, 26 (NK 2), 12 (PER_SM 2)
+    static constexpr int AGAIN = 16 * KEEP;            // two more score buffers, for the others
     static constexpr int RING = 0;
     static constexpr int Q = RING + SLOTS * SLOT;               // [NK][16 rows][128]
     static constexpr int P = Q + NK * 16 * 128;                 // [2][16 hi, 16 lo][128 keys]
     static constexpr int RED = P + 2 * 32 * 128;                // int64 [16 rows][NK * 128]
     static constexpr int KEY_SCALES = RED + 16 * NK * 128 * 8;  // [SCALES][sigma_k, sigma_v][128]
     static constexpr int ROWS = KEY_SCALES + SCALES * 2 * TILE_KEYS * 4;
-    // per row: theta; position; max and largest sigma of each warp and of each block of the cluster; total of the block and
-    // of each warp; the row's (max, -theta, 2^-E, 2^E); 2^21 / L
-    static constexpr int BARS = ROWS + FEW_ROWS * (4 + 4 + 64 + 128 + 8 + 64 + 16 + 8);
+    // per row: theta; position; max and largest sigma of each warp and of each block of the cluster; total of the cluster;
+    // the row's (max, -theta, 2^-E, 2^E); 2^21 / L
+    static constexpr int BARS = ROWS + FEW_ROWS * (4 + 4 + 64 + 128 + 8 + 16 + 8);
     static constexpr int BYTES = 1024 + BARS + 512;
     static_assert(AGAIN + 32 <= SUMS, "TMEM columns");
-    static_assert(BYTES <= 232448, "shared memory per block");
+    static_assert(PER_SM * (BYTES + 1024) <= 233472, "shared memory of an SM");
 };
 
 __device__ __forceinline__ uint32_t cluster_ctarank() {
@@ -94,39 +99,38 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int
         }
     }
 }
-__device__ __forceinline__ uint64_t peer_u64(uint32_t a) {
-    uint64_t v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-    return v;
+__device__ __forceinline__ void peer_add(uint32_t a, uint64_t v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.add.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
+// A float as an integer of the same order, and back.
+__device__ __forceinline__ int ordered(int b) { return b ^ ((b >> 31) & 0x7fffffff); }
 
-template <int NK>
-__global__ void __launch_bounds__(FEW_THREADS, 1)
+template <int NK, int PER_SM>
+__global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
     attend_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const AttendArgs a) {
     kt::pdl_enter();
-    using C = FewCfg<NK>;
+    using C = FewCfg<NK, PER_SM>;
+    constexpr int GROUPS = C::SOFT / 4;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     float4* s_row = (float4*)(sm + C::ROWS);                  // max, -theta, 2^-E, 2^E
-    unsigned long long* s_totals = (unsigned long long*)(s_row + FEW_ROWS);  // [8][16]
-    unsigned long long* s_total = s_totals + FEW_SOFT * FEW_ROWS;
+    unsigned long long* s_total = (unsigned long long*)(s_row + FEW_ROWS);
     double* s_inv = (double*)(s_total + FEW_ROWS);
-    float* s_tops = (float*)(s_inv + FEW_ROWS);               // [8][16]
-    uint32_t* s_sigs = (uint32_t*)(s_tops + FEW_SOFT * FEW_ROWS);  // [8][16]
-    uint32_t* s_top = s_sigs + FEW_SOFT * FEW_ROWS;           // [16 ranks][16], written by the ranks
+    int* s_tops = (int*)(s_inv + FEW_ROWS);                   // [8 warps][16]
+    uint32_t* s_sigs = (uint32_t*)(s_tops + 8 * FEW_ROWS);    // [8 warps][16]
+    uint32_t* s_top = s_sigs + 8 * FEW_ROWS;                  // [16 ranks][16], written by the ranks
     uint32_t* s_sig = s_top + 16 * FEW_ROWS;                  // [16 ranks][16]
     float* s_theta = (float*)(s_sig + 16 * FEW_ROWS);
     int* s_pos = (int*)(s_theta + FEW_ROWS);
     uint64_t* full = (uint64_t*)(sm + C::BARS);  // [SLOTS]
-    uint64_t* empty = full + C::SLOTS;           // [SLOTS]
-    uint64_t* s_full = empty + C::SLOTS;         // [4] scores that stay
-    uint64_t* s_free = s_full + 4;               // [4]
-    uint64_t* r_full = s_free + 4;               // [2] scores formed twice
-    uint64_t* r_free = r_full + 2;               // [2]
+    // [SLOTS] the products of a block are done: its slot is free, the scores of its tile are there (K), the digits of its
+    // tile have been read (V). One arrival for all: each costs the issuing warp 130 clocks.
+    uint64_t* empty = full + C::SLOTS;
+    uint64_t* s_free = empty + C::SLOTS;         // [2] scores that stay have been seen (the products run two tiles ahead)
+    uint64_t* r_free = s_free + 2;               // [2] scores formed again have been read
     uint64_t* p_full = r_free + 2;               // [2]
-    uint64_t* p_free = p_full + 2;               // [2]
-    uint64_t* k_full = p_free + 2;               // [SCALES]
+    uint64_t* k_full = p_full + 2;               // [SCALES]
     uint64_t* k_free = k_full + C::SCALES;       // [SCALES]
     uint64_t* q_full = k_free + C::SCALES;
     uint64_t* o_full = q_full + 1;
@@ -167,21 +171,16 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&s_free[i], 4);
-        }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&r_full[i], 1);
+            mbar_init(&s_free[i], 4);
             mbar_init(&r_free[i], 4);
             mbar_init(&p_full[i], 4);
-            mbar_init(&p_free[i], 1);
         }
         for (int i = 0; i < C::SCALES; ++i) {
             mbar_init(&k_full[i], 1);
             mbar_init(&k_free[i], 4);
         }
-        mbar_init(q_full, FEW_SOFT);
+        mbar_init(q_full, C::SOFT);
         mbar_init(o_full, 1);
         mbar_init(o_free, 4);
         mbar_init(x_full, FEW_ROWS * ranks);
@@ -200,11 +199,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     const int n = i_last - i_first, n_again = max(0, n - C::KEEP);
     auto tile_at = [&](int i) { return all_tiles.at(i_first + i); };
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(C::COLS));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         asm volatile("tcgen05.fence::before_thread_sync;");
     }
-    // the blocks of the cluster are there and their barriers stand
+    for (int i = threadIdx.x; i < FEW_ROWS * NK * 128; i += C::THREADS) ((long long*)(sm + C::RED))[i] = 0;
+    if (threadIdx.x < FEW_ROWS) s_total[threadIdx.x] = 0;
+    // the blocks of the cluster are there, their barriers stand and their sums are zero
     __syncwarp();
     cluster_arrive();
     cluster_wait();
@@ -213,9 +214,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     const int ps = 1 << a.c.page_shift;
     const int* pages = a.b.pages + (long long)seq * a.b.max_pages;
     int* err = a.err.word;
-    const bool soft = warp < FEW_SOFT;
+    // Blocks of K and V in the order in which they are loaded and used: all K, then V of tile i, preceded by K of tile
+    // i + 1 where its scores did not stay. The number of the last block of K (first, again) and of V of tile i:
+    auto k_block = [&](int i) { return (i + 1) * NK - 1; };
+    auto k_again = [&](int i) { return (n + i - 1 + (i - C::KEEP) + 1) * NK - 1; };
+    auto v_block = [&](int i) { return (n + i + max(0, min(i + 2, n) - C::KEEP) + 1) * NK - 1; };
+    const bool soft = warp < C::SOFT;
 
-    if (warp == FEW_SOFT) {
+    if (warp == C::SOFT) {
         // K of every tile; then V of tile after tile, and K of tile i + 1 ahead of V of tile i where its scores did not
         // stay. A lane holds one page of a tile; page numbers are read two tiles ahead.
         const int per_tile = TILE_KEYS >> a.c.page_shift, last_page = p1 >> a.c.page_shift;
@@ -266,7 +272,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             for (uint32_t j = q > (uint32_t)C::SLOTS ? q - C::SLOTS : 0; j < q; ++j)
                 dg::mbar_wait_drain(&full[j % C::SLOTS], (j / C::SLOTS) & 1u, err, dg::ERR_TIMEOUT_FULL);
         __syncwarp();
-    } else if (warp == FEW_SOFT + 1) {
+    } else if (warp == C::SOFT + 1) {
         if (n > 0) {
             const bool issue = lane == 0;
             const int ksteps = (dim + 31) / 32;
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
                 if (++s == C::SLOTS) s = 0, phase ^= 1;
             };
             auto scores = [&](int i, bool stays) {
-                const uint32_t b = stays ? i & 3 : again & 1, use = stays ? i >> 2 : again >> 1;
+                const uint32_t b = stays ? i & 1 : again & 1, use = stays ? i >> 1 : again >> 1;
                 ok = ok && warp_wait(stays ? &s_free[b] : &r_free[b], (use & 1u) ^ 1u, err, dg::ERR_TIMEOUT_ACCUM);
                 const uint32_t d = tmem + (stays ? 16 * i : C::AGAIN + 16 * b);
 #pragma unroll
@@ -295,7 +301,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
                     umma_arrive(issue, &empty[s]);
                     next();
                 }
-                umma_arrive(issue, stays ? &s_full[b] : &r_full[b]);
                 if (!stays) ++again;
             };
             for (int i = 0; ok && i < n; ++i) scores(i, i < C::KEEP);
@@ -315,7 +320,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
                     next();
                 }
                 if (!ok) break;
-                umma_arrive(issue, &p_free[i & 1]);
                 if (i + 1 == n || (i + 1) % FLUSH_TILES == 0) {
                     umma_arrive(issue, o_full);
                     if (i + 1 < n) {  // the sums are taken out and begin anew
@@ -329,7 +333,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             if (issue) dg::mbar_wait_drain(done, 0u, err, dg::ERR_TIMEOUT_ACCUM);
         }
         __syncwarp();
-    } else if (warp == FEW_SOFT + 2) {
+    } else if (warp == C::SOFT + 2) {
         // The scales of each tile's keys, four keys a lane, for both phases: read four tiles ahead, their pages eight.
         const int total = 2 * n;
         auto key_of = [&](int u) { return tile_at(u >= n ? u - n : u) * TILE_KEYS + 4 * lane; };
@@ -386,22 +390,22 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
     }
 
     // ── the softmax warps; the others go on to where the cluster meets ──
-    const int key = 32 * (warp & 3) + lane, grp = (warp >> 2) & 1;  // of a tile; this group takes tiles grp, grp + 2, ..
+    const int key = 32 * (warp & 3) + lane, grp = (warp >> 2) % GROUPS;  // of a tile; a group takes every GROUPSth
     const uint32_t lane_addr = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     bool ok = true;
     int32_t s16[16];
     float kf = 0.0f;
     uint32_t vf = 0;
+    // the products of block q of K and V are done
+    auto block_done = [&](int q) {
+        return wait(&empty[q % C::SLOTS], (uint32_t)(q / C::SLOTS) & 1u, err, dg::ERR_TIMEOUT_ACCUM);
+    };
     // the scores of tile i and its keys' scales; `stays` tiles of phase 1 are in TMEM already
     auto next_scores = [&](int i, int u) {
         const bool stays = i < C::KEEP;
         // the scores that do not stay are numbered over both phases
         const uint32_t again = (uint32_t)(i - C::KEEP + (u < n ? 0 : n_again)), b = again & 1;
-        if (!stays) {
-            ok = wait(&r_full[b], (again >> 1) & 1u, err, dg::ERR_TIMEOUT_ACCUM);
-        } else if (u < n) {
-            ok = wait(&s_full[i & 3], (i >> 2) & 1u, err, dg::ERR_TIMEOUT_ACCUM);
-        }
+        if (!stays || u < n) ok = block_done(u < n ? k_block(i) : k_again(i));
         ok = ok && wait(&k_full[u & 3], (u >> 2) & 1u, err, dg::ERR_TIMEOUT_FULL);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             if (!stays) {
                 mbar_arrive(&r_free[b]);
             } else if (u < n) {
-                mbar_arrive(&s_free[i & 3]);
+                mbar_arrive(&s_free[i & 1]);
             }
         }
     };
@@ -439,7 +443,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         if (threadIdx.x < FEW_ROWS) s_pos[threadIdx.x] = threadIdx.x < n_rows ? len - n_new + (row0 + (int)threadIdx.x) / g : -1;
         constexpr int B = RowBatch<NK>::B;
 #pragma unroll 1
-        for (int rb = B * warp; rb < n_rows; rb += FEW_SOFT * B) {
+        for (int rb = B * warp; rb < n_rows; rb += C::SOFT * B) {
             int count = 0;
 #pragma unroll 1
             for (int r = rb; r < min(rb + B, n_rows); r += count) {
@@ -469,13 +473,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // s_pos, s_theta
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * C::SOFT) : "memory");  // s_pos, s_theta
         // ── phase 0: the maxima ──
         float top[FEW_ROWS];
         uint32_t sig[FEW_ROWS];
 #pragma unroll
         for (int r = 0; r < FEW_ROWS; ++r) top[r] = -INFINITY, sig[r] = 0;
-        for (int i = grp; i < n; i += 2) {
+        for (int i = grp; i < n; i += GROUPS) {
             next_scores(i, i);
             if (!ok) break;
             const uint32_t m = seen_rows(tile_at(i) * TILE_KEYS);
@@ -492,28 +496,27 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         }
 #pragma unroll
         for (int r = 0; r < FEW_ROWS; ++r) {
-            float t = top[r];
-#pragma unroll
-            for (int o = 16; o; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            if (r >= n_rows) break;
+            const int t = __reduce_max_sync(0xffffffffu, ordered(__float_as_int(top[r])));
             const uint32_t sg = __reduce_max_sync(0xffffffffu, sig[r]);
             if (lane == 0) {
                 s_tops[warp * FEW_ROWS + r] = t;
                 s_sigs[warp * FEW_ROWS + r] = sg;
             }
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (threadIdx.x < FEW_ROWS) {
-            float t = -INFINITY;
-            uint32_t sg = 0;
-            for (int w = 0; w < FEW_SOFT; ++w) {
-                t = fmaxf(t, s_tops[w * FEW_ROWS + threadIdx.x]);
-                sg = max(sg, s_sigs[w * FEW_ROWS + threadIdx.x]);
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * C::SOFT) : "memory");
+        const int r = threadIdx.x % FEW_ROWS;
+        int t = ordered(__float_as_int(-INFINITY));
+        uint32_t sg = 0;
+        if (r < n_rows)
+            for (int w = 0; w < C::SOFT; ++w) {
+                t = max(t, s_tops[w * FEW_ROWS + r]);
+                sg = max(sg, s_sigs[w * FEW_ROWS + r]);
             }
-            for (uint32_t c = 0; c < ranks; ++c) {  // to every block of the cluster
-                peer_store(peer_addr(s_top + rank * FEW_ROWS + threadIdx.x, c), __float_as_uint(t));
-                peer_store(peer_addr(s_sig + rank * FEW_ROWS + threadIdx.x, c), sg);
-                peer_arrive(peer_addr(x_full, c));
-            }
+        for (uint32_t c = threadIdx.x / FEW_ROWS; c < ranks; c += 2 * C::SOFT) {  // to every block of the cluster
+            peer_store(peer_addr(s_top + rank * FEW_ROWS + r, c), (uint32_t)t);
+            peer_store(peer_addr(s_sig + rank * FEW_ROWS + r, c), sg);
+            peer_arrive(peer_addr(x_full, c));
         }
         __syncwarp();
     }
@@ -522,21 +525,21 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
         bool met = wait_cluster(x_full, 0, err, dg::ERR_TIMEOUT_ACCUM);
         ok = __all_sync(0xffffffffu, met && ok);
         if (threadIdx.x < FEW_ROWS) {
-            float t = -INFINITY;
+            int t = (int)s_top[threadIdx.x];
             for (uint32_t c = 0; c < ranks; ++c) {
-                t = fmaxf(t, __uint_as_float(s_top[c * FEW_ROWS + threadIdx.x]));
+                t = max(t, (int)s_top[c * FEW_ROWS + threadIdx.x]);
                 row_sig = max(row_sig, s_sig[c * FEW_ROWS + threadIdx.x]);
             }
             const int e = row_sig ? scale_exp(row_sig >> 16) : 0;
-            s_row[threadIdx.x] = make_float4(t, s_pos[threadIdx.x] >= 0 ? -s_theta[threadIdx.x] : 0.0f, pow2f(-e), pow2f(e));
+            s_row[threadIdx.x] = make_float4(__int_as_float(ordered(t)), s_pos[threadIdx.x] >= 0 ? -s_theta[threadIdx.x] : 0.0f, pow2f(-e), pow2f(e));
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * C::SOFT) : "memory");
         // ── phase 1: the weights and the sums ──
         uint32_t total[FEW_ROWS];  // at most 131072 tiles of one key a thread: below 2^32
 #pragma unroll
         for (int r = 0; r < FEW_ROWS; ++r) total[r] = 0;
-        long long* red = (long long*)(sm + C::RED);
-        // Sums number oc are taken by the group whose tile was the last; thread `key` has column 128 x + key of O.
+        // Sums number oc are taken by the group whose tile was the last; thread `key` has column 128 x + key of O. The 32
+        // columns of a warp's row go to one block of the cluster, the rows and warps round the blocks.
         auto take_sums = [&](uint32_t oc) {
             ok = ok && wait(o_full, oc & 1u, err, dg::ERR_TIMEOUT_ACCUM);
             ok = __all_sync(0xffffffffu, ok);
@@ -549,18 +552,20 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                 for (int r = 0; r < FEW_ROWS; ++r) {
-                    long long* w = red + r * (NK * 128) + x * 128 + key;
-                    *w = (oc ? *w : 0) + (long long)h[r] * 256 + h[16 + r];
+                    if (r >= n_rows) break;
+                    const uint32_t w = r * (NK * 128) + x * 128 + key;
+                    peer_add(peer_addr((long long*)(sm + C::RED) + w, (w >> 5) % ranks),
+                             (uint64_t)((long long)h[r] * 256 + h[16 + r]));
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;");
             __syncwarp();
             if (lane == 0) mbar_arrive(o_free);
         };
-        for (int i = grp; ok && i < n; i += 2) {
+        for (int i = grp; ok && i < n; i += GROUPS) {
             next_scores(i, n + i);
             if (!ok) break;
-            ok = wait(&p_free[i & 1], ((i >> 1) & 1u) ^ 1u, err, dg::ERR_TIMEOUT_EMPTY);
+            ok = i < 2 || block_done(v_block(i - 2));  // the digits of tile i - 2 have been read
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const uint32_t m = seen_rows(tile_at(i) * TILE_KEYS);
@@ -585,52 +590,39 @@ __global__ void __launch_bounds__(FEW_THREADS, 1)
             if (lane == 0) mbar_arrive(&p_full[i & 1]);
             if ((i + 1) % FLUSH_TILES == 0 || i + 1 == n) take_sums((uint32_t)i / FLUSH_TILES);
         }
-        if (n == 0)
-            for (int i = threadIdx.x; i < FEW_ROWS * NK * 128; i += 32 * FEW_SOFT) red[i] = 0;
 #pragma unroll
         for (int r = 0; r < FEW_ROWS; ++r) {
+            if (r >= n_rows) break;
             const unsigned long long lo = __reduce_add_sync(0xffffffffu, total[r] & 0xffffu),
                                      hi = __reduce_add_sync(0xffffffffu, total[r] >> 16);
-            if (lane == 0) s_totals[warp * FEW_ROWS + r] = lo + (hi << 16);
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (threadIdx.x < FEW_ROWS) {
-            unsigned long long t = 0;
-            for (int w = 0; w < FEW_SOFT; ++w) t += s_totals[w * FEW_ROWS + threadIdx.x];
-            s_total[threadIdx.x] = t;
-        }
-        __syncwarp();
-    }
-    cluster_arrive();
-    cluster_wait();
-    if (soft) {
-        // the cluster's sums: each block writes its share of the outputs
-        if (threadIdx.x < FEW_ROWS) {
-            unsigned long long t = 0;
-            for (uint32_t c = 0; c < ranks; ++c) t += peer_u64(peer_addr(s_total + threadIdx.x, c));
-            s_inv[threadIdx.x] = t ? __ddiv_rn(2097152.0, (double)t) : 0.0;
-            const int r = threadIdx.x;
-            if (rank == 0 && r < n_rows && (row0 + r) % g == 0)
-                a.o_scale[((long long)begin + (row0 + r) / g) * a.c.heads + head] =
-                    t ? make_longlong2(1, (long long)(uint32_t)(21 - scale_exp(row_sig >> 16))) : make_longlong2(0, 0);
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        const long long* red = (const long long*)(sm + C::RED);
-        for (int e = (int)(rank * 32 * FEW_SOFT + threadIdx.x); e < n_rows * dim; e += 32 * FEW_SOFT * (int)ranks) {
-            const int r = e / dim, d = e - r * dim;
-            long long v = 0;
-            for (uint32_t c = 0; c < ranks; ++c) v += (long long)peer_u64(peer_addr(red + r * (NK * 128) + d, c));
-            a.o[((long long)begin + (row0 + r) / g) * a.ld_o + (long long)(head * g + (row0 + r) % g) * dim + d] =
-                out_code(v, s_inv[r]);
+            if (lane < (int)ranks) peer_add(peer_addr(s_total + r, lane), lo + (hi << 16));
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;");
     __syncwarp();
     cluster_arrive();
-    cluster_wait();  // nobody leaves while its sums are being read
+    cluster_wait();  // all sums are in; nobody touches another block's memory from here on
+    if (soft) {
+        if (threadIdx.x < FEW_ROWS) {
+            const int r = threadIdx.x;
+            const unsigned long long t = s_total[r];
+            s_inv[r] = t ? __ddiv_rn(2097152.0, (double)t) : 0.0;
+            if (rank == 0 && r < n_rows && (row0 + r) % g == 0)
+                a.o_scale[((long long)begin + (row0 + r) / g) * a.c.heads + head] =
+                    t ? make_longlong2(1, (long long)(uint32_t)(21 - scale_exp(row_sig >> 16))) : make_longlong2(0, 0);
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * C::SOFT) : "memory");
+        const long long* red = (const long long*)(sm + C::RED);
+        for (uint32_t w = rank + ranks * (uint32_t)warp; w < (uint32_t)(n_rows * NK * 4); w += ranks * C::SOFT) {
+            const int r = (int)w / (NK * 4), d = (int)(w % (NK * 4)) * 32 + lane;
+            if (d < dim)
+                a.o[((long long)begin + (row0 + r) / g) * a.ld_o + (long long)(head * g + (row0 + r) % g) * dim + d] =
+                    out_code(red[w * 32 + lane], s_inv[r]);
+        }
+    }
     if (warp == 0) {
         asm volatile("tcgen05.fence::after_thread_sync;");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::COLS));
     }
 }
 
