@@ -11,8 +11,9 @@
 // the cluster exchanges its maxima, V is already on its way. Sums over the keys are integers, so the shares of a cluster
 // add up to the same bits in any order: each block adds its own into the shared memory of the block that writes them out.
 //
-// A block's start, exchange and end are latency (10 us of a block's 26 at 12 tiles), so where the sequences are not so
-// long that the scores of a block need all of TMEM, two blocks share an SM, one's waits under the other's stream.
+// A block's start, exchange and end are latency (10 us of a block's 26 at 12 tiles), so two blocks share an SM, one's waits
+// under the other's stream, although each then has room for the scores of 12 tiles only (28 alone): four sequences of
+// 65536 keys take 155 us, against 264 with one block an SM and every score kept.
 //
 // Roles: softmax warps, in one or two groups of four that take the tiles in turn; then one warp each for TMA, the
 // products and the keys' scales.
@@ -29,12 +30,12 @@ template <int NK, int PER_SM>
 struct FewCfg {
     static constexpr int SLOT = TILE_KEYS * 128;
     static constexpr int SLOTS = 8 / PER_SM;
-    static constexpr int SOFT = 8 / PER_SM;  // softmax warps
+    static constexpr int SOFT = 8;  // softmax warps
     static constexpr int THREADS = 32 * (SOFT + 3);
     static constexpr int COLS = 512 / PER_SM;  // of TMEM
     static constexpr int SCALES = 4;
     static constexpr int SUMS = COLS - 32 * NK;        // O^T of each 128 columns: 16 hi, 16 lo
-    static constexpr int KEEP = (SUMS - 32) / 16;      // tiles whose scores stay in TMEM: 28, 26 (NK 2), 12 (PER_SM 2)
+    static constexpr int KEEP = (SUMS - 32) / 16;      // tiles whose scores stay in TMEM: 12 (NK 1, PER_SM 2), 26 (NK 2, PER_SM 1)
     static constexpr int AGAIN = 16 * KEEP;            // two more score buffers, for the others
     static constexpr int RING = 0;
     static constexpr int Q = RING + SLOTS * SLOT;               // [NK][16 rows][128]
@@ -44,7 +45,7 @@ struct FewCfg {
     static constexpr int ROWS = KEY_SCALES + SCALES * 2 * TILE_KEYS * 4;
     // per row: theta; position; max and largest sigma of each warp and of each block of the cluster; total of the cluster;
     // the row's (max, -theta, 2^-E, 2^E); 2^21 / L
-    static constexpr int BARS = ROWS + FEW_ROWS * (4 + 4 + 64 + 128 + 8 + 16 + 8);
+    static constexpr int BARS = ROWS + FEW_ROWS * (4 + 4 + 64 + 64 + 8 + 16 + 8);
     static constexpr int BYTES = 1024 + BARS + 512;
     static_assert(AGAIN + 32 <= SUMS, "TMEM columns");
     static_assert(PER_SM * (BYTES + 1024) <= 233472, "shared memory of an SM");
@@ -119,9 +120,9 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
     double* s_inv = (double*)(s_total + FEW_ROWS);
     int* s_tops = (int*)(s_inv + FEW_ROWS);                   // [8 warps][16]
     uint32_t* s_sigs = (uint32_t*)(s_tops + 8 * FEW_ROWS);    // [8 warps][16]
-    uint32_t* s_top = s_sigs + 8 * FEW_ROWS;                  // [16 ranks][16], written by the ranks
-    uint32_t* s_sig = s_top + 16 * FEW_ROWS;                  // [16 ranks][16]
-    float* s_theta = (float*)(s_sig + 16 * FEW_ROWS);
+    uint32_t* s_top = s_sigs + 8 * FEW_ROWS;                  // [8 ranks][16], written by the ranks
+    uint32_t* s_sig = s_top + 8 * FEW_ROWS;                  // [8 ranks][16]
+    float* s_theta = (float*)(s_sig + 8 * FEW_ROWS);
     int* s_pos = (int*)(s_theta + FEW_ROWS);
     uint64_t* full = (uint64_t*)(sm + C::BARS);  // [SLOTS]
     // [SLOTS] the products of a block are done: its slot is free, the scores of its tile are there (K), the digits of its

@@ -2,7 +2,6 @@
 // over the cache. All on device buffers, ordered on the caller's stream, nothing allocated and no workspace kept, so
 // calls on several streams and captured graphs share nothing but the caller's own buffers.
 
-#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -103,12 +102,13 @@ int launch_tile(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
     return KTMOE_OK;
 }
 
-// Blocks of a cluster: twice as many while the blocks do not fill the GPU and each would keep two tiles or more, and while
-// over a third of a block's tiles would have their scores formed twice (as far as the page table tells: the lengths are
-// on the device).
-int few_cluster(const ktmoe_ctx* ctx, int64_t tiles, int64_t jobs, int keep) {
+// Blocks of a cluster: twice as many while they do not fill the GPU and each would keep two tiles or more (as far as the
+// page table tells: the lengths are on the device). Clusters of 16 leave SMs of a GPC idle: four sequences of 65536 keys
+// by 8 KV heads took 211 us in sixteens, 155 in eights, 240 in fours; a batch that fills the GPU by itself, 64 sequences of
+// 4096, 127 us in ones, 121 in twos, 162 in fours.
+int few_cluster(const ktmoe_ctx* ctx, int64_t tiles, int64_t jobs, int per_sm) {
     int c = 1;
-    while (c < 16 && tiles >= 4 * c && (jobs * c < ctx->num_sms || 2 * tiles > 3 * keep * c)) c *= 2;
+    while (c < 8 && tiles >= 2 * c && jobs * c < (int64_t)per_sm * ctx->num_sms) c *= 2;
     return c;
 }
 
@@ -119,30 +119,10 @@ int launch_few(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
     static bool attr_set[64] = {};
     if (!attr_set[ctx->device & 63]) {
         CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
-        CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         attr_set[ctx->device & 63] = true;
     }
     const int64_t jobs = (a.b.rows * a.group / kv::FEW_ROWS + a.b.n_seqs) * a.c.heads;
-    int c = few_cluster(ctx, ((int64_t)a.b.max_pages << a.c.page_shift) / kv::TILE_KEYS, jobs, C::KEEP);
-    static int most[64] = {};  // the largest cluster that fits this device at this kernel's shared memory
-    int& top = most[ctx->device & 63];
-    for (int t = 16; top == 0; t /= 2) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)t);
-        cfg.blockDim = dim3(C::THREADS);
-        cfg.dynamicSmemBytes = C::BYTES;
-        cudaLaunchAttribute at[1];
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = (unsigned)t;
-        at[0].val.clusterDim.y = 1;
-        at[0].val.clusterDim.z = 1;
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-        int n = 0;
-        if (t == 1 || (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0)) top = t;
-        cudaGetLastError();
-    }
-    c = std::min(c, top);
+    const int c = few_cluster(ctx, ((int64_t)a.b.max_pages << a.c.page_shift) / kv::TILE_KEYS, jobs, PER_SM);
     if (jobs * c > INT32_MAX) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "too many query rows for one launch");
     CUtensorMap mk, mv;
     if (int r = make_pool_map(ctx, &mk, a.c.k, a.c)) return r;
@@ -256,10 +236,7 @@ int ktmoe_attention_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe
     // few rows a sequence: bound by the keys' and values' bytes; many: by the arithmetic on the scores
     if ((int64_t)a.group * batch->rows > (int64_t)2 * kv::FEW_ROWS * batch->n_seqs)
         return a.c.dim <= 128 ? launch_tile<1>(ctx, st, a) : launch_tile<2>(ctx, st, a);
-    // two blocks an SM where the scores of 16 blocks hold two thirds of the longest sequence's tiles, or more
-    if (a.c.dim > 128) return launch_few<2, 1>(ctx, st, a);
-    const int64_t tiles = ((int64_t)a.b.max_pages << a.c.page_shift) / kv::TILE_KEYS;
-    return 2 * tiles <= 3 * 16 * kv::FewCfg<1, 2>::KEEP ? launch_few<1, 2>(ctx, st, a) : launch_few<1, 1>(ctx, st, a);
+    return a.c.dim <= 128 ? launch_few<1, 2>(ctx, st, a) : launch_few<2, 1>(ctx, st, a);
 }
 
 }  // extern "C"
