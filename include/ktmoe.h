@@ -295,15 +295,15 @@ typedef struct ktmoe_rope {
 int ktmoe_rope_table(double theta, int32_t rot_dim, int64_t positions, int32_t* table);
 
 /* Write the batch's new keys and values: k, v [rows][n_kv_heads][head_dim] int32 codes with row strides ld_k and ld_v
- * (in elements) at scale[row * scale_stride] (scale_stride 1: a scale per row; 0: one for all), keys rotated when rope
- * is not NULL. With y a row's codes after the rotation and s its scale (2^-30 of it after a rotation):
+ * (in elements) at k_scale[row * scale_stride] and v_scale[row * scale_stride] (NULL v_scale: as the keys; scale_stride
+ * 1: a scale per row; 0: one for all), keys rotated when rope is not NULL. With y a row's codes after the rotation and s its scale (2^-30 of it after a rotation):
  * t = RN64(RN64(max|y| s) / 127) held within [2^-64, 2^63], sigma = t rounded up to 8 significant bits, codes
  * rne(RN64(y RN64(s / sigma))) held within +-127. A scale's shift counts as at least -900 and at most 2000, here and in
  * ktmoe_attention_dev. Stream-ordered (NULL: the context stream), not synchronised. Two
  * rows of one call must not share a place in the cache. */
 int ktmoe_kv_append_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* k,
-                        int64_t ld_k, const int32_t* v, int64_t ld_v, const ktmoe_scale* scale, int32_t scale_stride,
-                        const ktmoe_rope* rope, void* stream);
+                        int64_t ld_k, const int32_t* v, int64_t ld_v, const ktmoe_scale* k_scale,
+                        const ktmoe_scale* v_scale, int32_t scale_stride, const ktmoe_rope* rope, void* stream);
 /* Read the same rows back: k, v [rows][n_kv_heads][head_dim] f32, code * sigma (exact). A whole sequence is read with
  * q_begin spanning its kv_len tokens. */
 int ktmoe_kv_read_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, float* k, int64_t ld_k,
@@ -322,6 +322,38 @@ int ktmoe_attention_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe
                         int64_t ld_q, const ktmoe_scale* scale, int32_t scale_stride, const ktmoe_rope* rope,
                         int32_t n_heads, double softmax_scale, int32_t window, int32_t sinks, int32_t* o, int64_t ld_o,
                         ktmoe_scale* o_scale, void* stream);
+
+/* ── the attention half of a decoder block (the reference's attention.rs and sdpa.rs have its place in the block,
+ * model.rs:175-181; the cache and the softmax are this library's definitions above) ──
+ * y = add(x, o(attention(q, k, v))) with q, k, v = the linears of rms_norm(x): the RmsNorm and the residual add of
+ * ktmoe_block_forward (over all rows), each linear as QuantLinear::forward_int on every row by itself
+ * (layers.rs:275-328), the heads' outputs and then the rows merged into one tensor at one scale as the experts' are
+ * (layers.rs:1001-1019). Rows of the batch that belong to no sequence get no attention (their y is x, requantised). */
+typedef struct ktmoe_attn ktmoe_attn;
+typedef struct ktmoe_attn_config {
+    int32_t d_model;
+    int32_t n_heads;    /* a multiple of n_kv_heads */
+    int32_t n_kv_heads;
+    int32_t head_dim;   /* a multiple of 16 from 16 to 256 */
+} ktmoe_attn_config;
+int ktmoe_attn_create(ktmoe_ctx* ctx, const ktmoe_attn_config* cfg, ktmoe_attn** out);
+int ktmoe_attn_destroy(ktmoe_attn* attn);
+/* Codes and scales of QuantLinear::from_weights: q [n_heads * head_dim][d_model], k and v [n_kv_heads * head_dim]
+ * [d_model], out [d_model][n_heads * head_dim]; the norm's as for ktmoe_layer_set_norm. Host pointers. */
+int ktmoe_attn_set_qkv(ktmoe_attn* attn, const int32_t* q, ktmoe_scale q_scale, const int32_t* k, ktmoe_scale k_scale,
+                       const int32_t* v, ktmoe_scale v_scale);
+int ktmoe_attn_set_out(ktmoe_attn* attn, const int32_t* out, ktmoe_scale out_scale);
+int ktmoe_attn_set_norm(ktmoe_attn* attn, const int32_t* w_codes, ktmoe_scale w_scale, ktmoe_scale eps_scale);
+/* Rotary positions (ktmoe_rope_table's table, made and kept here); positions 0 turns them off. */
+int ktmoe_attn_set_rope(ktmoe_attn* attn, double theta, int32_t rot_dim, int64_t positions, int32_t interleaved);
+/* softmax_scale 0: head_dim^-1/2. window, sinks as for ktmoe_attention_dev. */
+int ktmoe_attn_set_mask(ktmoe_attn* attn, double softmax_scale, int32_t window, int32_t sinks);
+/* The half on device buffers x, y [batch->rows][d_model] with their scales (x may be y), stream-ordered and not
+ * synchronised; the new keys and values go into `cache` before the attention reads it. The object's scratch serves one
+ * forward at a time (order calls that share it) and grows with the rows (not while a stream is captured). */
+int ktmoe_attn_forward_dev(ktmoe_attn* attn, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch,
+                           const int32_t* x_dev, const ktmoe_scale* x_scale_dev, int32_t* y_dev,
+                           ktmoe_scale* y_scale_dev, void* stream);
 
 /* ── host-side, offline preparation (f64, as the reference does it once on the host) ── */
 int ktmoe_quantize_weights(const float* w, int64_t n, int32_t* codes, ktmoe_scale* scale);

@@ -54,9 +54,10 @@ def rows_of(begin, kv_len):
             yield t, b, int(kv_len[b]) - (begin[b + 1] - t)
 
 
-def append(k, v, scale, begin, kv_len, write, table=None, interleaved=False):
-    """Calls write(which, sequence, position, head, codes, sigma) for each new row; k, v: [rows][heads][dim]; scale:
-    [rows][2] or [2]."""
+def append(k, v, scale, begin, kv_len, write, table=None, interleaved=False, v_scale=None):
+    """Calls write(which, sequence, position, head, codes, sigma) for each new row; k, v: [rows][heads][dim]; scale (and
+    v_scale, when the values have their own): [rows][2] or [2]."""
+    v_scale = scale if v_scale is None else v_scale
     for t, b, pos in rows_of(begin, kv_len):
         if pos < 0:
             continue
@@ -64,7 +65,7 @@ def append(k, v, scale, begin, kv_len, write, table=None, interleaved=False):
         for h in range(k.shape[1]):
             y, f = rotate(k[t, h], None if table is None else table[pos], interleaved)
             write("k", b, pos, h, *quantise_row(y, s * f))
-            write("v", b, pos, h, *quantise_row(v[t, h].astype(np.int64), s))
+            write("v", b, pos, h, *quantise_row(v[t, h].astype(np.int64), value(v_scale[t] if np.ndim(v_scale) == 2 else v_scale)))
 
 
 def weights(dots, sigma_k, theta):

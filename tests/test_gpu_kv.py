@@ -132,9 +132,11 @@ def test_append_and_read(ctx, case):
     scale[-4] = (0, 5)
     table = None if rot is None else tb.rope_table(1e4, rot[0], max(kv for _, kv in lens) + 1)
     rope = None if rot is None else tb.Rope(torch.from_numpy(table).cuda(), rot[1])
+    v_scale = s.scales(20, 50) if dim % 32 == 0 else None
     R.append(k.reshape(s.rows, hk, dim), v.reshape(s.rows, hk, dim), scale, s.begin, s.kv_len, s.write, table,
-             rot is not None and rot[1])
-    s.cache.append(s.batch, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), torch.from_numpy(scale).cuda(), rope)
+             rot is not None and rot[1], v_scale)
+    s.cache.append(s.batch, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), torch.from_numpy(scale).cuda(), rope,
+                   v_scale=None if v_scale is None else torch.from_numpy(v_scale).cuda())
     ko, vo = (torch.full((s.rows, hk * dim), -5.0, device="cuda") for _ in range(2))
     s.cache.read(s.batch, ko, vo)
     ctx.sync()
@@ -546,11 +548,12 @@ def test_refusals_of_the_c_entry_points(ctx):
     c3 = cache(n_kv_heads=3)
     assert attend(c=c3) == ARG  # two query heads over three KV heads
     a = [ctx.handle, cache(), batch()]
-    assert L.ktmoe_kv_append_dev(*a, q.data_ptr(), 15, q.data_ptr(), 16, sc.data_ptr(), 1, None, None) == ARG
-    assert L.ktmoe_kv_append_dev(*a, q.data_ptr(), 16, q.data_ptr(), 15, sc.data_ptr(), 1, None, None) == ARG
-    assert L.ktmoe_kv_append_dev(*a, None, 16, q.data_ptr(), 16, sc.data_ptr(), 1, None, None) == ARG
-    assert L.ktmoe_kv_append_dev(*a, q.data_ptr(), 16, q.data_ptr(), 16, None, 1, None, None) == ARG
-    assert L.ktmoe_kv_append_dev(*a, q.data_ptr(), 16, q.data_ptr(), 16, sc.data_ptr(), 1, rope(rot_dim=5), None) == ARG
+    assert L.ktmoe_kv_append_dev(*a, q.data_ptr(), 15, q.data_ptr(), 16, sc.data_ptr(), None, 1, None, None) == ARG
+    assert L.ktmoe_kv_append_dev(*a, q.data_ptr(), 16, q.data_ptr(), 15, sc.data_ptr(), None, 1, None, None) == ARG
+    assert L.ktmoe_kv_append_dev(*a, None, 16, q.data_ptr(), 16, sc.data_ptr(), None, 1, None, None) == ARG
+    assert L.ktmoe_kv_append_dev(*a, q.data_ptr(), 16, q.data_ptr(), 16, None, None, 1, None, None) == ARG
+    assert L.ktmoe_kv_append_dev(*a, q.data_ptr(), 16, q.data_ptr(), 16, sc.data_ptr(), sc.data_ptr() + 8, 1, None, None) == ARG
+    assert L.ktmoe_kv_append_dev(*a, q.data_ptr(), 16, q.data_ptr(), 16, sc.data_ptr(), None, 1, rope(rot_dim=5), None) == ARG
     assert L.ktmoe_kv_read_dev(*a, o.data_ptr(), 16, None, 16, None) == ARG
     assert L.ktmoe_kv_read_dev(*a, o.data_ptr(), 12, o.data_ptr(), 16, None) == ARG
     torch.cuda.synchronize()

@@ -26,7 +26,7 @@ from typing import Callable, List, Optional, Sequence
 import numpy as np
 
 from . import _native
-from ._native import KtmoeError, KtmoeLayerConfig, KtmoeScale, check, lib
+from ._native import KtmoeAttnConfig, KtmoeError, KtmoeLayerConfig, KtmoeScale, check, lib
 from .kv_cache import KvBatch, KvCache, Rope, rope_table
 
 __all__ = [
@@ -34,7 +34,7 @@ __all__ = [
     "B200Linear", "Context", "DeviceLayer", "LayerSlot", "MoeStack", "device_count", "synth_normal", "synth_normal_portable", "lcg_uniform", "table",
     "route_margins", "hash_int", "repro_hash",
     "KtmoeError",
-    "ep_unique_id", "KvCache", "KvBatch", "Rope", "rope_table",
+    "ep_unique_id", "KvCache", "KvBatch", "Rope", "rope_table", "AttentionHalf",
 ]
 
 WLEVELS = 265720  # (3^12 - 1) / 2, layers.rs:16
@@ -794,15 +794,77 @@ class LayerSlot:
         self.dev.forward_dev(x_ptr, rows, x_scale_ptr, y_ptr, y_scale_ptr, stream)
 
 
+class AttentionHalf:
+    """The attention half of a decoder block on a device (ktmoe_attn): x ← add(x, o(attention(q, k, v))) with q, k, v the
+    linears of rms_norm(x), rotary positions, and a :class:`KvCache` that holds the sequences. Set the weights (QuantLinear
+    codes and scales) once; each forward writes the new tokens' keys and values into the cache and attends over it."""
+
+    def __init__(self, ctx: Context, d_model: int, n_heads: int, n_kv_heads: int, head_dim: int):
+        self.ctx, self.d_model = ctx, int(d_model)
+        self.n_heads, self.n_kv_heads, self.head_dim = int(n_heads), int(n_kv_heads), int(head_dim)
+        cfg = KtmoeAttnConfig(self.d_model, self.n_heads, self.n_kv_heads, self.head_dim)
+        h = ctypes.c_void_p()
+        ctx.check(lib().ktmoe_attn_create(ctx.handle, ctypes.byref(cfg), ctypes.byref(h)))
+        self._h = h
+
+    def __del__(self):
+        try:
+            if self._h:
+                lib().ktmoe_attn_destroy(self._h)
+                self._h = None
+        except Exception:
+            pass
+
+    def _codes(self, lin: QuantLinear, out: int, k: int, name: str):
+        if lin.out_features != out or lin.in_features != k or lin.bias is not None:
+            raise ValueError(f"{name}: a [{out}, {k}] linear without a bias")
+        return _p(lin.w_codes, ctypes.c_int32), lin.w_scale._c()
+
+    def set_qkv(self, q: QuantLinear, k: QuantLinear, v: QuantLinear) -> None:
+        d, w, kv = self.d_model, self.n_heads * self.head_dim, self.n_kv_heads * self.head_dim
+        self.ctx.check(lib().ktmoe_attn_set_qkv(self._h, *self._codes(q, w, d, "q"), *self._codes(k, kv, d, "k"),
+                                                *self._codes(v, kv, d, "v")))
+
+    def set_out(self, out: QuantLinear) -> None:
+        self.ctx.check(lib().ktmoe_attn_set_out(self._h, *self._codes(out, self.d_model, self.n_heads * self.head_dim, "out")))
+
+    def set_norm(self, w_codes: np.ndarray, w_scale: Scale, eps_scale: Scale) -> None:
+        """The half's input RmsNorm (RmsNorm::new codes and scales)."""
+        w = np.ascontiguousarray(w_codes, dtype=np.int32).reshape(-1)
+        if w.size != self.d_model:
+            raise ValueError("the norm has d_model codes")
+        self.ctx.check(lib().ktmoe_attn_set_norm(self._h, _p(w, ctypes.c_int32), w_scale._c(), eps_scale._c()))
+
+    def set_rope(self, theta: float, rot_dim: int, positions: int, interleaved: bool = False) -> None:
+        """Rotary positions below ``positions`` (0: none)."""
+        self.ctx.check(lib().ktmoe_attn_set_rope(self._h, float(theta), int(rot_dim), int(positions), 1 if interleaved else 0))
+
+    def set_mask(self, window: int = 0, sinks: int = 0, softmax_scale: float = 0.0) -> None:
+        """A sliding window with the first ``sinks`` positions kept; softmax_scale 0: head_dim ** -0.5."""
+        self.ctx.check(lib().ktmoe_attn_set_mask(self._h, float(softmax_scale), int(window), int(sinks)))
+
+    def forward_dev(self, cache: KvCache, batch: KvBatch, x_ptr: int, x_scale_ptr: int, y_ptr: int, y_scale_ptr: int,
+                    stream: int = 0) -> None:
+        """Device buffers [batch.rows][d_model] (raw pointers), stream-ordered, not synchronised."""
+        if cache.ctx is not self.ctx:
+            raise ValueError("the cache lies on another context")
+        self.ctx.check(lib().ktmoe_attn_forward_dev(self._h, cache._c, batch._c, ctypes.c_void_p(x_ptr),
+                                                    ctypes.c_void_p(x_scale_ptr), ctypes.c_void_p(y_ptr),
+                                                    ctypes.c_void_p(y_scale_ptr),
+                                                    ctypes.c_void_p(stream) if stream else None))
+
+
 class MoeStack:
-    """A stack of MoE decoder-block FFN halves with attention excluded (the shape of a GLM-4.5-Air-style model's 45
-    MoE layers): for each layer l, x ← add(x, moe_l(rms_norm_l(x))) (kt-core model.rs:175-181), the residual stream
-    staying on the device between layers in two ping-pong buffers. Every layer is a :class:`DeviceLayer` with its norm
+    """A stack of MoE decoder blocks (kt-core model.rs:175-181), the residual stream staying on the device between layers
+    in ping-pong buffers: for each layer l its FFN half x ← add(x, moe_l(rms_norm_l(x))), and before it, with
+    ``attention``, its attention half (:class:`AttentionHalf`) over the layer's own cache; without, attention is excluded
+    (the shape of a GLM-4.5-Air-style model's 45 MoE layers). Every layer is a :class:`DeviceLayer` with its norm
     set (``set_norm``), all on one context; each layer's block is one ``ktmoe_block_forward_dev`` on that context's
     stream (with the layer's CUDA graphs when enabled: the buffers a layer sees are the same on every call)."""
 
-    def __init__(self, layers: Sequence):
-        """``layers``: DeviceLayers, or the LayerSlots of one DeviceLayer with several weight slots."""
+    def __init__(self, layers: Sequence, attention: Optional[Sequence] = None, caches: Optional[Sequence] = None):
+        """``layers``: DeviceLayers, or the LayerSlots of one DeviceLayer with several weight slots. ``attention``: an
+        AttentionHalf for each layer (one may serve several), ``caches``: a KvCache for each."""
         if not layers:
             raise ValueError("a stack needs at least one layer")
         self.layers = list(layers)
@@ -810,33 +872,55 @@ class MoeStack:
         self.d_model = self.layers[0].d_model
         if any(L.ctx is not self.ctx or L.d_model != self.d_model for L in self.layers):
             raise ValueError("the layers of a stack share one context and one d_model")
+        self.attention = list(attention) if attention is not None else None
+        self.caches = list(caches) if caches is not None else None
+        if (self.attention is None) != (self.caches is None):
+            raise ValueError("attention halves and caches come together")
+        if self.attention is not None:
+            if len(self.attention) != len(self.layers) or len(self.caches) != len(self.layers):
+                raise ValueError("a stack with attention has an attention half and a cache for every layer")
+            if any(a.ctx is not self.ctx or a.d_model != self.d_model for a in self.attention):
+                raise ValueError("the attention halves of a stack share its context and d_model")
+            if len({id(c) for c in self.caches}) != len(self.caches):
+                raise ValueError("every layer has a cache of its own")
         self._bufs = None
 
     def _buffers(self, rows: int):
-        """Four int32 [rows·d] buffers and their scales: the input, two ping-pong, the output. Kept across calls, so a
-        layer sees the same pointers every time (its CUDA graphs are reused)."""
+        """Five int32 [rows·d] buffers and their scales: the input, two ping-pong, the output, the attention half's.
+        Kept across calls, so a layer sees the same pointers every time (its CUDA graphs are reused)."""
         import torch  # device memory for the residual stream (plumbing only)
 
         if self._bufs is None or self._bufs[0] < rows:
             dev = torch.device("cuda", self.ctx.device)
             n = max(1, rows) * self.d_model
-            self._bufs = (rows, [torch.empty(n, dtype=torch.int32, device=dev) for _ in range(4)],
-                          [torch.zeros(2, dtype=torch.int64, device=dev) for _ in range(4)])
+            self._bufs = (rows, [torch.empty(n, dtype=torch.int32, device=dev) for _ in range(5)],
+                          [torch.zeros(2, dtype=torch.int64, device=dev) for _ in range(5)])
         return self._bufs
 
-    def forward_dev(self, x_ptr: int, rows: int, x_scale_ptr: int, y_ptr: int, y_scale_ptr: int) -> None:
+    def _check_batch(self, rows: int, batch: Optional[KvBatch]) -> None:
+        if (batch is None) != (self.attention is None):
+            raise ValueError("a stack with attention takes a batch of sequences, one without takes none")
+        if batch is not None and batch.rows != rows:
+            raise ValueError("the batch's rows are not the input's")
+
+    def forward_dev(self, x_ptr: int, rows: int, x_scale_ptr: int, y_ptr: int, y_scale_ptr: int,
+                    batch: Optional[KvBatch] = None) -> None:
         """Device buffers (raw pointers; a Scale is 16 bytes {i64 mant, i32 shift}); ordered on the context's stream,
-        not synchronised."""
+        not synchronised. ``batch``: where the rows stand in their sequences (a stack with attention)."""
+        self._check_batch(rows, batch)
         _, xb, sb = self._buffers(rows)
         src, src_s = x_ptr, x_scale_ptr
         for i, L in enumerate(self.layers):
             last = i == len(self.layers) - 1
+            if self.attention is not None:
+                self.attention[i].forward_dev(self.caches[i], batch, src, src_s, xb[4].data_ptr(), sb[4].data_ptr())
+                src, src_s = xb[4].data_ptr(), sb[4].data_ptr()
             dst = y_ptr if last else xb[1 + i % 2].data_ptr()
             dst_s = y_scale_ptr if last else sb[1 + i % 2].data_ptr()
             L.block_forward_dev(src, rows, src_s, dst, dst_s)
             src, src_s = dst, dst_s
 
-    def forward(self, x: IntTensor) -> IntTensor:
+    def forward(self, x: IntTensor, batch: Optional[KvBatch] = None) -> IntTensor:
         """Host tensors in and out (synchronous)."""
         import torch
 
@@ -844,12 +928,13 @@ class MoeStack:
         if len(x) % d != 0:
             raise ValueError("stack input length must be a multiple of d_model")
         rows = len(x) // d
+        self._check_batch(rows, batch)
         _, xb, sb = self._buffers(rows)
         n = rows * d
         xb[0][:n].copy_(torch.from_numpy(np.ascontiguousarray(x.data, dtype=np.int32)))
         sb[0].copy_(torch.tensor([x.scale.mant, x.scale.shift & 0xFFFFFFFF], dtype=torch.int64))
         torch.cuda.synchronize(xb[0].device)  # the uploads ran on torch's stream; the layers run on the context's
-        self.forward_dev(xb[0].data_ptr(), rows, sb[0].data_ptr(), xb[3].data_ptr(), sb[3].data_ptr())
+        self.forward_dev(xb[0].data_ptr(), rows, sb[0].data_ptr(), xb[3].data_ptr(), sb[3].data_ptr(), batch)
         self.ctx.sync()
         y = xb[3][:n].cpu().numpy().copy()
         s = sb[3].cpu().numpy()

@@ -57,6 +57,11 @@ class KtmoeKvBatch(ctypes.Structure):
     ]
 
 
+class KtmoeAttnConfig(ctypes.Structure):
+    _fields_ = [("d_model", ctypes.c_int32), ("n_heads", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32)]
+
+
 class KtmoeRope(ctypes.Structure):
     _fields_ = [
         ("table", ctypes.c_void_p),
@@ -129,11 +134,19 @@ SIGNATURES = {
     "ktmoe_table": ([_i32, _i64p, _P(KtmoeScale), _i64p, _P(KtmoeScale)], ctypes.c_int),
     "ktmoe_synth_normal": ([_u64, ctypes.c_float, _u64, _i64, _f32p], ctypes.c_int),
     "ktmoe_rope_table": ([ctypes.c_double, _i32, _i64, _i32p], ctypes.c_int),
-    "ktmoe_kv_append_dev": ([_vp, _P(KtmoeKvCache), _P(KtmoeKvBatch), _vp, _i64, _vp, _i64, _vp, _i32, _P(KtmoeRope),
-                             _vp], ctypes.c_int),
+    "ktmoe_kv_append_dev": ([_vp, _P(KtmoeKvCache), _P(KtmoeKvBatch), _vp, _i64, _vp, _i64, _vp, _vp, _i32,
+                             _P(KtmoeRope), _vp], ctypes.c_int),
     "ktmoe_kv_read_dev": ([_vp, _P(KtmoeKvCache), _P(KtmoeKvBatch), _vp, _i64, _vp, _i64, _vp], ctypes.c_int),
     "ktmoe_attention_dev": ([_vp, _P(KtmoeKvCache), _P(KtmoeKvBatch), _vp, _i64, _vp, _i32, _P(KtmoeRope), _i32,
                              ctypes.c_double, _i32, _i32, _vp, _i64, _vp, _vp], ctypes.c_int),
+    "ktmoe_attn_create": ([_vp, _P(KtmoeAttnConfig), _P(_vp)], ctypes.c_int),
+    "ktmoe_attn_destroy": ([_vp], ctypes.c_int),
+    "ktmoe_attn_set_qkv": ([_vp, _i32p, KtmoeScale, _i32p, KtmoeScale, _i32p, KtmoeScale], ctypes.c_int),
+    "ktmoe_attn_set_out": ([_vp, _i32p, KtmoeScale], ctypes.c_int),
+    "ktmoe_attn_set_norm": ([_vp, _i32p, KtmoeScale, KtmoeScale], ctypes.c_int),
+    "ktmoe_attn_set_rope": ([_vp, ctypes.c_double, _i32, _i64, _i32], ctypes.c_int),
+    "ktmoe_attn_set_mask": ([_vp, ctypes.c_double, _i32, _i32], ctypes.c_int),
+    "ktmoe_attn_forward_dev": ([_vp, _P(KtmoeKvCache), _P(KtmoeKvBatch), _vp, _vp, _vp, _vp, _vp], ctypes.c_int),
     "ktmoe_lcg_uniform": ([_u64, _i64, _i64, _i64, _i32p], ctypes.c_int),
 }
 

@@ -21,7 +21,7 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES_CU = ["ktmoe.cu", "kv_cache.cu", "noalloc.cu"]
 SOURCES_CPP = ["host_prep.cpp", "wire.cpp"]
 KV_HEADERS = ["kv_kernels.cuh", "kv_attend_few.cuh", "kv_attend_tile.cuh"]  # of kv_cache.cu alone
-HEADERS = ["context.cuh", "fixed_point.cuh", "digit_gemm.cuh", "digit_gemm_pair.cuh", "moe_kernels.cuh", "ep_peer.cuh", "synth.cuh",
+HEADERS = ["context.cuh", "kv_host.h", "fixed_point.cuh", "digit_gemm.cuh", "digit_gemm_pair.cuh", "moe_kernels.cuh", "ep_peer.cuh", "synth.cuh",
            "host_prep.h"]
 
 

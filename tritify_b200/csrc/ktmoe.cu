@@ -14,6 +14,7 @@
 #include <nccl.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -30,6 +31,7 @@
 #include "fixed_point.cuh"
 #include "host_prep.h"
 #include "ktmoe.h"
+#include "kv_host.h"
 #include "moe_kernels.cuh"
 #include "synth.cuh"
 
@@ -3214,6 +3216,282 @@ int ktmoe_lcg_uniform(uint64_t seed, int64_t lo, int64_t hi, int64_t n, int32_t*
     if (n < 0 || (n > 0 && !out) || hi < lo) return KTMOE_ERR_ARG;
     hp::lcg_uniform(seed, lo, hi, (size_t)n, out);
     return KTMOE_OK;
+}
+
+}  // extern "C"
+
+// ───────────────────────────── the attention half of a decoder block ─────────────────────────────
+
+struct ktmoe_attn {
+    ktmoe_ctx* ctx = nullptr;
+    ktmoe_attn_config cfg{};
+    int64_t d = 0, q = 0, kv = 0;  // widths: d_model, n_heads * head_dim, n_kv_heads * head_dim
+    Planes w_qkv, w_out;
+    DevBuf b_qkv, b_out, b_norm, b_rope;
+    Scale q_ws{0, 0}, k_ws{0, 0}, v_ws{0, 0}, out_ws{0, 0}, norm_ws{0, 0}, norm_eps{0, 0};
+    bool qkv_set = false, out_set = false, norm_set = false;
+    ktmoe_rope rope{nullptr, 0, 0, 0};
+    double softmax_scale = 0.0;
+    int32_t window = 0, sinks = 0;
+    // scratch for `cap` rows
+    int64_t cap = 0;
+    DevBuf c_rows, xn, planes, xmax, sqx, acc, qkv, qkv_scale, o, o_scale, merged, out, out_scale, m, scal;
+};
+
+namespace {
+
+// Scalars of a forward: Scales, then u64 words.
+enum AttnScale { A_NORM = 0, A_XN = 2, A_HEADS = 3, A_MERGED = 5, A_ROWS = 6, A_M = 8, A_ADD = 9, A_NSCALES = 12 };
+enum AttnWord { AU_NORM = 0, AU_HEADS, AU_ROWS, AU_ADD, AU_N };
+
+int attn_scratch(ktmoe_attn* A, int64_t T) {
+    ktmoe_ctx* ctx = A->ctx;
+    if (T <= A->cap) return KTMOE_OK;
+    const int64_t T_pad = round_up(T, 64), w = A->q + 2 * A->kv;
+    const int64_t k_pad = std::max(A->w_qkv.k_pad, A->w_out.k_pad);
+    CK(A->c_rows.ensure(T * sizeof(Scale)));
+    CK(A->xn.ensure(T * A->d * 4));
+    CK(A->planes.ensure(3 * T_pad * k_pad));
+    CK(A->xmax.ensure(T * 8));
+    CK(A->sqx.ensure(T * sizeof(Scale)));
+    CK(A->acc.ensure(T * std::max(w, A->d) * 8));
+    CK(A->qkv.ensure(T * w * 4));
+    CK(A->qkv_scale.ensure(3 * T * sizeof(Scale)));
+    CK(A->o.ensure(T * A->q * 4));
+    CK(A->o_scale.ensure(T * A->cfg.n_kv_heads * sizeof(Scale)));
+    CK(A->merged.ensure(T * A->q * 4));
+    CK(A->out.ensure(T * A->d * 4));
+    CK(A->out_scale.ensure(T * sizeof(Scale)));
+    CK(A->m.ensure(T * A->d * 4));
+    CK(A->scal.ensure(A_NSCALES * sizeof(Scale) + AU_N * 8));
+    A->cap = T;
+    return KTMOE_OK;
+}
+
+// QuantLinear::forward_int of `n` stacked linears on every row of x (rows x k at one scale) by itself.
+int attn_linear(ktmoe_attn* A, const int32_t* x, const Scale* x_scale, int64_t T, const Planes& W, int64_t width,
+                const mk::RowLinears& p, int n, int32_t* y, Scale* ys, cudaStream_t st) {
+    ktmoe_ctx* ctx = A->ctx;
+    const int64_t T_pad = round_up(T, 64);
+    KLAUNCH(st, (unsigned)T, 256, 0, (mk::quant_rows_kernel), x, (int)T, (int)W.k, (int)W.k_pad, (long long)T_pad,
+            A->planes.as<int8_t>(), A->xmax.as<int64_t>(), A->sqx.as<Scale>(), x_scale, nullptr);
+    GemmCall g;
+    g.A = W;
+    g.M_valid = width;
+    g.B = Planes{A->planes.as<int8_t>(), 1, T_pad, W.k, W.k_pad};
+    g.out = A->acc.as<int64_t>();
+    g.ld_out = width;
+    g.BN = pick_bn((double)T, W.rows_pad % dg::pair::BM2 == 0);
+    g.grid_y = (T + g.BN - 1) / g.BN;
+    g.single_rows = T;
+    if (int r = run_gemm(ctx, st, g)) return r;
+    KLAUNCH(st, dim3((unsigned)T, (unsigned)n), 256, 0, (mk::linear_rows_out_kernel), A->acc.as<int64_t>(), (int)T, (int)width,
+            A->sqx.as<Scale>(), p, y, ys);
+    return KTMOE_OK;
+}
+
+// Rows at their own scales into one tensor at one scale (layers.rs:1001-1019; a single row stays as it is).
+int attn_merge(ktmoe_attn* A, const int32_t* x, const Scale* xs, int64_t rows, int64_t width, Scale* common,
+               unsigned long long* gmax, int32_t* y, Scale* ys, cudaStream_t st) {
+    ktmoe_ctx* ctx = A->ctx;
+    if (rows == 1) {
+        KLAUNCH(st, (unsigned)((width + 255) / 256), 256, 0, (mk::copy_row_kernel), x, xs, (int)width, y, ys);
+        return KTMOE_OK;
+    }
+    KLAUNCH(st, 1, 1024, 0, (mk::common_scale_kernel), xs, (int)rows, 0, common, nullptr, nullptr);
+    KLAUNCH(st, (unsigned)rows, 256, 0, (mk::merge_max_kernel), x, xs, (int)rows, (int)width, common, gmax);
+    KLAUNCH(st, (unsigned)rows, 256, 0, (mk::merge_final_kernel), x, xs, (int)rows, (int)width, common, gmax, y, ys, nullptr);
+    return KTMOE_OK;
+}
+
+int attn_forward(ktmoe_attn* A, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* x, const Scale* xs,
+                 int32_t* y, Scale* ys, cudaStream_t st) {
+    ktmoe_ctx* ctx = A->ctx;
+    const int64_t T = batch->rows, d = A->d, w = A->q + 2 * A->kv, hk = A->cfg.n_kv_heads;
+    Scale* sc = A->scal.as<Scale>();
+    unsigned long long* u = (unsigned long long*)(sc + A_NSCALES);
+    int32_t* xn = A->xn.as<int32_t>();
+    CK(cudaMemsetAsync(u, 0, AU_N * 8, st));
+    CK(cudaMemsetAsync(A->o_scale.p, 0, T * hk * sizeof(Scale), st));  // rows of no sequence: zeros
+    Scale* c = A->c_rows.as<Scale>();
+    KLAUNCH(st, (unsigned)T, 256, 0, (mk::rms_rows_kernel), x, (int)T, (int)d, xs, A->norm_ws, A->norm_eps, c);
+    KLAUNCH(st, 1, 1024, 0, (mk::common_scale_kernel), c, (int)T, 0, sc + A_NORM, nullptr, nullptr);
+    KLAUNCH(st, (unsigned)T, 256, 0, (mk::rms_max_kernel), x, A->b_norm.as<int32_t>(), (int)T, (int)d, c, sc + A_NORM, u + AU_NORM);
+    KLAUNCH(st, (unsigned)T, 256, 0, (mk::rms_final_kernel), x, A->b_norm.as<int32_t>(), (int)T, (int)d, c, sc + A_NORM,
+            u + AU_NORM, xn);
+    KLAUNCH(st, 1, 1, 0, (mk::gmax_scale_kernel), sc + A_NORM, u + AU_NORM, sc + A_XN);
+    const mk::RowLinears pq{{0, (int)A->q, (int)(A->q + A->kv), (int)w}, {A->q_ws, A->k_ws, A->v_ws}};
+    int32_t* qkv = A->qkv.as<int32_t>();
+    Scale* qs = A->qkv_scale.as<Scale>();
+    if (int r = attn_linear(A, xn, sc + A_XN, T, A->w_qkv, w, pq, 3, qkv, qs, st)) return r;
+    const ktmoe_rope* rope = A->rope.table ? &A->rope : nullptr;
+    if (int r = kv_append(ctx, cache, batch, qkv + A->q, w, qkv + A->q + A->kv, w, (const ktmoe_scale*)(qs + T),
+                          (const ktmoe_scale*)(qs + 2 * T), 1, rope, (void*)st))
+        return r;
+    const double soft = A->softmax_scale > 0.0 ? A->softmax_scale : std::pow((double)A->cfg.head_dim, -0.5);
+    int32_t* o = A->o.as<int32_t>();
+    if (int r = kv_attention(ctx, cache, batch, qkv, w, (const ktmoe_scale*)qs, 1, rope, A->cfg.n_heads, soft, A->window,
+                             A->sinks, o, A->q, A->o_scale.as<ktmoe_scale>(), (void*)st))
+        return r;
+    // the heads of a KV head share a scale; all of them into one tensor
+    if (int r = attn_merge(A, o, A->o_scale.as<Scale>(), T * hk, A->q / hk, sc + A_HEADS, u + AU_HEADS, A->merged.as<int32_t>(),
+                           sc + A_MERGED, st))
+        return r;
+    const mk::RowLinears po{{0, (int)d, (int)d, (int)d}, {A->out_ws, A->out_ws, A->out_ws}};
+    if (int r = attn_linear(A, A->merged.as<int32_t>(), sc + A_MERGED, T, A->w_out, d, po, 1, A->out.as<int32_t>(),
+                            A->out_scale.as<Scale>(), st))
+        return r;
+    if (int r = attn_merge(A, A->out.as<int32_t>(), A->out_scale.as<Scale>(), T, d, sc + A_ROWS, u + AU_ROWS, A->m.as<int32_t>(),
+                           sc + A_M, st))
+        return r;
+    const int64_t n = T * d;
+    const unsigned rb = (unsigned)std::max<int64_t>(1, std::min<int64_t>(1184, (n + 255) / 256));
+    KLAUNCH(st, 1, 1, 0, (mk::add2_prepare_kernel), xs, sc + A_M, sc + A_ADD);
+    KLAUNCH(st, rb, 256, 0, (mk::add2_max_kernel), x, A->m.as<int32_t>(), n, sc + A_ADD, u + AU_ADD);
+    KLAUNCH(st, rb, 256, 0, (mk::add2_final_kernel), x, A->m.as<int32_t>(), n, sc + A_ADD, u + AU_ADD, y);
+    KLAUNCH(st, 1, 1, 0, (mk::gmax_scale_kernel), sc + A_ADD, u + AU_ADD, ys);
+    return KTMOE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ktmoe_attn_create(ktmoe_ctx* ctx, const ktmoe_attn_config* cfg, ktmoe_attn** out) {
+    if (!ctx || !cfg || !out) return KTMOE_ERR_ARG;
+    *out = nullptr;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    if (cfg->d_model < 1 || cfg->n_kv_heads < 1 || cfg->n_kv_heads > 1024 || cfg->n_heads < 1 ||
+        cfg->n_heads % cfg->n_kv_heads != 0)
+        return fail(ctx, KTMOE_ERR_ARG, "n_heads must be a positive multiple of n_kv_heads (1 to 1024), d_model positive");
+    if (cfg->head_dim < 16 || cfg->head_dim > 256 || cfg->head_dim % 16 != 0)
+        return fail(ctx, KTMOE_ERR_UNSUPPORTED, "head_dim must be a multiple of 16 from 16 to 256");
+    if (((int64_t)cfg->n_heads + 2 * cfg->n_kv_heads) * cfg->head_dim > INT32_MAX / 2)
+        return fail(ctx, KTMOE_ERR_UNSUPPORTED, "the heads are wider than 2^30");
+    if (int r = set_device(ctx)) return r;
+    ktmoe_attn* A = new ktmoe_attn();
+    A->ctx = ctx;
+    A->cfg = *cfg;
+    A->d = cfg->d_model;
+    A->q = (int64_t)cfg->n_heads * cfg->head_dim;
+    A->kv = (int64_t)cfg->n_kv_heads * cfg->head_dim;
+    int r = alloc_planes(ctx, A->b_qkv, A->w_qkv, 1, A->q + 2 * A->kv, A->d);
+    if (r == KTMOE_OK) r = alloc_planes(ctx, A->b_out, A->w_out, 1, A->d, A->q);
+    if (r != KTMOE_OK) {
+        A->b_qkv.release();
+        A->b_out.release();
+        delete A;
+        return r;
+    }
+    *out = A;
+    return KTMOE_OK;
+}
+
+int ktmoe_attn_destroy(ktmoe_attn* A) {
+    if (!A) return KTMOE_ERR_ARG;
+    ktmoe_ctx* ctx = A->ctx;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    cudaSetDevice(ctx->device);
+    cudaStreamSynchronize(ctx->stream);
+    DevBuf* bufs[] = {&A->b_qkv, &A->b_out, &A->b_norm, &A->b_rope, &A->c_rows, &A->xn,     &A->planes,    &A->xmax,
+                      &A->sqx,   &A->acc,   &A->qkv,    &A->qkv_scale, &A->o,    &A->o_scale, &A->merged, &A->out,
+                      &A->out_scale, &A->m, &A->scal};
+    for (DevBuf* b : bufs) b->release();
+    delete A;
+    return KTMOE_OK;
+}
+
+int ktmoe_attn_set_qkv(ktmoe_attn* A, const int32_t* q, ktmoe_scale q_scale, const int32_t* k, ktmoe_scale k_scale,
+                       const int32_t* v, ktmoe_scale v_scale) {
+    if (!A || !q || !k || !v) return KTMOE_ERR_ARG;
+    ktmoe_ctx* ctx = A->ctx;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    if (int r = set_device(ctx)) return r;
+    A->qkv_set = false;
+    if (int r = upload_matrix(ctx, A->w_qkv, 0, q, A->q, A->d, 0)) return r;
+    if (int r = upload_matrix(ctx, A->w_qkv, 0, k, A->kv, A->d, A->q)) return r;
+    if (int r = upload_matrix(ctx, A->w_qkv, 0, v, A->kv, A->d, A->q + A->kv)) return r;
+    A->q_ws = S(q_scale);
+    A->k_ws = S(k_scale);
+    A->v_ws = S(v_scale);
+    A->qkv_set = true;
+    return KTMOE_OK;
+}
+
+int ktmoe_attn_set_out(ktmoe_attn* A, const int32_t* out, ktmoe_scale out_scale) {
+    if (!A || !out) return KTMOE_ERR_ARG;
+    ktmoe_ctx* ctx = A->ctx;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    if (int r = set_device(ctx)) return r;
+    A->out_set = false;
+    if (int r = upload_matrix(ctx, A->w_out, 0, out, A->d, A->q, 0)) return r;
+    A->out_ws = S(out_scale);
+    A->out_set = true;
+    return KTMOE_OK;
+}
+
+int ktmoe_attn_set_norm(ktmoe_attn* A, const int32_t* w_codes, ktmoe_scale w_scale, ktmoe_scale eps_scale) {
+    if (!A || !w_codes) return KTMOE_ERR_ARG;
+    ktmoe_ctx* ctx = A->ctx;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    if (int r = set_device(ctx)) return r;
+    CK(A->b_norm.ensure(A->d * 4));
+    CK(cudaMemcpy(A->b_norm.p, w_codes, A->d * 4, cudaMemcpyHostToDevice));
+    A->norm_ws = S(w_scale);
+    A->norm_eps = S(eps_scale);
+    A->norm_set = true;
+    return KTMOE_OK;
+}
+
+int ktmoe_attn_set_rope(ktmoe_attn* A, double theta, int32_t rot_dim, int64_t positions, int32_t interleaved) {
+    if (!A) return KTMOE_ERR_ARG;
+    ktmoe_ctx* ctx = A->ctx;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    if (positions == 0) {
+        A->rope = ktmoe_rope{nullptr, 0, 0, 0};
+        return KTMOE_OK;
+    }
+    if (positions < 0 || positions > (int64_t)1 << 24 || rot_dim < 2 || rot_dim % 2 != 0 || rot_dim > A->cfg.head_dim)
+        return fail(ctx, KTMOE_ERR_ARG, "rot_dim must be even, from 2 to head_dim, positions from 0 to 2^24");
+    if (int r = set_device(ctx)) return r;
+    std::vector<int32_t> table((size_t)positions * rot_dim);
+    if (ktmoe_rope_table(theta, rot_dim, positions, table.data()) != KTMOE_OK)
+        return fail(ctx, KTMOE_ERR_ARG, "theta must be positive and finite");
+    CK(cudaStreamSynchronize(ctx->stream));
+    CK(A->b_rope.ensure(table.size() * 4));
+    CK(cudaMemcpy(A->b_rope.p, table.data(), table.size() * 4, cudaMemcpyHostToDevice));
+    A->rope = ktmoe_rope{A->b_rope.as<int32_t>(), positions, rot_dim, interleaved ? 1 : 0};
+    return KTMOE_OK;
+}
+
+int ktmoe_attn_set_mask(ktmoe_attn* A, double softmax_scale, int32_t window, int32_t sinks) {
+    if (!A) return KTMOE_ERR_ARG;
+    std::lock_guard<std::mutex> lk(A->ctx->mu);
+    if (!(softmax_scale >= 0.0) || !std::isfinite(softmax_scale) || window < 0 || sinks < 0)
+        return fail(A->ctx, KTMOE_ERR_ARG, "softmax_scale, window and sinks must not be negative");
+    A->softmax_scale = softmax_scale;
+    A->window = window;
+    A->sinks = sinks;
+    return KTMOE_OK;
+}
+
+int ktmoe_attn_forward_dev(ktmoe_attn* A, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* x_dev,
+                           const ktmoe_scale* x_scale_dev, int32_t* y_dev, ktmoe_scale* y_scale_dev, void* stream) {
+    if (!A || !cache || !batch) return KTMOE_ERR_ARG;
+    ktmoe_ctx* ctx = A->ctx;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    if (!A->qkv_set || !A->out_set || !A->norm_set)
+        return fail(ctx, KTMOE_ERR_STATE, "a weight of the attention half is not set");
+    if (cache->n_kv_heads != A->cfg.n_kv_heads || cache->head_dim != A->cfg.head_dim)
+        return fail(ctx, KTMOE_ERR_ARG, "the cache's heads are not the attention's");
+    if (batch->rows < 0 || batch->rows * A->cfg.n_kv_heads > INT32_MAX || batch->rows * A->d > (int64_t)1 << 40)
+        return fail(ctx, KTMOE_ERR_ARG, "too many rows");
+    if (batch->rows == 0) return KTMOE_OK;
+    if (!x_dev || !x_scale_dev || !y_dev || !y_scale_dev) return KTMOE_ERR_ARG;
+    if (int r = set_device(ctx)) return r;
+    if (int r = attn_scratch(A, batch->rows)) return r;
+    cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
+    return attn_forward(A, cache, batch, x_dev, (const Scale*)x_scale_dev, y_dev, (Scale*)y_scale_dev, st);
 }
 
 }  // extern "C"

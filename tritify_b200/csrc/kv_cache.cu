@@ -6,6 +6,7 @@
 #include <cstdint>
 
 #include "context.cuh"
+#include "kv_host.h"
 #include "kv_attend_few.cuh"
 #include "kv_attend_tile.cuh"
 #include "kv_kernels.cuh"
@@ -150,18 +151,28 @@ int ktmoe_rope_table(double theta, int32_t rot_dim, int64_t positions, int32_t* 
 }
 
 int ktmoe_kv_append_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* k,
-                        int64_t ld_k, const int32_t* v, int64_t ld_v, const ktmoe_scale* scale, int32_t scale_stride,
-                        const ktmoe_rope* rope, void* stream) {
+                        int64_t ld_k, const int32_t* v, int64_t ld_v, const ktmoe_scale* k_scale,
+                        const ktmoe_scale* v_scale, int32_t scale_stride, const ktmoe_rope* rope, void* stream) {
     if (!ctx || !cache || !batch) return KTMOE_ERR_ARG;
     std::lock_guard<std::mutex> lk(ctx->mu);
+    return kv_append(ctx, cache, batch, k, ld_k, v, ld_v, k_scale, v_scale, scale_stride, rope, stream);
+}
+
+}  // extern "C"
+
+int kv_append(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* k, int64_t ld_k,
+              const int32_t* v, int64_t ld_v, const ktmoe_scale* k_scale, const ktmoe_scale* v_scale,
+              int32_t scale_stride, const ktmoe_rope* rope, void* stream) {
+    if (!v_scale) v_scale = k_scale;
     kv::AppendArgs a{};
     if (int r = check_cache(ctx, cache, batch, &a.c, &a.b)) return r;
     if (int r = check_rope(ctx, rope, a.c.dim, &a.rope)) return r;
-    if (int r = check_scale(ctx, scale, scale_stride)) return r;
+    if (int r = check_scale(ctx, k_scale, scale_stride)) return r;
+    if (int r = check_scale(ctx, v_scale, scale_stride)) return r;
     const int64_t width = (int64_t)a.c.heads * a.c.dim;
     if (ld_k < width || ld_v < width) return fail(ctx, KTMOE_ERR_ARG, "a row stride is below n_kv_heads * head_dim");
     if (batch->n_seqs == 0 || batch->rows == 0) return KTMOE_OK;
-    if (!k || !v || !scale || !aligned(k, 4) || !aligned(v, 4))
+    if (!k || !v || !k_scale || !aligned(k, 4) || !aligned(v, 4))
         return fail(ctx, KTMOE_ERR_ARG, "keys, values or scales are null or not aligned");
     if (int r = set_device(ctx)) return r;
     a.err = error_of(ctx);
@@ -169,12 +180,15 @@ int ktmoe_kv_append_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe
     a.v = v;
     a.ld_k = ld_k;
     a.ld_v = ld_v;
-    a.scale = (const longlong2*)scale;
+    a.scale[0] = (const longlong2*)k_scale;
+    a.scale[1] = (const longlong2*)v_scale;
     a.scale_stride = scale_stride;
     a.vec = aligned(k, 16) && aligned(v, 16) && ld_k % 4 == 0 && ld_v % 4 == 0;
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
     return a.c.dim <= 128 ? launch_append<1>(ctx, st, a) : launch_append<2>(ctx, st, a);
 }
+
+extern "C" {
 
 int ktmoe_kv_read_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, float* k, int64_t ld_k,
                       float* v, int64_t ld_v, void* stream) {
@@ -204,6 +218,16 @@ int ktmoe_attention_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe
                         ktmoe_scale* o_scale, void* stream) {
     if (!ctx || !cache || !batch) return KTMOE_ERR_ARG;
     std::lock_guard<std::mutex> lk(ctx->mu);
+    return kv_attention(ctx, cache, batch, q, ld_q, scale, scale_stride, rope, n_heads, softmax_scale, window, sinks, o, ld_o,
+                        o_scale, stream);
+}
+
+}  // extern "C"
+
+int kv_attention(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* q, int64_t ld_q,
+                 const ktmoe_scale* scale, int32_t scale_stride, const ktmoe_rope* rope, int32_t n_heads,
+                 double softmax_scale, int32_t window, int32_t sinks, int32_t* o, int64_t ld_o, ktmoe_scale* o_scale,
+                 void* stream) {
     kv::AttendArgs a{};
     if (int r = check_cache(ctx, cache, batch, &a.c, &a.b)) return r;
     if (int r = check_rope(ctx, rope, a.c.dim, &a.rope)) return r;
@@ -238,5 +262,3 @@ int ktmoe_attention_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe
         return a.c.dim <= 128 ? launch_tile<1>(ctx, st, a) : launch_tile<2>(ctx, st, a);
     return a.c.dim <= 128 ? launch_few<1, 2>(ctx, st, a) : launch_few<2, 1>(ctx, st, a);
 }
-
-}  // extern "C"

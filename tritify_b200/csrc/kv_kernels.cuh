@@ -301,7 +301,7 @@ struct AppendArgs {
     Error err;
     const int32_t *k, *v;
     long long ld_k, ld_v;
-    const longlong2* scale;
+    const longlong2* scale[2];  // of K, of V
     int scale_stride;
     int vec;  // rows are 16-byte aligned: 16-byte loads
 };
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) append_kernel(const AppendArgs
     const RawBatch<NB> raw = fetch_rows<NB>(x, heads, dim, a.vec, rope);
     Place p;
     if (!locate(a.b, a.err, t, a.c.page_shift, p) || p.pos < 0) return;
-    const longlong2 sc = a.scale[(long long)t * a.scale_stride];
+    const longlong2 sc = a.scale[is_v][(long long)t * a.scale_stride];
     const long long page = pool_page(a.b, a.c, a.err, p.seq, p.pos >> a.c.page_shift);
     const int2* cs = rope_row(rope, a.err, p.pos);
     RowBatch<NB> rows;

@@ -2259,4 +2259,29 @@ __global__ void pack_codes_kernel(const int32_t* __restrict__ codes, long long r
     if (nbig && big) atomicAdd(big, (unsigned long long)nbig);
 }
 
+// ───────────── linears of rows by themselves (the attention half of a block) ─────────────
+// The output of QuantLinear::forward_int (layers.rs:299-328) for each row alone, from the int64 accumulators acc
+// [rows][ld]: columns [begin[p], begin[p + 1]) are linear p's; its row is requantised at the row's largest |acc| to y
+// [rows][ld] and its scale goes to ys[p * rows + row] = ratio(max)·s_qx·w_scale. One block per (row, linear).
+struct RowLinears {
+    int begin[4];
+    Scale w[3];
+};
+__global__ void linear_rows_out_kernel(const int64_t* __restrict__ acc, int rows, int ld, const Scale* __restrict__ row_sqx,
+                                       const RowLinears p, int32_t* __restrict__ y, Scale* __restrict__ ys) {
+    kt::pdl_enter();
+    __shared__ uint64_t red[32];
+    const int r = blockIdx.x, l = blockIdx.y;
+    const int64_t* a = acc + (long long)r * ld;
+    uint64_t m = 0;
+    for (int c = p.begin[l] + threadIdx.x; c < p.begin[l + 1]; c += blockDim.x) m = max(m, uabs64(a[c]));
+    const int64_t ymax = (int64_t)block_max_u64(m, red);
+    const Scale cd = kt::scale_mul(row_sqx[r], p.w[l]);
+    const bool zero = ymax == 0 || cd.mant == 0;
+    const kt::ReqDiv rq = kt::make_req(zero ? 1 : ymax);
+    for (int c = p.begin[l] + threadIdx.x; c < p.begin[l + 1]; c += blockDim.x)
+        y[(long long)r * ld + c] = zero ? 0 : kt::requant_row(a[c], rq);
+    if (threadIdx.x == 0) ys[(long long)l * rows + r] = zero ? kt::scale_zero() : kt::scale_mul(kt::ratio_act(ymax), cd);
+}
+
 }  // namespace mk

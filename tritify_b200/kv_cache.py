@@ -132,17 +132,21 @@ class KvCache:
         _need(scale.shape[0] >= rows, "scale: one for all rows or one a row")
         return 1
 
-    def append(self, batch: KvBatch, k, v, scale, rope: Optional[Rope] = None, stream: Optional[int] = None) -> None:
+    def append(self, batch: KvBatch, k, v, scale, rope: Optional[Rope] = None, v_scale=None,
+               stream: Optional[int] = None) -> None:
         """Write the batch's new keys and values (int32 codes [rows][n_kv_heads * head_dim], row strides allowed) at
-        ``scale`` into their pages, the keys rotated by ``rope``."""
+        ``scale`` (the values at ``v_scale`` when given) into their pages, the keys rotated by ``rope``."""
         width = self.n_kv_heads * self.head_dim
         ld_k = _matrix(k, "k", "int32", batch.rows, width)
         ld_v = _matrix(v, "v", "int32", batch.rows, width)
         stride = self._scale(scale, batch.rows)
-        self._on_device(self.k, k, v, scale, batch.kv_len, *([rope.table] if rope else []))
+        if v_scale is None:
+            v_scale = scale
+        _need(self._scale(v_scale, batch.rows) == stride, "scale and v_scale: both one for all rows or both one a row")
+        self._on_device(self.k, k, v, scale, v_scale, batch.kv_len, *([rope.table] if rope else []))
         self.ctx.check(lib().ktmoe_kv_append_dev(self.ctx.handle, self._c, batch._c, k.data_ptr(), ld_k, v.data_ptr(),
-                                                 ld_v, scale.data_ptr(), stride, rope._c if rope else None,
-                                                 self._stream(stream)))
+                                                 ld_v, scale.data_ptr(), v_scale.data_ptr(), stride,
+                                                 rope._c if rope else None, self._stream(stream)))
 
     def read(self, batch: KvBatch, k, v, stream: Optional[int] = None) -> None:
         """Read the batch's rows back as values (float32 [rows][n_kv_heads * head_dim]) into ``k`` and ``v``."""
