@@ -30,27 +30,49 @@ def rope_table(theta: float, rot_dim: int, positions: int) -> np.ndarray:
     return out
 
 
+_torch = None  # torch and what the calls below take from it, imported with the first class that needs it
+_raw_stream = None
+
+
+def _load_torch():
+    global _torch, _raw_stream
+    if _torch is None:
+        import torch
+
+        # the current stream's handle without building a Stream object, where torch offers it
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _torch = torch
+    return _torch
+
+
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
 
 
-def _tensor(t, name: str, dtype: str, dims: Optional[int] = None, contiguous: bool = True) -> None:
-    import torch
+def _tensor(t, name: str, dtype: str, dims: int) -> None:
+    torch = _load_torch()
+    _need(isinstance(t, torch.Tensor) and t.dtype is getattr(torch, dtype), f"{name}: a torch tensor of {dtype}")
+    _need(t.dim() == dims, f"{name}: {dims} dimensions")
+    _need(t.is_contiguous(), f"{name}: contiguous")
 
-    _need(isinstance(t, torch.Tensor) and t.dtype == getattr(torch, dtype), f"{name}: a torch tensor of {dtype}")
-    _need(dims is None or t.dim() == dims, f"{name}: {dims} dimensions")
-    _need(not contiguous or t.is_contiguous(), f"{name}: contiguous")
 
-
-def _matrix(t, name: str, dtype: str, rows: int, width: int) -> int:
-    """Check a [rows or more][width] matrix whose rows are contiguous; returns its row stride."""
-    _tensor(t, name, dtype, 2, contiguous=False)
-    _need(t.shape[0] >= rows and t.shape[1] == width, f"{name}: at least {rows} rows of {width}")
-    _need(t.stride(1) == 1 or width == 1, f"{name}: the elements of a row lie side by side")
-    # one row has no stride of its own (torch reports any), and a broadcast row is not a matrix
-    ld = t.stride(0) if t.shape[0] > 1 else width
-    _need(ld >= width, f"{name}: rows that do not overlap")
+def _matrix(t, name: str, dtype, rows: int, width: int) -> int:
+    """Check a [rows or more][width] matrix whose rows are contiguous; returns its row stride. (These checks run before
+    every launch, so they touch each property of a tensor once and build no message unless one fails.)"""
+    if not isinstance(t, _torch.Tensor) or t.dtype is not dtype:
+        raise ValueError(f"{name}: a torch tensor of {dtype}")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] < rows or shape[1] != width:
+        raise ValueError(f"{name}: at least {rows} rows of {width}")
+    ld, step = t.stride()
+    if step != 1 and width != 1:
+        raise ValueError(f"{name}: the elements of a row lie side by side")
+    if shape[0] <= 1:
+        return width  # one row has no stride of its own (torch reports any)
+    if ld < width:
+        raise ValueError(f"{name}: rows that do not overlap")
     return ld
 
 
@@ -63,6 +85,7 @@ class Rope:
         _need(table.shape[0] >= 1 and table.shape[1] >= 1 and table.shape[2] == 2,
               "rotation table: [positions][rot_dim / 2][2]")
         self.table, self.interleaved = table, bool(interleaved)
+        self.device_index = table.get_device()
         self._c = KtmoeRope(table.data_ptr(), table.shape[0], 2 * table.shape[1], 1 if interleaved else 0)
 
 
@@ -79,6 +102,7 @@ class KvBatch:
         _need(q_begin.shape[0] == n + 1 and page_table.shape[0] == n, "q_begin has one entry more than kv_len, page_table as many rows")
         _need(0 <= int(rows) <= 1 << 30, "rows: from 0 to 2^30")
         _need(q_begin.device == kv_len.device == page_table.device, "the batch's tensors lie on one device")
+        self.device_index = kv_len.get_device()
         self.q_begin, self.kv_len, self.page_table, self.rows = q_begin, kv_len, page_table, int(rows)
         self._c = KtmoeKvBatch(n, page_table.shape[1], q_begin.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
                                self.rows)
@@ -96,9 +120,8 @@ class KvCache:
         self.ctx = ctx
         self.n_pages, self.page_tokens, self.n_kv_heads, self.head_dim = n_pages, page_tokens, n_kv_heads, head_dim
         shape = (n_pages, n_kv_heads, page_tokens)
+        torch = _load_torch()
         if pools is None:
-            import torch
-
             dev = torch.device("cuda", ctx.device)
             pools = [torch.zeros(*shape, head_dim, dtype=torch.int8, device=dev) for _ in range(2)]
             pools += [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(2)]
@@ -109,53 +132,65 @@ class KvCache:
         for t, name in ((self.k_scale, "k scales"), (self.v_scale, "v scales")):
             _tensor(t, name, "bfloat16", 3)
             _need(tuple(t.shape) == shape, f"{name}: [n_pages][n_kv_heads][page_tokens]")
+        self.device_index = self.k.get_device()
+        if any(t.get_device() != self.device_index for t in (self.v, self.k_scale, self.v_scale)):
+            raise ValueError("the pools lie on one device")
+        L = lib()
+        self._append, self._read, self._attend = L.ktmoe_kv_append_dev, L.ktmoe_kv_read_dev, L.ktmoe_attention_dev
         self._c = KtmoeKvCache(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
                                n_pages, page_tokens, n_kv_heads, head_dim)
 
-    def _on_device(self, *tensors) -> None:
+    def _prepare(self, batch: KvBatch, rope: Optional[Rope], stream: Optional[int], *tensors):
+        """Every tensor on the context's device; the stream to launch on."""
+        device = self.ctx.device
         for t in tensors:
-            _need(t.device.type == "cuda" and t.device.index == self.ctx.device,
-                  f"every tensor lies on the context's device (cuda:{self.ctx.device})")
-
-    def _stream(self, stream: Optional[int]):
+            if t.get_device() != device:
+                raise ValueError(f"every tensor lies on the context's device (cuda:{device})")
+        if batch.device_index != device or self.device_index != device or (rope and rope.device_index != device):
+            raise ValueError(f"every tensor lies on the context's device (cuda:{device})")
         if stream is None:
-            import torch
-
-            stream = torch.cuda.current_stream(self.ctx.device).cuda_stream or STREAM_LEGACY
-        return ctypes.c_void_p(stream) if stream else None
+            return _raw_stream(device) or STREAM_LEGACY
+        return stream or None
 
     def _scale(self, scale, rows: int) -> int:
-        _tensor(scale, "scale", "int64")
-        _need(scale.shape[-1:] == (2,) and scale.numel() in (2, 2 * scale.shape[0]), "scale: [2] or [rows][2]")
-        if scale.numel() == 2 and (scale.dim() == 1 or rows != 1):
+        """0: one scale for all rows, 1: one a row."""
+        if not isinstance(scale, _torch.Tensor) or scale.dtype is not _torch.int64 or not scale.is_contiguous():
+            raise ValueError("scale: a contiguous torch tensor of int64")
+        shape = scale.shape
+        if len(shape) == 2 and shape[1] == 2 and shape[0] >= rows:
+            return 1
+        if shape == (2,) or shape == (1, 2):
             return 0
-        _need(scale.shape[0] >= rows, "scale: one for all rows or one a row")
-        return 1
+        raise ValueError("scale: [2], or [rows][2] with a scale for each row")
 
     def append(self, batch: KvBatch, k, v, scale, rope: Optional[Rope] = None, v_scale=None,
                stream: Optional[int] = None) -> None:
         """Write the batch's new keys and values (int32 codes [rows][n_kv_heads * head_dim], row strides allowed) at
         ``scale`` (the values at ``v_scale`` when given) into their pages, the keys rotated by ``rope``."""
-        width = self.n_kv_heads * self.head_dim
-        ld_k = _matrix(k, "k", "int32", batch.rows, width)
-        ld_v = _matrix(v, "v", "int32", batch.rows, width)
-        stride = self._scale(scale, batch.rows)
+        width, rows, int32 = self.n_kv_heads * self.head_dim, batch.rows, _torch.int32
+        ld_k = _matrix(k, "k", int32, rows, width)
+        ld_v = _matrix(v, "v", int32, rows, width)
+        stride = self._scale(scale, rows)
         if v_scale is None:
-            v_scale = scale
-        _need(self._scale(v_scale, batch.rows) == stride, "scale and v_scale: both one for all rows or both one a row")
-        self._on_device(self.k, k, v, scale, v_scale, batch.kv_len, *([rope.table] if rope else []))
-        self.ctx.check(lib().ktmoe_kv_append_dev(self.ctx.handle, self._c, batch._c, k.data_ptr(), ld_k, v.data_ptr(),
-                                                 ld_v, scale.data_ptr(), v_scale.data_ptr(), stride,
-                                                 rope._c if rope else None, self._stream(stream)))
+            at = self._prepare(batch, rope, stream, k, v, scale)
+        else:
+            _need(self._scale(v_scale, rows) == stride, "scale and v_scale: both one for all rows or both one a row")
+            at = self._prepare(batch, rope, stream, k, v, scale, v_scale)
+        status = self._append(self.ctx.handle, self._c, batch._c, k.data_ptr(), ld_k, v.data_ptr(), ld_v,
+                              scale.data_ptr(), None if v_scale is None else v_scale.data_ptr(), stride,
+                              rope._c if rope else None, at)
+        if status:
+            self.ctx.check(status)
 
     def read(self, batch: KvBatch, k, v, stream: Optional[int] = None) -> None:
         """Read the batch's rows back as values (float32 [rows][n_kv_heads * head_dim]) into ``k`` and ``v``."""
-        width = self.n_kv_heads * self.head_dim
-        ld_k = _matrix(k, "k", "float32", batch.rows, width)
-        ld_v = _matrix(v, "v", "float32", batch.rows, width)
-        self._on_device(self.k, k, v, batch.kv_len)
-        self.ctx.check(lib().ktmoe_kv_read_dev(self.ctx.handle, self._c, batch._c, k.data_ptr(), ld_k, v.data_ptr(),
-                                               ld_v, self._stream(stream)))
+        width, rows, float32 = self.n_kv_heads * self.head_dim, batch.rows, _torch.float32
+        ld_k = _matrix(k, "k", float32, rows, width)
+        ld_v = _matrix(v, "v", float32, rows, width)
+        at = self._prepare(batch, None, stream, k, v)
+        status = self._read(self.ctx.handle, self._c, batch._c, k.data_ptr(), ld_k, v.data_ptr(), ld_v, at)
+        if status:
+            self.ctx.check(status)
 
     def attention(self, batch: KvBatch, q, scale, out, out_scale, n_heads: int, rope: Optional[Rope] = None,
                   softmax_scale: Optional[float] = None, window: int = 0, sinks: int = 0,
@@ -164,19 +199,20 @@ class KvCache:
         cache, which already holds their keys and values, into ``out`` (int32 [rows][n_heads * head_dim]) at
         ``out_scale`` (int64 [rows][n_kv_heads][2]). ``softmax_scale`` defaults to head_dim ** -0.5; ``window`` > 0
         keeps the last ``window`` positions and the first ``sinks``."""
-        _need(n_heads >= 1 and n_heads % self.n_kv_heads == 0, "n_heads: a multiple of n_kv_heads")
-        _need(window >= 0 and sinks >= 0, "window and sinks: not negative")
-        width = n_heads * self.head_dim
-        ld_q = _matrix(q, "q", "int32", batch.rows, width)
-        ld_o = _matrix(out, "out", "int32", batch.rows, width)
-        stride = self._scale(scale, batch.rows)
-        _tensor(out_scale, "out_scale", "int64", 3)
-        _need(out_scale.shape[0] >= batch.rows and tuple(out_scale.shape[1:]) == (self.n_kv_heads, 2),
-              "out_scale: [rows][n_kv_heads][2]")
-        if softmax_scale is None:
-            softmax_scale = self.head_dim ** -0.5
-        self._on_device(self.k, q, out, scale, out_scale, batch.kv_len, *([rope.table] if rope else []))
-        self.ctx.check(lib().ktmoe_attention_dev(self.ctx.handle, self._c, batch._c, q.data_ptr(), ld_q,
-                                                 scale.data_ptr(), stride, rope._c if rope else None, n_heads,
-                                                 float(softmax_scale), window, sinks, out.data_ptr(), ld_o,
-                                                 out_scale.data_ptr(), self._stream(stream)))
+        if n_heads < 1 or n_heads % self.n_kv_heads != 0 or window < 0 or sinks < 0:
+            raise ValueError("n_heads: a multiple of n_kv_heads; window and sinks: not negative")
+        width, rows, int32 = n_heads * self.head_dim, batch.rows, _torch.int32
+        ld_q = _matrix(q, "q", int32, rows, width)
+        ld_o = _matrix(out, "out", int32, rows, width)
+        stride = self._scale(scale, rows)
+        shape = out_scale.shape
+        if (out_scale.dtype is not _torch.int64 or len(shape) != 3 or shape[0] < rows or shape[1] != self.n_kv_heads
+                or shape[2] != 2 or not out_scale.is_contiguous()):
+            raise ValueError("out_scale: a contiguous torch tensor of int64, [rows][n_kv_heads][2]")
+        at = self._prepare(batch, rope, stream, q, out, scale, out_scale)
+        status = self._attend(self.ctx.handle, self._c, batch._c, q.data_ptr(), ld_q, scale.data_ptr(), stride,
+                              rope._c if rope else None, n_heads,
+                              self.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale), window, sinks,
+                              out.data_ptr(), ld_o, out_scale.data_ptr(), at)
+        if status:
+            self.ctx.check(status)
