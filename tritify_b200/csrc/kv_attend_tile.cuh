@@ -31,12 +31,20 @@ constexpr int TILE_KEYS = 128;
 constexpr int TILE_ROWS = 128;
 
 // A bounded wait (2 s): false when it expires, or when another wait of the context has (the error word then holds a
-// code below 100; what a kernel finds wrong in a batch does not end waits).
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, int code) {
-    if (dg::mbar_try_wait(bar, parity)) return true;
+// code below 100; what a kernel finds wrong in a batch does not end waits). The loop is out of line: the kernels wait in
+// some twenty places, and with it inline a fifth of their stalls were for instructions.
+static __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, int* err, int code) {
     const uint64_t t0 = dg::globaltimer();
     for (uint32_t it = 1;; ++it) {
-        if (dg::mbar_try_wait(bar, parity)) return true;
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
         if ((it & 255u) == 0) {
             const int e = *(volatile int*)err;
             if (e > 0 && e < 100) return false;
@@ -46,6 +54,9 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, i
             }
         }
     }
+}
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+    return dg::mbar_try_wait(bar, parity) || wait_on(smem_u32(bar), parity, err, code);
 }
 
 // wait() by a whole warp.
