@@ -152,7 +152,7 @@ constexpr uint32_t MAGIC_BITS = 0x4B400000u;
 // 3 * 2^22, so what arrives is 3 * 2^22 + s as a float, and (3 * 2^22 + s) sigma - 3 * 2^22 sigma is one fused operation
 // whose constant is exact.
 __device__ __forceinline__ f2 scaled2(int32_t s0, int32_t s1, f2 sigma, f2 csigma) {
-    return fma2(pk(__int_as_float(s0), __int_as_float(s1)), sigma, csigma);
+    return fma2(pk(__int_as_float(s0 + (int)MAGIC_BITS), __int_as_float(s1 + (int)MAGIC_BITS)), sigma, csigma);
 }
 
 // What a row's weights need: the maximum, -theta, the cubic's coefficients times 2^-E, and 2^E.
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     const uint32_t qx = qd + x * (C::SLOT >> 4), kx = kd + ks * (C::SLOT >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        if (4 * x + kk < ksteps) umma(issue, tmem + b * 128, qx + 2 * kk, kx + 2 * kk, id_s, 1u);
+                        if (4 * x + kk < ksteps) umma(issue, tmem + b * 128, qx + 2 * kk, kx + 2 * kk, id_s, x + kk > 0);
                     umma_arrive(issue, &empty[ks]);
                     if (++ks == C::K_SLOTS) ks = 0, kph ^= 1;
                 }
@@ -584,8 +584,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         const int quad = warp & 3, part = (warp >> 2) & 1, grp = warp >> 3;
         const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
         const uint32_t s_addr = lane_addr + grp * 128 + part * 64;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) tmem_fill32(s_addr + (c >> 1) * 256 + (c & 1) * 32);
         // the queries' codes, from where query_kernel left them, into the K-major operand
         if (n_pass > 0) {
             const int per_row = dim / 16;
@@ -629,9 +627,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         auto load_scores = [&](uint32_t addr, int c, uint64_t* bar) {
             dg::tmem_ld32(addr + c * 32, s32);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            tmem_fill32(addr + c * 32);
             if (c == 1) {
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar);
