@@ -438,7 +438,6 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
         }
         return m;
     };
-    const float kc_of = -MAGIC;
     if (soft) {
         // the queries, up to B rows of one token at a time
         if (threadIdx.x < FEW_ROWS) s_pos[threadIdx.x] = threadIdx.x < n_rows ? len - n_new + (row0 + (int)threadIdx.x) / g : -1;
@@ -484,11 +483,10 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
             next_scores(i, i);
             if (!ok) break;
             const uint32_t m = seen_rows(tile_at(i) * TILE_KEYS);
-            const float kc = kc_of * kf;
 #pragma unroll
             for (int r = 0; r < FEW_ROWS; ++r) {
                 if (r >= n_rows) break;
-                const float x = __fmaf_rn(__int_as_float(s16[r] + (int)MAGIC_BITS), kf, kc);
+                const float x = __fmul_rn(__int2float_rn(s16[r]), kf);
                 if (m >> r & 1) {
                     top[r] = fmaxf(top[r], x);
                     sig[r] = max(sig[r], vf);
@@ -570,14 +568,14 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const uint32_t m = seen_rows(tile_at(i) * TILE_KEYS);
-            const float kc = kc_of * kf, sv = __uint_as_float(vf);
+            const float sv = __uint_as_float(vf);
             uint8_t* pp = sm + C::P + (i & 1) * 4096 + (key & 15);
             const int chunk = key >> 4;
 #pragma unroll
             for (int r = 0; r < FEW_ROWS; ++r) {
                 if (r >= n_rows) break;
                 const float4 row = s_row[r];
-                const float x = __fmaf_rn(__int_as_float(s16[r] + (int)MAGIC_BITS), kf, kc);
+                const float x = __fmul_rn(__int2float_rn(s16[r]), kf);
                 float w = weight(x, row.x, -row.y);
                 if (!(m >> r & 1)) w = 0.0f;
                 total[r] += __float_as_uint(__fadd_rn(w, MAGIC)) - MAGIC_BITS;

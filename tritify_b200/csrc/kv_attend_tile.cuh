@@ -137,22 +137,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const int32_t (&r)[16]
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 
-// 32 TMEM columns of 3 * 2^22, what the scores of a tile are summed onto (see scaled2).
-__device__ __forceinline__ void tmem_fill32(uint32_t taddr) {
-    const uint32_t v = 0x4B400000u;
-#pragma unroll
-    for (int c = 0; c < 32; c += 8)
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1};" ::"r"(taddr + c), "r"(v));
-}
-
 constexpr float MAGIC = 12582912.0f;  // 3 * 2^22: adding it rounds to a whole number, left in the low bits
 constexpr uint32_t MAGIC_BITS = 0x4B400000u;
 
-// Dot products s (|s| <= 2^22) of two adjacent keys times their scales, RN24. The products are summed onto the bits of
-// 3 * 2^22, so what arrives is 3 * 2^22 + s as a float, and (3 * 2^22 + s) sigma - 3 * 2^22 sigma is one fused operation
-// whose constant is exact.
-__device__ __forceinline__ f2 scaled2(int32_t s0, int32_t s1, f2 sigma, f2 csigma) {
-    return fma2(pk(__int_as_float(s0 + (int)MAGIC_BITS), __int_as_float(s1 + (int)MAGIC_BITS)), sigma, csigma);
+// Dot products (|s| <= 2^22, exact in binary32) of two adjacent keys times their scales, RN24.
+__device__ __forceinline__ f2 scaled2(int32_t s0, int32_t s1, f2 sigma) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pk(__int2float_rn(s0), __int2float_rn(s1))), "l"(sigma));
+    return r;
 }
 
 // What a row's weights need: the maximum, -theta, the cubic's coefficients times 2^-E, and 2^E.
@@ -252,8 +244,8 @@ struct TileCfg {
     static constexpr int P = Q + NK * SLOT;           // [2][hi, lo]
     static constexpr int RING = P + 4 * SLOT;
     static constexpr int CARRY = RING + SLOTS * SLOT;  // int16 [128 columns][128 rows]
-    // [SCALES]: sigma_k, -MAGIC sigma_k and sigma_v [128], the largest sigma_v
-    static constexpr int KEY_STAGE = 3 * TILE_KEYS + 4;
+    // [SCALES]: sigma_k and sigma_v [128], the largest sigma_v
+    static constexpr int KEY_STAGE = 2 * TILE_KEYS + 4;
     static constexpr int KEY_SCALES = CARRY + TILE_ROWS * 128 * 2;
     static constexpr int ROWS = KEY_SCALES + SCALES * KEY_STAGE * 4;  // theta, max [4], largest sigma [4], L [4]
     static constexpr int BARS = ROWS + TILE_ROWS * (4 + 16 + 16 + 32);
@@ -565,11 +557,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                                        __uint_as_float(w.y << 16), __uint_as_float(w.y & hi16)};
                     const uint4 vf = {w.z << 16, w.z & hi16, w.w << 16, w.w & hi16};
                     *(float4*)(f + 4 * lane) = kf;
-                    *(float4*)(f + TILE_KEYS + 4 * lane) = {-MAGIC * kf.x, -MAGIC * kf.y, -MAGIC * kf.z, -MAGIC * kf.w};
-                    *(uint4*)(f + 2 * TILE_KEYS + 4 * lane) = vf;
+                    *(uint4*)(f + TILE_KEYS + 4 * lane) = vf;
                     const unsigned big = max(max(vf.x, vf.y), max(vf.z, vf.w));
                     const unsigned tile_big = __reduce_max_sync(0xffffffffu, big);
-                    if (lane == 0) ((uint32_t*)f)[3 * TILE_KEYS] = tile_big;
+                    if (lane == 0) ((uint32_t*)f)[2 * TILE_KEYS] = tile_big;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&k_full[j]);
                     val[j] = scales_of(u + 4, pg[j]);
@@ -595,8 +586,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 if (c == 0) s_theta[r] = __int_as_float(x[dim / 4]);
             }
         }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        asm volatile("tcgen05.fence::before_thread_sync;");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
@@ -615,7 +604,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         };
         // the first tile of a pass that this group takes: scores number sc with sc % 2 == grp
         auto first_of = [&](int pass) { return (grp ^ (pass * n)) & 1; };
-        int32_t s32[32];
         // wait for scores number sc, the `use`th in their buffer, and their key scales
         auto next_scores = [&](uint64_t* bar, uint32_t use) {
             ok = wait(bar, use & 1u, a.err.word, dg::ERR_TIMEOUT_ACCUM) &&
@@ -624,13 +612,14 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             asm volatile("tcgen05.fence::after_thread_sync;");
         };
         // 32 of this thread's 64 scores; after the second half the buffer goes back to the products
-        auto load_scores = [&](uint32_t addr, int c, uint64_t* bar) {
-            dg::tmem_ld32(addr + c * 32, s32);
+        int32_t s32[32];
+        auto load_scores = [&](int c) {
+            dg::tmem_ld32(s_addr + c * 32, s32);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
             if (c == 1) {
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar);
+                if (lane == 0) mbar_arrive(&s_free[grp]);
             }
         };
         auto key_scales = [&]() { return (const float*)(sm + C::KEY_SCALES) + (sc % C::SCALES) * C::KEY_STAGE + part * 64; };
@@ -645,18 +634,24 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             if (!ok) break;
             const int j0 = kt_.at(i) * TILE_KEYS;
             const bool all = whole(j0);
-            if (all) sig = max(sig, ((const uint32_t*)key_scales())[3 * TILE_KEYS - part * 64]);
+            const float* f = key_scales();
+            if (all) sig = max(sig, ((const uint32_t*)f)[2 * TILE_KEYS - part * 64]);
+            int32_t s64[2][32];
+            dg::tmem_ld32(s_addr + (i & 2) * 128, s64[0]);
+            dg::tmem_ld32(s_addr + (i & 2) * 128 + 32, s64[1]);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&m_free[i & 3]);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const float* f = key_scales() + c * 32;
-                load_scores(s_addr + (i & 2) * 128, c, &m_free[i & 3]);
                 if (all) {
 #pragma unroll
                     for (int k = 0; k < 32; k += 4) {
-                        const ulonglong2 kf = *(const ulonglong2*)(f + k), kc = *(const ulonglong2*)(f + TILE_KEYS + k);
+                        const ulonglong2 kf = *(const ulonglong2*)(f + c * 32 + k);
                         float x0, x1, x2, x3;
-                        upk(scaled2(s32[k], s32[k + 1], kf.x, kc.x), x0, x1);
-                        upk(scaled2(s32[k + 2], s32[k + 3], kf.y, kc.y), x2, x3);
+                        upk(scaled2(s64[c][k], s64[c][k + 1], kf.x), x0, x1);
+                        upk(scaled2(s64[c][k + 2], s64[c][k + 3], kf.y), x2, x3);
                         top = fmaxf(fmaxf(top, x0), x1);
                         top = fmaxf(fmaxf(top, x2), x3);
                     }
@@ -664,10 +659,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     const uint32_t m = seen_bits(j0 + part * 64 + c * 32, pos, a.window, a.sinks);
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
-                        const f2 kf = *(const f2*)(f + k), kc = *(const f2*)(f + TILE_KEYS + k);
-                        const uint2 vf = *(const uint2*)(f + 2 * TILE_KEYS + k);
+                        const f2 kf = *(const f2*)(f + c * 32 + k);
+                        const uint2 vf = *(const uint2*)(f + TILE_KEYS + c * 32 + k);
                         float x0, x1;
-                        upk(scaled2(s32[k], s32[k + 1], kf, kc), x0, x1);
+                        upk(scaled2(s64[c][k], s64[c][k + 1], kf), x0, x1);
                         if (m >> k & 1) {
                             top = fmaxf(top, x0);
                             sig = max(sig, vf.x);
@@ -748,7 +743,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 #pragma unroll 1
                 for (int c = 0; c < 2; ++c) {
                     const float* f = key_scales() + c * 32;
-                    load_scores(s_addr, c, &s_free[grp]);
+                    load_scores(c);
                     auto digits = [&](auto mask_tag, uint32_t seen) {
                         constexpr bool MASK = decltype(mask_tag)::value;
 #pragma unroll
@@ -758,11 +753,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                             for (int k4 = 0; k4 < 4; ++k4) {
                                 const int k = k16 + 4 * k4;
                                 const ulonglong2 kf = *(const ulonglong2*)(f + k);
-                                const ulonglong2 kc = *(const ulonglong2*)(f + TILE_KEYS + k);
-                                const ulonglong2 vf = *(const ulonglong2*)(f + 2 * TILE_KEYS + k);
+                                const ulonglong2 vf = *(const ulonglong2*)(f + TILE_KEYS + k);
                                 const uint32_t m = MASK ? seen >> k : 0u;
-                                const f2 w0 = weight2<MASK>(scaled2(s32[k], s32[k + 1], kf.x, kc.x), rw, m);
-                                const f2 w1 = weight2<MASK>(scaled2(s32[k + 2], s32[k + 3], kf.y, kc.y), rw, m >> 2);
+                                const f2 w0 = weight2<MASK>(scaled2(s32[k], s32[k + 1], kf.x), rw, m);
+                                const f2 w1 = weight2<MASK>(scaled2(s32[k + 2], s32[k + 3], kf.y), rw, m >> 2);
                                 const f2 mg = pk(MAGIC, MAGIC), mg128 = pk(MAGIC + 128.0f, MAGIC + 128.0f);
                                 float a0, a1, a2, a3;
                                 upk(fma2(w0, rw.two_e, mg), a0, a1);
