@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
                     for (int b = 0; b < NK; ++b)
                         if (i < count && 4 * lane + 128 * b < dim)
                             *(uint32_t*)(sm + C::Q + b * 2048 + ri * 128 + (((lane >> 2) ^ (ri & 7)) << 4) + 4 * (lane & 3)) =
-                                codes4<false>(rows.y[i][b], mi);
+                                codes4(rows.y[i][b], mi);
                 }
             }
         }

@@ -74,12 +74,30 @@ int make_pool_map(ktmoe_ctx* ctx, CUtensorMap* map, const int8_t* pool, const kv
     return KTMOE_OK;
 }
 
-unsigned row_blocks(int64_t warps) { return (unsigned)((warps + kv::ROW_WARPS - 1) / kv::ROW_WARPS); }
+// Blocks of ROW_WARPS warps, a warp per row and chunk of its heads.
+int row_blocks(ktmoe_ctx* ctx, int64_t rows, int chunks, unsigned* blocks) {
+    const int64_t n = (rows * chunks + kv::ROW_WARPS - 1) / kv::ROW_WARPS;
+    if (n > INT32_MAX) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "too many rows for one launch");
+    *blocks = (unsigned)n;
+    return KTMOE_OK;
+}
 
 template <int NB>
 int launch_append(ktmoe_ctx* ctx, cudaStream_t st, const kv::AppendArgs& a) {
     const int chunks = (a.c.heads + kv::RowBatch<NB>::B - 1) / kv::RowBatch<NB>::B;
-    KLAUNCH(st, row_blocks(a.b.rows * 2 * chunks), 32 * kv::ROW_WARPS, 0, (kv::append_kernel<NB>), a, chunks);
+    unsigned blocks;
+    if (int r = row_blocks(ctx, a.b.rows, 2 * chunks, &blocks)) return r;
+    KLAUNCH(st, blocks, 32 * kv::ROW_WARPS, 0, (kv::append_kernel<NB>), a, chunks);
+    return KTMOE_OK;
+}
+
+template <int NB>
+int launch_read(ktmoe_ctx* ctx, cudaStream_t st, const kv::ReadArgs& a) {
+    constexpr int B = kv::READ_ROWS / NB;
+    const int chunks = (2 * a.c.heads + B - 1) / B;
+    unsigned blocks;
+    if (int r = row_blocks(ctx, a.b.rows, chunks, &blocks)) return r;
+    KLAUNCH(st, blocks, 32 * kv::ROW_WARPS, 0, (kv::read_kernel<NB>), a, chunks);
     return KTMOE_OK;
 }
 
@@ -97,7 +115,9 @@ int launch_tile(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
     if (int r = make_pool_map(ctx, &mk, a.c.k, a.c)) return r;
     if (int r = make_pool_map(ctx, &mv, a.c.v, a.c)) return r;
     const int chunks = (a.c.heads * a.group + kv::RowBatch<NK>::B - 1) / kv::RowBatch<NK>::B;
-    KLAUNCH(st, row_blocks(a.b.rows * chunks), 32 * kv::ROW_WARPS, 0, (kv::query_kernel<NK>), a, chunks);
+    unsigned blocks;
+    if (int r = row_blocks(ctx, a.b.rows, chunks, &blocks)) return r;
+    KLAUNCH(st, blocks, 32 * kv::ROW_WARPS, 0, (kv::query_kernel<NK>), a, chunks);
     KLAUNCH(st, (unsigned)(slots * a.c.heads), kv::TILE_THREADS, kv::TileCfg<NK>::BYTES, (kv::attend_tile_kernel<NK>), mk,
             mv, a, (long long)slots);
     return KTMOE_OK;
@@ -208,8 +228,7 @@ int ktmoe_kv_read_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_k
     a.ld_v = ld_v;
     a.vec = aligned(k, 16) && aligned(v, 16) && ld_k % 4 == 0 && ld_v % 4 == 0;
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
-    KLAUNCH(st, (unsigned)batch->rows, 32 * kv::READ_WARPS, 0, (kv::read_kernel), a);
-    return KTMOE_OK;
+    return a.c.dim <= 128 ? launch_read<1>(ctx, st, a) : launch_read<2>(ctx, st, a);
 }
 
 int ktmoe_attention_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* q,

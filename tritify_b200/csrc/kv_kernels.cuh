@@ -97,19 +97,12 @@ __device__ __forceinline__ long long pool_page(const Batch& b, const Cache& c, c
     return page;
 }
 
-__device__ __forceinline__ uint64_t uabs(int64_t v) { return v < 0 ? (uint64_t)(-v) : (uint64_t)v; }
-
-__device__ __forceinline__ uint64_t warp_umax(uint64_t v) {
-    const uint32_t hi = (uint32_t)(v >> 32);
-    const uint32_t mh = __reduce_max_sync(0xffffffffu, hi);
-    const uint32_t ml = __reduce_max_sync(0xffffffffu, hi == mh ? (uint32_t)v : 0u);
-    return (uint64_t)mh << 32 | ml;
-}
-
-// A scale in float64, its shift held within [-900, 2000] so that the value is finite; `extra_shift` more places down.
+// A scale in float64, its shift held within [-900, 2000] so that the value is finite; `extra_shift` (at most 30) more
+// places down. The power of two in halves: the first product is a normal number, so only the second one rounds.
 __device__ __forceinline__ double scale_value(longlong2 s, int extra_shift) {
-    const int shift = max(-900, min(2000, (int)s.y)) + extra_shift;
-    return s.x <= 0 ? 0.0 : ldexp((double)s.x, -shift);
+    const int shift = max(-900, min(2000, (int)s.y)) + extra_shift, half = shift >> 1;
+    if (s.x <= 0) return 0.0;
+    return (double)s.x * __hiloint2double((1023 - half) << 20, 0) * __hiloint2double((1023 - (shift - half)) << 20, 0);
 }
 
 // Element e of a row after the rotation. x: the row; cs: its row of the rotation table.
@@ -166,6 +159,8 @@ __device__ __forceinline__ double to_double(int32_t v) {
 }
 __device__ __forceinline__ int to_int(double v) { return __double2loint(__dadd_rn(v, 6755399441055744.0)); }
 
+__device__ __forceinline__ uint32_t uabs(int32_t v) { return v < 0 ? 0u - (uint32_t)v : (uint32_t)v; }
+
 // ── rows of codes: rotation, largest element, quantisation ──
 // A warp takes up to B heads of one token, which share the rotation's entries, the scale and one division; lane l has
 // the elements 4 l .. 4 l + 3 of each 128 (NB of them). Elements are turned into RN64 of their codes at once, which is
@@ -199,19 +194,20 @@ template <int NB>
 __device__ __forceinline__ RawBatch<NB> fetch_rows(const int32_t* __restrict__ x, int heads, int dim, int vec, const Rope& r) {
     const int lane = threadIdx.x & 31;
     const bool far = r.table && turns_by_four(r) && !r.interleaved;
-    auto four = [&](const int32_t* p) {
-        return vec ? __ldg((const int4*)p) : make_int4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
-    };
     RawBatch<NB> w;
+    auto fetch = [&](auto four) {
 #pragma unroll
-    for (int i = 0; i < RowBatch<NB>::B; ++i)
+        for (int i = 0; i < RowBatch<NB>::B; ++i)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int e = 4 * lane + 128 * b;
-            w.v[i][b] = w.o[i][b] = make_int4(0, 0, 0, 0);
-            if (i < heads && e < dim) w.v[i][b] = four(x + i * dim + e);
-            if (far && i < heads && e < 2 * r.half) w.o[i][b] = four(x + i * dim + (e < r.half ? e + r.half : e - r.half));
-        }
+            for (int b = 0; b < NB; ++b) {
+                const int e = 4 * lane + 128 * b;
+                w.v[i][b] = w.o[i][b] = make_int4(0, 0, 0, 0);
+                if (i < heads && e < dim) w.v[i][b] = four(x + i * dim + e);
+                if (far && i < heads && e < 2 * r.half) w.o[i][b] = four(x + i * dim + (e < r.half ? e + r.half : e - r.half));
+            }
+    };
+    if (vec) fetch([](const int32_t* p) { return __ldg((const int4*)p); });
+    else fetch([](const int32_t* p) { return make_int4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3)); });
     return w;
 }
 
@@ -258,6 +254,18 @@ __device__ __forceinline__ void turn_rows(RowBatch<NB>& out, const RawBatch<NB>&
                     out.y[i][b][k] = i < heads && e < dim ? to_double(rotated(x + i * dim, e, r, cs)) : 0.0;
                 }
     }
+    if (!cs) {  // the elements are whole 32-bit numbers
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                most = max(max(most, max(uabs(v[i][b].x), uabs(v[i][b].y))), max(uabs(v[i][b].z), uabs(v[i][b].w)));
+            most = __reduce_max_sync(0xffffffffu, most);
+            if (lane == i || i == 0) out.top = (double)most;
+        }
+        return;
+    }
     // the largest: the upper words of |y| first, then the lower words of those that have it
 #pragma unroll
     for (int i = 0; i < B; ++i) {
@@ -278,16 +286,11 @@ __device__ __forceinline__ void turn_rows(RowBatch<NB>& out, const RawBatch<NB>&
     }
 }
 
-// rne(RN64(y m)) of four elements, as the bytes of a word; CLAMP: held within +-127.
-template <bool CLAMP>
+// rne(RN64(y m)) of four elements, |y m| < 2^31, as the bytes of a word.
 __device__ __forceinline__ uint32_t codes4(const double (&y)[4], double m) {
     int c[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const double v = __dmul_rn(y[k], m);
-        // beyond 2^31 to_int does not hold
-        c[k] = CLAMP ? to_int(fmin(fmax(v, -127.0), 127.0)) : to_int(v);
-    }
+    for (int k = 0; k < 4; ++k) c[k] = to_int(__dmul_rn(y[k], m));
     return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
@@ -330,8 +333,21 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) append_kernel(const AppendArgs
     RowBatch<NB> rows;
     turn_rows<NB>(rows, raw, x, heads, dim, rope, cs);
     const double s = scale_value(sc, cs ? 30 : 0);
-    const uint32_t sg = sigma_bits(__ddiv_rn(__dmul_rn(rows.top, s), 127.0));
+    const double want = __ddiv_rn(__dmul_rn(rows.top, s), 127.0);
+    const uint32_t sg = sigma_bits(want);
     const double m = __ddiv_rn(s, (double)bf16_value(sg));
+    // sigma >= want, so that |y m| <= 127 (1 + 2^-51) and the codes stay within +-127; but for rows whose scale would
+    // be above the largest sigma, 2^63: those are held within +-127 first
+    if (__any_sync(0xffffffffu, want > 0x1p63)) {
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const double mi = __shfl_sync(0xffffffffu, m, i), limit = __ddiv_rn(127.0, mi);
+            if (__shfl_sync(0xffffffffu, want, i) > 0x1p63)
+#pragma unroll
+                for (int j = 0; j < 4 * NB; ++j)
+                    rows.y[i][j / 4][j % 4] = fmin(fmax(rows.y[i][j / 4][j % 4], -limit), limit);
+        }
+    }
     const long long row0 = ((page * a.c.heads + h0) << a.c.page_shift) + (p.pos & ((1 << a.c.page_shift) - 1));
     if (lane < heads) (is_v ? a.c.vs : a.c.ks)[row0 + ((long long)lane << a.c.page_shift)] = (uint16_t)sg;
 #pragma unroll
@@ -341,12 +357,13 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) append_kernel(const AppendArgs
 #pragma unroll
         for (int b = 0; b < NB; ++b)
             if (i < heads && 4 * lane + 128 * b < dim)
-                *(uint32_t*)(dst + 4 * lane + 128 * b) = codes4<true>(rows.y[i][b], mi);
+                *(uint32_t*)(dst + 4 * lane + 128 * b) = codes4(rows.y[i][b], mi);
     }
 }
 
 // ── reading back ──
-constexpr int READ_WARPS = 8;
+// A warp per token and eight rows (four of more than 128 elements): all its codes and scales are asked for together.
+constexpr int READ_ROWS = 8;
 
 struct ReadArgs {
     Cache c;
@@ -357,26 +374,43 @@ struct ReadArgs {
     int vec;
 };
 
-__global__ void __launch_bounds__(32 * READ_WARPS) read_kernel(const ReadArgs a) {
+template <int NB>
+__global__ void __launch_bounds__(32 * ROW_WARPS) read_kernel(const ReadArgs a, int chunks) {
     kt::pdl_enter();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int t = blockIdx.x;
+    constexpr int B = READ_ROWS / NB;
+    const int lane = threadIdx.x & 31, dim = a.c.dim;
+    const long long u = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    const int t = (int)(u / chunks), r0 = (int)(u % chunks) * B, rows = min(B, 2 * a.c.heads - r0);
+    if (t >= a.b.rows) return;
     Place p;
     if (!locate(a.b, a.err, t, a.c.page_shift, p) || p.pos < 0) return;
     const long long page = pool_page(a.b, a.c, a.err, p.seq, p.pos >> a.c.page_shift);
     const int in_page = p.pos & ((1 << a.c.page_shift) - 1);
-    const int dim = a.c.dim;
-    for (int r = warp; r < 2 * a.c.heads; r += READ_WARPS) {
-        const bool is_v = r >= a.c.heads;
-        const int h = is_v ? r - a.c.heads : r;
-        const long long row = ((page * a.c.heads + h) << a.c.page_shift) + in_page;
-        const int8_t* src = (is_v ? a.c.v : a.c.k) + row * dim;
-        const float sg = bf16_value((is_v ? a.c.vs : a.c.ks)[row]);
-        float* dst = (is_v ? a.v + (long long)t * a.ld_v : a.k + (long long)t * a.ld_k) + (long long)h * dim;
-        for (int e = 4 * lane; e < dim; e += 128) {
-            const char4 o = *(const char4*)(src + e);
-            const float4 f = {__fmul_rn((float)o.x, sg), __fmul_rn((float)o.y, sg), __fmul_rn((float)o.z, sg),
-                              __fmul_rn((float)o.w, sg)};  // 7 by 8 significant bits: exact
+    const long long row0 = ((page * a.c.heads) << a.c.page_shift) + in_page;
+    uint32_t code[B][NB];
+    float sigma[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        if (i >= rows) break;
+        const bool is_v = r0 + i >= a.c.heads;
+        const long long row = row0 + ((long long)(r0 + i - (is_v ? a.c.heads : 0)) << a.c.page_shift);
+        sigma[i] = bf16_value((is_v ? a.c.vs : a.c.ks)[row]);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            if (4 * lane + 128 * b < dim) code[i][b] = *(const uint32_t*)((is_v ? a.c.v : a.c.k) + row * dim + 4 * lane + 128 * b);
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        if (i >= rows) break;
+        const bool is_v = r0 + i >= a.c.heads;
+        float* dst = (is_v ? a.v + (long long)t * a.ld_v - (long long)a.c.heads * dim : a.k + (long long)t * a.ld_k) + (long long)(r0 + i) * dim;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int e = 4 * lane + 128 * b;
+            if (e >= dim) continue;
+            const char4 o = *(const char4*)&code[i][b];
+            const float4 f = {__fmul_rn((float)o.x, sigma[i]), __fmul_rn((float)o.y, sigma[i]), __fmul_rn((float)o.z, sigma[i]),
+                              __fmul_rn((float)o.w, sigma[i])};  // 7 by 8 significant bits: exact
             if (a.vec) {
                 *(float4*)(dst + e) = f;
             } else {
@@ -466,7 +500,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) query_kernel(const AttendArgs 
         const double mi = __shfl_sync(0xffffffffu, m, i);
 #pragma unroll
         for (int b = 0; b < NB; ++b)  // |y m| <= 127 (1 + 2^-52): the codes stay within +-127
-            if (i < heads && 4 * lane + 128 * b < dim) out[i * dim + lane + 32 * b] = (int)codes4<false>(rows.y[i][b], mi);
+            if (i < heads && 4 * lane + 128 * b < dim) out[i * dim + lane + 32 * b] = (int)codes4(rows.y[i][b], mi);
     }
 }
 
