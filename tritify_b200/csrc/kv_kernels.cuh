@@ -146,17 +146,12 @@ __device__ __forceinline__ uint32_t sigma_bits(double t) {
 
 __device__ __forceinline__ float bf16_value(uint32_t bits) { return __uint_as_float(bits << 16); }
 
-// RN64 of a 64-bit integer and the nearest whole number to a double (ties to even, |v| < 2^31) on the FP64 pipe: the
-// conversion instructions run at a quarter of its rate. 2^52 + 2^31 + hi and 2^52 + lo are doubles whose low words are
-// the integer's halves.
-__device__ __forceinline__ double to_double(int64_t v) {
-    const double hi = __dsub_rn(__hiloint2double(0x43300000, (int)(v >> 32) ^ (int)0x80000000), 4503601774854144.0);
-    const double lo = __dsub_rn(__hiloint2double(0x43300000, (int)v), 4503599627370496.0);
-    return __fma_rn(hi, 4294967296.0, lo);
-}
-__device__ __forceinline__ double to_double(int32_t v) {
-    return __dsub_rn(__hiloint2double(0x43300000, v ^ (int)0x80000000), 4503601774854144.0);
-}
+// RN64 of an integer, and the nearest whole number to a double (ties to even, |v| < 2^31): the addition leaves it in the
+// low word. The conversions run at a quarter of the FP64 pipe's rate, but put nothing on the pipe of the integer
+// operations, which has the most to do here: built of those and FP64 additions instead, the decode of 64 sequences of
+// 4096 took 121 us against 117, a window's 8192 tokens 563 against 551.
+__device__ __forceinline__ double to_double(int64_t v) { return __ll2double_rn(v); }
+__device__ __forceinline__ double to_double(int32_t v) { return __int2double_rn(v); }
 __device__ __forceinline__ int to_int(double v) { return __double2loint(__dadd_rn(v, 6755399441055744.0)); }
 
 __device__ __forceinline__ uint32_t uabs(int32_t v) { return v < 0 ? 0u - (uint32_t)v : (uint32_t)v; }
