@@ -74,20 +74,19 @@ int make_pool_map(ktmoe_ctx* ctx, CUtensorMap* map, const int8_t* pool, const kv
     return KTMOE_OK;
 }
 
-// Blocks of ROW_WARPS warps, a warp per row and chunk of its heads.
+// Blocks of ROW_WARPS warps, a warp per row and chunk of its heads (counted in 32 bits on the device).
 int row_blocks(ktmoe_ctx* ctx, int64_t rows, int chunks, unsigned* blocks) {
-    const int64_t n = (rows * chunks + kv::ROW_WARPS - 1) / kv::ROW_WARPS;
-    if (n > INT32_MAX) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "too many rows for one launch");
-    *blocks = (unsigned)n;
+    if (rows * chunks > INT32_MAX) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "too many rows for one launch");
+    *blocks = (unsigned)((rows * chunks + kv::ROW_WARPS - 1) / kv::ROW_WARPS);
     return KTMOE_OK;
 }
 
 template <int NB>
 int launch_append(ktmoe_ctx* ctx, cudaStream_t st, const kv::AppendArgs& a) {
-    const int chunks = (a.c.heads + kv::RowBatch<NB>::B - 1) / kv::RowBatch<NB>::B;
+    const int chunks = 2 * ((a.c.heads + kv::RowBatch<NB>::B - 1) / kv::RowBatch<NB>::B);  // of keys and of values
     unsigned blocks;
-    if (int r = row_blocks(ctx, a.b.rows, 2 * chunks, &blocks)) return r;
-    KLAUNCH(st, blocks, 32 * kv::ROW_WARPS, 0, (kv::append_kernel<NB>), a, chunks);
+    if (int r = row_blocks(ctx, a.b.rows, chunks, &blocks)) return r;
+    KLAUNCH(st, blocks, 32 * kv::ROW_WARPS, 0, (kv::append_kernel<NB>), a, (unsigned)chunks);
     return KTMOE_OK;
 }
 
@@ -97,7 +96,7 @@ int launch_read(ktmoe_ctx* ctx, cudaStream_t st, const kv::ReadArgs& a) {
     const int chunks = (2 * a.c.heads + B - 1) / B;
     unsigned blocks;
     if (int r = row_blocks(ctx, a.b.rows, chunks, &blocks)) return r;
-    KLAUNCH(st, blocks, 32 * kv::ROW_WARPS, 0, (kv::read_kernel<NB>), a, chunks);
+    KLAUNCH(st, blocks, 32 * kv::ROW_WARPS, 0, (kv::read_kernel<NB>), a, (unsigned)chunks);
     return KTMOE_OK;
 }
 
@@ -117,7 +116,7 @@ int launch_tile(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
     const int chunks = (a.c.heads * a.group + kv::RowBatch<NK>::B - 1) / kv::RowBatch<NK>::B;
     unsigned blocks;
     if (int r = row_blocks(ctx, a.b.rows, chunks, &blocks)) return r;
-    KLAUNCH(st, blocks, 32 * kv::ROW_WARPS, 0, (kv::query_kernel<NK>), a, chunks);
+    KLAUNCH(st, blocks, 32 * kv::ROW_WARPS, 0, (kv::query_kernel<NK>), a, (unsigned)chunks);
     KLAUNCH(st, (unsigned)(slots * a.c.heads), kv::TILE_THREADS, kv::TileCfg<NK>::BYTES, (kv::attend_tile_kernel<NK>), mk,
             mv, a, (long long)slots);
     return KTMOE_OK;

@@ -290,8 +290,10 @@ __device__ __forceinline__ uint32_t codes4(const double (&y)[4], double m) {
 }
 
 // ── writing ──
-// A warp per (token, keys or values, up to four KV heads). Bound by memory at large sizes: 4 bytes read and 1 written
-// per element.
+// A warp per (token, keys or values, up to four KV heads). Four bytes are read and one written per element; bound by the
+// instructions all the same (about 45 an element and lane: the exact products, conversions, the largest, two divisions
+// a warp): 16384 tokens of 8 + 8 heads of 128, 168 MB, take 68 us. Eight blocks an SM although a few registers are
+// spilled: with six, and none, writing and reading those tokens took 107 us against 99.
 struct AppendArgs {
     Cache c;
     Batch b;
@@ -307,15 +309,16 @@ struct AppendArgs {
 constexpr int ROW_WARPS = 4;
 
 template <int NB>
-__global__ void __launch_bounds__(32 * ROW_WARPS) append_kernel(const AppendArgs a, int chunks) {
+__global__ void __launch_bounds__(32 * ROW_WARPS, 8) append_kernel(const AppendArgs a, unsigned chunks) {
     kt::pdl_enter();
     constexpr int B = RowBatch<NB>::B;
     const int lane = threadIdx.x & 31, dim = a.c.dim;
-    const long long u = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
-    const int t = (int)(u / (2 * chunks)), c = (int)(u % (2 * chunks));
+    const unsigned u = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    const int t = (int)(u / chunks), c = (int)(u % chunks);
     if (t >= a.b.rows) return;
-    const bool is_v = c >= chunks;
-    const int h0 = (is_v ? c - chunks : c) * B, heads = min(B, a.c.heads - h0);
+    const int half = (int)chunks / 2;
+    const bool is_v = c >= half;
+    const int h0 = (is_v ? c - half : c) * B, heads = min(B, a.c.heads - h0);
     const int32_t* x = (is_v ? a.v + (long long)t * a.ld_v : a.k + (long long)t * a.ld_k) + (long long)h0 * dim;
     Rope rope = a.rope;
     if (is_v) rope.table = nullptr;
@@ -370,11 +373,11 @@ struct ReadArgs {
 };
 
 template <int NB>
-__global__ void __launch_bounds__(32 * ROW_WARPS) read_kernel(const ReadArgs a, int chunks) {
+__global__ void __launch_bounds__(32 * ROW_WARPS) read_kernel(const ReadArgs a, unsigned chunks) {
     kt::pdl_enter();
     constexpr int B = READ_ROWS / NB;
     const int lane = threadIdx.x & 31, dim = a.c.dim;
-    const long long u = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    const unsigned u = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
     const int t = (int)(u / chunks), r0 = (int)(u % chunks) * B, rows = min(B, 2 * a.c.heads - r0);
     if (t >= a.b.rows) return;
     Place p;
@@ -470,11 +473,11 @@ __device__ __forceinline__ float row_theta(double top, double s, double soft) {
 // hold the head_dim codes, then theta; whoever reads them writes the output over them. No other memory is needed. Bound
 // by memory at large sizes: 4 bytes read and 1 written per element.
 template <int NB>
-__global__ void __launch_bounds__(32 * ROW_WARPS) query_kernel(const AttendArgs a, int chunks) {
+__global__ void __launch_bounds__(32 * ROW_WARPS, 8) query_kernel(const AttendArgs a, unsigned chunks) {
     kt::pdl_enter();
     constexpr int B = RowBatch<NB>::B;
     const int lane = threadIdx.x & 31, dim = a.c.dim;
-    const long long u = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    const unsigned u = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
     const int t = (int)(u / chunks), h0 = (int)(u % chunks) * B, heads = min(B, a.c.heads * a.group - h0);
     if (t >= a.b.rows) return;
     const int32_t* x = a.q + (long long)t * a.ld_q + (long long)h0 * dim;
