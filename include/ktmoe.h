@@ -253,7 +253,7 @@ int ktmoe_layer_debug_fetch(ktmoe_layer* layer, int32_t which, void* host, int64
  * The cache: a row is one token's key or value of one KV head, int8 codes within +-127 at a scale sigma of 8
  * significant bits (stored as bfloat16). Pools are device memory of the caller, the same layout for K and V: codes
  * [n_pages][n_kv_heads][page_tokens][head_dim], scales [n_pages][n_kv_heads][page_tokens]. head_dim is a multiple of
- * 16 from 16 to 256, page_tokens 16, 32, 64 or 128; the code pools are 16-byte aligned. */
+ * 16 from 16 to 256, page_tokens 16, 32, 64 or 128, 1 to 1024 KV heads; the four pools are 16-byte aligned. */
 typedef struct ktmoe_kv_cache {
     int8_t* k;
     int8_t* v;
@@ -272,7 +272,8 @@ typedef struct ktmoe_kv_cache {
  * are. A row at a negative position (a length below the new tokens) has no place in the cache: append and read skip
  * it, attention gives zeros. What only the device can see wrong (a page outside the pool, offsets that do not ascend
  * or leave the rows, a length beyond the page table, a position beyond the rotation table) touches nothing outside
- * the buffers and makes the next ktmoe_sync on the context return KTMOE_ERR_ARG; results of that batch are undefined. */
+ * the buffers and makes the next ktmoe_sync on the context return KTMOE_ERR_ARG; results of that batch are undefined,
+ * other work on the context is not disturbed. At most 2^30 rows and 2^24 tokens a sequence (max_pages * page_tokens). */
 typedef struct ktmoe_kv_batch {
     int32_t n_seqs;
     int32_t max_pages;
@@ -350,7 +351,9 @@ int ktmoe_attn_set_rope(ktmoe_attn* attn, double theta, int32_t rot_dim, int64_t
 int ktmoe_attn_set_mask(ktmoe_attn* attn, double softmax_scale, int32_t window, int32_t sinks);
 /* The half on device buffers x, y [batch->rows][d_model] with their scales (x may be y), stream-ordered and not
  * synchronised; the new keys and values go into `cache` before the attention reads it. The object's scratch serves one
- * forward at a time (order calls that share it) and grows with the rows (not while a stream is captured). */
+ * forward at a time (order calls that share it, replays of captured ones among them) and grows with the rows: a capture
+ * needs a forward of as many rows before it (else KTMOE_ERR_STATE). A captured forward keeps the scales, rotation and
+ * mask of its capture. Destroy the object before its context, and its graphs before the object. */
 int ktmoe_attn_forward_dev(ktmoe_attn* attn, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch,
                            const int32_t* x_dev, const ktmoe_scale* x_scale_dev, int32_t* y_dev,
                            ktmoe_scale* y_scale_dev, void* stream);

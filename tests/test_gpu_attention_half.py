@@ -250,3 +250,54 @@ def test_refusals(ctx):
     with pytest.raises(tb.KtmoeError) as e:
         a.set_qkv(tb.QuantLinear("q", bad, tb.Scale(1, 0), 32, 64), lin(16, 64), lin(16, 64))
     assert e.value.status == _native.ERR_RANGE
+
+
+def test_a_context_closed_first(ctx):
+    """The half ends with its context; what is called on it afterwards is refused."""
+    own = tb.Context(0)
+    a, b = tb.AttentionHalf(own, 64, 2, 1, 16), tb.AttentionHalf(own, 64, 2, 1, 16)
+    del b
+    own.close()
+    with pytest.raises(tb.KtmoeError):
+        a.set_mask(window=3)
+    del a
+    own.close()
+    ctx.sync()
+
+
+def test_captured_forwards(ctx, oracle):
+    """A step captured into a graph, the scratch outgrown by a longer batch and the rotation changed after that, and the
+    graph replayed: what the capture gave. A capture that would grow the scratch is refused and the stream's capture
+    goes on."""
+    import torch
+
+    half = Half(ctx, 64, 4, 2, 16, 16, 12, 700, (1e4, 16, 64))
+    _, _, prompt = batch_of([(9, 9)], [[1, 2, 3, 4]])
+    run_half(ctx, half, *x_of(9, 64, 1), prompt)
+    _, _, one = batch_of([(1, 10)], [[1, 2, 3, 4]])
+    x, xs = x_of(1, 64, 2)
+    want = run_half(ctx, half, x, xs, one)  # writes position 9, as each replay does
+    xd = torch.from_numpy(np.ascontiguousarray(x)).cuda()
+    s = torch.tensor([xs[0], xs[1] & 0xFFFFFFFF], dtype=torch.int64, device="cuda")
+    yd, ys = torch.empty_like(xd), torch.zeros(2, dtype=torch.int64, device="cuda")
+    _, _, long = batch_of([(40, 50)], [[1, 2, 3, 4]])
+    xl = torch.zeros(40, 64, dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        at = torch.cuda.current_stream().cuda_stream
+        half.dev.forward_dev(half.cache, one, xd.data_ptr(), s.data_ptr(), yd.data_ptr(), ys.data_ptr(), at)
+        with pytest.raises(tb.KtmoeError) as e:
+            half.dev.forward_dev(half.cache, long, xl.data_ptr(), s.data_ptr(), xl.data_ptr(), ys.data_ptr(), at)
+        assert e.value.status == _native.ERR_STATE
+    _, _, other = batch_of([(40, 40)], [[6, 7, 8, 9]])
+    run_half(ctx, half, *x_of(40, 64, 3), other)
+    half.dev.set_rope(5e3, 16, 4096)
+    for _ in range(2):
+        yd.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        ctx.sync()
+        assert (yd.cpu().numpy() == want[0]).all()
+        a, b = ys.cpu().tolist()
+        assert (a, (b & 0xFFFFFFFF) - (1 << 32) if b & 1 << 31 else b & 0xFFFFFFFF) == want[1]

@@ -434,7 +434,7 @@ def test_two_streams_and_a_replayed_graph(ctx):
     ctx.sync()
 
 
-@pytest.mark.parametrize("what", ["page", "negative_page", "long", "negative", "descending", "rows", "position"])
+@pytest.mark.parametrize("what", ["page", "negative_page", "long", "longest", "negative", "descending", "rows", "position"])
 @pytest.mark.parametrize("new", [1, 40])
 def test_wrong_batches_are_reported_and_harmless(ctx, what, new):
     """What only the device can see: the calls touch nothing outside their buffers, sync reports it, and the context
@@ -448,6 +448,8 @@ def test_wrong_batches_are_reported_and_harmless(ctx, what, new):
         s.batch.page_table[0, 0] = -1
     elif what == "long":
         s.batch.kv_len[1] = s.max_pages * 16 + 1
+    elif what == "longest":
+        s.batch.kv_len[1] = 2 ** 31 - 1  # rounded up to pages it would pass 32 bits
     elif what == "negative":
         s.batch.kv_len[0] = -3
     elif what == "descending":
@@ -481,6 +483,27 @@ def test_wrong_batches_are_reported_and_harmless(ctx, what, new):
     assert (guard[0] == 77).all() and (guard[-1] == 77).all()
     assert (ko[0] == 7).all() and (ko[-1] == 7).all()
     Setup(ctx, [(new, 100)], 4, 2, 64, 16).check(s.codes(256)[:new], s.scales()[:new])
+
+
+def test_a_wrong_batch_leaves_other_work_alone(ctx):
+    """Between a wrong batch and the sync that reports it, linears run and report for themselves."""
+    torch = _torch()
+    s = Setup(ctx, [(1, 100)], 4, 2, 64, 16)
+    s.batch.page_table[0, 2] = s.cache.n_pages
+    q = torch.from_numpy(s.codes(256)).cuda()
+    scale = torch.from_numpy(s.scales()).cuda()
+    out, os_ = torch.zeros_like(q), torch.zeros(1, 2, 2, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    s.cache.attention(s.batch, q, scale, out, os_, 4)
+    torch.cuda.synchronize()
+    rng = np.random.default_rng(5)
+    x, w = rng.integers(-1000, 1000, (96, 256), dtype=np.int32), rng.integers(-1000, 1000, (128, 256), dtype=np.int32)
+    y = ctx.linear(x, w, 96, 128, 256)
+    assert (np.asarray(y).reshape(96, 128) == x.astype(np.int64) @ w.astype(np.int64).T).all()
+    with pytest.raises(tb.KtmoeError) as e:
+        ctx.sync()
+    assert e.value.status == _native.ERR_ARG
+    ctx.sync()
 
 
 def test_nothing_to_do(ctx):
@@ -529,6 +552,8 @@ def test_refusals_of_the_c_entry_points(ctx):
     rope = lambda **kw: _native.KtmoeRope(*{**dict(table=table.data_ptr(), positions=4, rot_dim=16, interleaved=0), **kw}.values())
     for kw, want in [
         (dict(c=cache(k=0)), ARG), (dict(c=cache(v_scale=0)), ARG), (dict(c=cache(k=s.cache.k.data_ptr() + 8)), ARG),
+        (dict(c=cache(v=s.cache.v.data_ptr() + 8)), ARG), (dict(c=cache(k_scale=s.cache.k_scale.data_ptr() + 8)), ARG),
+        (dict(c=cache(v_scale=s.cache.v_scale.data_ptr() + 8)), ARG),
         (dict(c=cache(head_dim=24)), UNS), (dict(c=cache(head_dim=272)), UNS), (dict(c=cache(head_dim=0)), UNS),
         (dict(c=cache(page_tokens=8)), UNS), (dict(c=cache(page_tokens=48)), UNS), (dict(c=cache(page_tokens=256)), UNS),
         (dict(c=cache(n_pages=0)), ARG), (dict(c=cache(n_kv_heads=0)), ARG), (dict(c=cache(n_kv_heads=1025)), ARG),

@@ -176,6 +176,7 @@ class Context:
         self._h = h
         self.device = device
         self._lock = threading.Lock()
+        self._attn = {}  # handles of the live AttentionHalf objects, by address
 
     @property
     def handle(self):
@@ -183,6 +184,10 @@ class Context:
 
     def close(self) -> None:
         if self._h:
+            for h in list(self._attn.values()):  # they end with their context, whichever is collected first
+                lib().ktmoe_attn_destroy(h)
+                h.value = None
+            self._attn.clear()
             lib().ktmoe_close(self._h)
             self._h = None
 
@@ -806,12 +811,14 @@ class AttentionHalf:
         h = ctypes.c_void_p()
         ctx.check(lib().ktmoe_attn_create(ctx.handle, ctypes.byref(cfg), ctypes.byref(h)))
         self._h = h
+        ctx._attn[h.value] = h
 
     def __del__(self):
         try:
-            if self._h:
+            if self._h:  # null when the context has been closed
+                del self.ctx._attn[self._h.value]
                 lib().ktmoe_attn_destroy(self._h)
-                self._h = None
+                self._h.value = None
         except Exception:
             pass
 

@@ -115,7 +115,7 @@ struct ktmoe_ctx {
     cudaEvent_t ev_fork = nullptr, ev_join = nullptr;
     cudaEvent_t ev_g0 = nullptr, ev_g1 = nullptr;  // around the last linear call's GEMM (ktmoe_linear_last_gemm)
     int last_gemm_planes = 0;                      // 0: no GEMM timed yet; 3: nine-plane kernel; 1: (1, 2) kernel
-    int* d_err = nullptr;
+    int* d_err = nullptr;  // [2]
     // pinned host words for the status a linear call reads back with its result: [0..2] the packing counters, [3]
     // the error word (one synchronisation for both, instead of a blocking copy each)
     unsigned long long* h_status = nullptr;
@@ -234,29 +234,25 @@ inline int set_device(ktmoe_ctx* ctx) {
     return KTMOE_OK;
 }
 
-// Error words a kernel leaves: below ERR_DATA a bounded wait that expired, from ERR_DATA on something wrong in a batch
-// description that only the device could see (kv_kernels.cuh).
-enum : int { ERR_DATA = 100, ERR_BAD_PAGE = 100, ERR_BAD_LENGTH = 101, ERR_BAD_POSITION = 102 };
+// What a kernel leaves in the second error word: something wrong in a batch description that only the device could see
+// (kv_kernels.cuh). The first word has the code of a bounded wait that expired, and ends the other waits of the context.
+enum : int { ERR_BAD_PAGE = 1, ERR_BAD_LENGTH = 2, ERR_BAD_POSITION = 3 };
 
 inline int fail_err_word(ktmoe_ctx* ctx, int code) {
-    switch (code) {
-        case ERR_BAD_PAGE: return fail(ctx, KTMOE_ERR_ARG, "a page table entry lies outside the cache's pages");
-        case ERR_BAD_LENGTH:
-            return fail(ctx, KTMOE_ERR_ARG, "a batch's row offsets or lengths do not fit its rows and page table");
-        case ERR_BAD_POSITION: return fail(ctx, KTMOE_ERR_ARG, "a position lies beyond the rotation table");
-        default:
-            return fail(ctx, KTMOE_ERR_KERNEL, "a kernel's bounded wait expired (code " + std::to_string(code) + ")");
-    }
+    return fail(ctx, KTMOE_ERR_KERNEL, "a kernel's bounded wait expired (code " + std::to_string(code) + ")");
 }
 
-inline int check_err_word(ktmoe_ctx* ctx) {
-    int h = 0;
-    CK(cudaMemcpy(&h, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost));
-    if (h != 0) {
-        CK(cudaMemset(ctx->d_err, 0, sizeof(int)));
-        return fail_err_word(ctx, h);
-    }
-    return KTMOE_OK;
+// The first error word; with `batches` the second one too.
+inline int check_err_word(ktmoe_ctx* ctx, bool batches = false) {
+    int h[2] = {0, 0};
+    CK(cudaMemcpy(h, ctx->d_err, batches ? sizeof(h) : sizeof(int), cudaMemcpyDeviceToHost));
+    if (h[0] == 0 && h[1] == 0) return KTMOE_OK;
+    CK(cudaMemset(ctx->d_err, 0, batches ? sizeof(h) : sizeof(int)));
+    if (h[0] != 0) return fail_err_word(ctx, h[0]);
+    return fail(ctx, KTMOE_ERR_ARG,
+                h[1] == ERR_BAD_PAGE     ? "a page table entry lies outside the cache's pages"
+                : h[1] == ERR_BAD_LENGTH ? "a batch's row offsets or lengths do not fit its rows and page table"
+                                         : "a position lies beyond the rotation table");
 }
 
 }  // namespace ktc

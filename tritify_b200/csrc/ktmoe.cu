@@ -1762,7 +1762,7 @@ int ktmoe_open(int device, ktmoe_ctx** out) {
     ktmoe_ctx* ctx = new ktmoe_ctx();
     ctx->device = device;
     if (cudaSetDevice(device) != cudaSuccess || cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking) != cudaSuccess ||
-        cudaMalloc(&ctx->d_err, sizeof(int)) != cudaSuccess || cudaMemset(ctx->d_err, 0, sizeof(int)) != cudaSuccess) {
+        cudaMalloc(&ctx->d_err, 2 * sizeof(int)) != cudaSuccess || cudaMemset(ctx->d_err, 0, 2 * sizeof(int)) != cudaSuccess) {
         delete ctx;
         return KTMOE_ERR_CUDA;
     }
@@ -1826,7 +1826,7 @@ int ktmoe_sync(ktmoe_ctx* ctx, void* stream) {
     if (int r = set_device(ctx)) return r;
     if (stream) CK(cudaStreamSynchronize((cudaStream_t)stream));
     CK(cudaStreamSynchronize(ctx->stream));
-    return check_err_word(ctx);
+    return check_err_word(ctx, true);
 }
 
 int ktmoe_set_weight_budget(ktmoe_ctx* ctx, uint64_t bytes) {
@@ -3233,8 +3233,11 @@ struct ktmoe_attn {
     ktmoe_rope rope{nullptr, 0, 0, 0};
     double softmax_scale = 0.0;
     int32_t window = 0, sinks = 0;
-    // scratch for `cap` rows
+    // scratch for `cap` rows. Once a forward has been captured into a graph, buffers that are outgrown stay (`retired`):
+    // the graph's launches hold their addresses.
     int64_t cap = 0;
+    bool captured = false;
+    std::vector<DevBuf> retired;
     DevBuf c_rows, xn, planes, xmax, sqx, acc, qkv, qkv_scale, o, o_scale, merged, out, out_scale, m, scal;
 };
 
@@ -3244,26 +3247,46 @@ namespace {
 enum AttnScale { A_NORM = 0, A_XN = 2, A_HEADS = 3, A_MERGED = 5, A_ROWS = 6, A_M = 8, A_ADD = 9, A_NSCALES = 12 };
 enum AttnWord { AU_NORM = 0, AU_HEADS, AU_ROWS, AU_ADD, AU_N };
 
-int attn_scratch(ktmoe_attn* A, int64_t T) {
+cudaError_t attn_ensure(ktmoe_attn* A, DevBuf& b, size_t bytes) {
+    if (A->captured && b.p && bytes > b.bytes) {
+        A->retired.push_back(b);
+        b = DevBuf{};
+    }
+    return b.ensure(bytes);
+}
+
+int attn_scratch(ktmoe_attn* A, int64_t T, cudaStream_t st) {
     ktmoe_ctx* ctx = A->ctx;
-    if (T <= A->cap) return KTMOE_OK;
+    cudaStreamCaptureStatus capture;
+    CK(cudaStreamIsCapturing(st, &capture));
+    const bool capturing = capture != cudaStreamCaptureStatusNone;
+    if (T <= A->cap) {
+        A->captured |= capturing;
+        return KTMOE_OK;
+    }
+    if (capturing)
+        return fail(ctx, KTMOE_ERR_STATE, "the scratch would grow while the stream is captured: run a forward of as many rows first");
+    A->cap = 0;
     const int64_t T_pad = round_up(T, 64), w = A->q + 2 * A->kv;
     const int64_t k_pad = std::max(A->w_qkv.k_pad, A->w_out.k_pad);
-    CK(A->c_rows.ensure(T * sizeof(Scale)));
-    CK(A->xn.ensure(T * A->d * 4));
-    CK(A->planes.ensure(3 * T_pad * k_pad));
-    CK(A->xmax.ensure(T * 8));
-    CK(A->sqx.ensure(T * sizeof(Scale)));
-    CK(A->acc.ensure(T * std::max(w, A->d) * 8));
-    CK(A->qkv.ensure(T * w * 4));
-    CK(A->qkv_scale.ensure(3 * T * sizeof(Scale)));
-    CK(A->o.ensure(T * A->q * 4));
-    CK(A->o_scale.ensure(T * A->cfg.n_kv_heads * sizeof(Scale)));
-    CK(A->merged.ensure(T * A->q * 4));
-    CK(A->out.ensure(T * A->d * 4));
-    CK(A->out_scale.ensure(T * sizeof(Scale)));
-    CK(A->m.ensure(T * A->d * 4));
-    CK(A->scal.ensure(A_NSCALES * sizeof(Scale) + AU_N * 8));
+    const std::pair<DevBuf*, int64_t> sizes[] = {
+        {&A->c_rows, T * (int64_t)sizeof(Scale)},
+        {&A->xn, T * A->d * 4},
+        {&A->planes, 3 * T_pad * k_pad},
+        {&A->xmax, T * 8},
+        {&A->sqx, T * (int64_t)sizeof(Scale)},
+        {&A->acc, T * std::max(w, A->d) * 8},
+        {&A->qkv, T * w * 4},
+        {&A->qkv_scale, 3 * T * (int64_t)sizeof(Scale)},
+        {&A->o, T * A->q * 4},
+        {&A->o_scale, T * A->cfg.n_kv_heads * (int64_t)sizeof(Scale)},
+        {&A->merged, T * A->q * 4},
+        {&A->out, T * A->d * 4},
+        {&A->out_scale, T * (int64_t)sizeof(Scale)},
+        {&A->m, T * A->d * 4},
+        {&A->scal, A_NSCALES * (int64_t)sizeof(Scale) + AU_N * 8},
+    };
+    for (const auto& [buf, bytes] : sizes) CK(attn_ensure(A, *buf, (size_t)bytes));
     A->cap = T;
     return KTMOE_OK;
 }
@@ -3397,6 +3420,7 @@ int ktmoe_attn_destroy(ktmoe_attn* A) {
                       &A->sqx,   &A->acc,   &A->qkv,    &A->qkv_scale, &A->o,    &A->o_scale, &A->merged, &A->out,
                       &A->out_scale, &A->m, &A->scal};
     for (DevBuf* b : bufs) b->release();
+    for (DevBuf& b : A->retired) b.release();
     delete A;
     return KTMOE_OK;
 }
@@ -3458,6 +3482,10 @@ int ktmoe_attn_set_rope(ktmoe_attn* A, double theta, int32_t rot_dim, int64_t po
     if (ktmoe_rope_table(theta, rot_dim, positions, table.data()) != KTMOE_OK)
         return fail(ctx, KTMOE_ERR_ARG, "theta must be positive and finite");
     CK(cudaStreamSynchronize(ctx->stream));
+    if (A->captured && A->b_rope.p) {  // a captured forward keeps the table that it was captured with
+        A->retired.push_back(A->b_rope);
+        A->b_rope = DevBuf{};
+    }
     CK(A->b_rope.ensure(table.size() * 4));
     CK(cudaMemcpy(A->b_rope.p, table.data(), table.size() * 4, cudaMemcpyHostToDevice));
     A->rope = ktmoe_rope{A->b_rope.as<int32_t>(), positions, rot_dim, interleaved ? 1 : 0};
@@ -3489,8 +3517,8 @@ int ktmoe_attn_forward_dev(ktmoe_attn* A, const ktmoe_kv_cache* cache, const ktm
     if (batch->rows == 0) return KTMOE_OK;
     if (!x_dev || !x_scale_dev || !y_dev || !y_scale_dev) return KTMOE_ERR_ARG;
     if (int r = set_device(ctx)) return r;
-    if (int r = attn_scratch(A, batch->rows)) return r;
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
+    if (int r = attn_scratch(A, batch->rows, st)) return r;
     return attn_forward(A, cache, batch, x_dev, (const Scale*)x_scale_dev, y_dev, (Scale*)y_scale_dev, st);
 }
 

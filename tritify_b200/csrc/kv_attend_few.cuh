@@ -91,8 +91,7 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int
             : "memory");
         if (ok) return true;
         if ((it & 255u) == 0) {
-            const int e = *(volatile int*)err;
-            if (e > 0 && e < 100) return false;
+            if (*(volatile int*)err != 0) return false;
             if (dg::globaltimer() - t0 > 2000000000ull) {
                 atomicCAS(err, 0, code);
                 return false;
@@ -154,8 +153,8 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
         const int begin = a.b.begin[b], end = a.b.begin[b + 1], len = a.b.kv_len[b];
         const long long row0 = (slot - first_slot(b)) * FEW_ROWS;
         bool live = row0 >= 0 && row0 < (long long)(end - begin) * g;
-        if (begin < 0 || begin > end || end > a.b.begin[a.b.n_seqs] || end > a.b.rows || len < 0 ||
-            ((len + (1 << a.c.page_shift) - 1) >> a.c.page_shift) > a.b.max_pages) {
+        if (begin < 0 || begin > end || end > a.b.begin[a.b.n_seqs] || end > a.b.rows ||
+            !length_fits(a.b, len, a.c.page_shift)) {
             if (lane == 0) a.err.raise(a.err.bad_length);
             live = false;
         }

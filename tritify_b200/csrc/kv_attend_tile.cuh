@@ -30,9 +30,8 @@ using dg::smem_u32;
 constexpr int TILE_KEYS = 128;
 constexpr int TILE_ROWS = 128;
 
-// A bounded wait (2 s): false when it expires, or when another wait of the context has (the error word then holds a
-// code below 100; what a kernel finds wrong in a batch does not end waits). The loop is out of line: the kernels wait in
-// some twenty places, and with it inline a fifth of their stalls were for instructions.
+// A bounded wait (2 s): false when it expires, or when another wait of the context has. The loop is out of line: the kernels wait in
+// some twenty places, and with it inline a sixth of the few-row kernel's stalls were for instructions, and it took 126 us against 120.
 static __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, int* err, int code) {
     const uint64_t t0 = dg::globaltimer();
     for (uint32_t it = 1;; ++it) {
@@ -46,8 +45,7 @@ static __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, int* 
             : "memory");
         if (ok) return true;
         if ((it & 255u) == 0) {
-            const int e = *(volatile int*)err;
-            if (e > 0 && e < 100) return false;
+            if (*(volatile int*)err != 0) return false;
             if (dg::globaltimer() - t0 > 2000000000ull) {
                 atomicCAS(err, 0, code);
                 return false;
@@ -81,9 +79,9 @@ __device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) |
 __device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return (addr >> 4) | (1024u >> 4) << 16; }
 
 // D += A B (or D = A B, accumulate = 0) of 8-bit operands given by their descriptors' low words, and the arrival of a
-// barrier when every product issued so far is done. A whole warp comes here and the one lane with `issue` set acts: with
-// the loop around them uniform the operands stay in uniform registers (issuing the four products of a tile from a branch
-// of one lane took 850 clocks, moving operands over).
+// barrier when every product issued so far is done. A whole warp comes here and the one lane with `issue` set acts, so
+// that the loop around them stays uniform. A product of K = 32 takes some 67 clocks whatever N up to 128 is, an arrival
+// about 130 of the issuing warp's: a tile's four products and two arrivals, 530.
 __device__ __forceinline__ void umma(bool issue, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
@@ -299,8 +297,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
         const int begin = a.b.begin[b], end = a.b.begin[b + 1], len = a.b.kv_len[b];
         const long long row0 = (slot - first_slot(b)) * TILE_ROWS;
         bool live = row0 >= 0 && row0 < (long long)(end - begin) * g;
-        if (begin < 0 || begin > end || end > a.b.begin[a.b.n_seqs] || end > a.b.rows || len < 0 ||
-            ((len + (1 << a.c.page_shift) - 1) >> a.c.page_shift) > a.b.max_pages) {
+        if (begin < 0 || begin > end || end > a.b.begin[a.b.n_seqs] || end > a.b.rows ||
+            !length_fits(a.b, len, a.c.page_shift)) {
             if (lane == 0) a.err.raise(a.err.bad_length);
             live = false;
         }
@@ -611,18 +609,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
             ok = __all_sync(0xffffffffu, ok);
             asm volatile("tcgen05.fence::after_thread_sync;");
         };
-        // 32 of this thread's 64 scores; after the second half the buffer goes back to the products
-        int32_t s32[32];
-        auto load_scores = [&](int c) {
-            dg::tmem_ld32(s_addr + c * 32, s32);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            if (c == 1) {
-                asm volatile("tcgen05.fence::before_thread_sync;");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s_free[grp]);
-            }
-        };
         auto key_scales = [&]() { return (const float*)(sm + C::KEY_SCALES) + (sc % C::SCALES) * C::KEY_STAGE + part * 64; };
+        // the buffer of scores goes back to the products
+        auto scores_read = [&]() {
+            asm volatile("tcgen05.fence::before_thread_sync;");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[grp]);
+        };
         auto scales_read = [&]() {
             __syncwarp();
             if (lane == 0) mbar_arrive(&k_free[sc % C::SCALES]);
@@ -740,47 +733,51 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                 uint8_t* hi = sm + C::P + grp * 2 * C::SLOT + r * 128;
                 uint8_t* lo = hi + C::SLOT;
                 uint32_t sum = 0;
+                const float* f = key_scales();
+                auto digits = [&](auto mask_tag, const int32_t (&s)[16], int k0, uint32_t seen) {  // of keys k0 .. k0 + 15
+                    constexpr bool MASK = decltype(mask_tag)::value;
+                    uint32_t h4[4], l4[4];
+#pragma unroll
+                    for (int k4 = 0; k4 < 4; ++k4) {
+                        const int k = 4 * k4;
+                        const ulonglong2 kf = *(const ulonglong2*)(f + k0 + k);
+                        const ulonglong2 vf = *(const ulonglong2*)(f + TILE_KEYS + k0 + k);
+                        const uint32_t m = MASK ? seen >> k : 0u;
+                        const f2 w0 = weight2<MASK>(scaled2(s[k], s[k + 1], kf.x), rw, m);
+                        const f2 w1 = weight2<MASK>(scaled2(s[k + 2], s[k + 3], kf.y), rw, m >> 2);
+                        const f2 mg = pk(MAGIC, MAGIC), mg128 = pk(MAGIC + 128.0f, MAGIC + 128.0f);
+                        float a0, a1, a2, a3;
+                        upk(fma2(w0, rw.two_e, mg), a0, a1);
+                        upk(fma2(w1, rw.two_e, mg), a2, a3);
+                        sum += __float_as_uint(a0) + __float_as_uint(a1);
+                        sum += __float_as_uint(a2) + __float_as_uint(a3);
+                        upk(fma2(w0, vf.x, mg128), a0, a1);
+                        upk(fma2(w1, vf.y, mg128), a2, a3);
+                        // w + 128 in the low 16 bits: the upper byte is hi, the lower one lo + 128
+                        const uint32_t u = __byte_perm(__float_as_uint(a0), __float_as_uint(a1), 0x5140);
+                        const uint32_t v = __byte_perm(__float_as_uint(a2), __float_as_uint(a3), 0x5140);
+                        l4[k4] = __byte_perm(u, v, 0x5410) ^ 0x80808080u;
+                        h4[k4] = __byte_perm(u, v, 0x7632);
+                    }
+                    const int chunk = ((part * 4 + (k0 >> 4)) ^ (r & 7)) * 16;
+                    *(uint4*)(hi + chunk) = make_uint4(h4[0], h4[1], h4[2], h4[3]);
+                    *(uint4*)(lo + chunk) = make_uint4(l4[0], l4[1], l4[2], l4[3]);
+                };
+                // 16 of this thread's 64 scores at a time: the next ones asked for under the arithmetic cost as much in
+                // registers as they gained (380 us against 378 for a prompt of 4096)
+                auto walk = [&](auto mask_tag) {
+                    constexpr bool MASK = decltype(mask_tag)::value;
 #pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    const float* f = key_scales() + c * 32;
-                    load_scores(c);
-                    auto digits = [&](auto mask_tag, uint32_t seen) {
-                        constexpr bool MASK = decltype(mask_tag)::value;
-#pragma unroll
-                        for (int k16 = 0; k16 < 32; k16 += 16) {
-                            uint32_t h4[4], l4[4];
-#pragma unroll
-                            for (int k4 = 0; k4 < 4; ++k4) {
-                                const int k = k16 + 4 * k4;
-                                const ulonglong2 kf = *(const ulonglong2*)(f + k);
-                                const ulonglong2 vf = *(const ulonglong2*)(f + TILE_KEYS + k);
-                                const uint32_t m = MASK ? seen >> k : 0u;
-                                const f2 w0 = weight2<MASK>(scaled2(s32[k], s32[k + 1], kf.x), rw, m);
-                                const f2 w1 = weight2<MASK>(scaled2(s32[k + 2], s32[k + 3], kf.y), rw, m >> 2);
-                                const f2 mg = pk(MAGIC, MAGIC), mg128 = pk(MAGIC + 128.0f, MAGIC + 128.0f);
-                                float a0, a1, a2, a3;
-                                upk(fma2(w0, rw.two_e, mg), a0, a1);
-                                upk(fma2(w1, rw.two_e, mg), a2, a3);
-                                sum += __float_as_uint(a0) + __float_as_uint(a1);
-                                sum += __float_as_uint(a2) + __float_as_uint(a3);
-                                upk(fma2(w0, vf.x, mg128), a0, a1);
-                                upk(fma2(w1, vf.y, mg128), a2, a3);
-                                // w + 128 in the low 16 bits: the upper byte is hi, the lower one lo + 128
-                                const uint32_t u = __byte_perm(__float_as_uint(a0), __float_as_uint(a1), 0x5140);
-                                const uint32_t v = __byte_perm(__float_as_uint(a2), __float_as_uint(a3), 0x5140);
-                                l4[k4] = __byte_perm(u, v, 0x5410) ^ 0x80808080u;
-                                h4[k4] = __byte_perm(u, v, 0x7632);
-                            }
-                            const int chunk = ((part * 4 + c * 2 + (k16 >> 4)) ^ (r & 7)) * 16;
-                            *(uint4*)(hi + chunk) = make_uint4(h4[0], h4[1], h4[2], h4[3]);
-                            *(uint4*)(lo + chunk) = make_uint4(l4[0], l4[1], l4[2], l4[3]);
-                        }
-                    };
-                    if (all)
-                        digits(Bool<false>{}, 0);
-                    else
-                        digits(Bool<true>{}, seen_bits(j0 + part * 64 + c * 32, pos, a.window, a.sinks));
-                }
+                    for (int k0 = 0; k0 < 64; k0 += 16) {
+                        int32_t s[16];
+                        dg::tmem_ld16(s_addr + k0, s);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        if (k0 == 48) scores_read();
+                        digits(mask_tag, s, k0, MASK ? seen_bits(j0 + part * 64 + k0, pos, a.window, a.sinks) : 0u);
+                    }
+                };
+                if (all) walk(Bool<false>{});
+                else walk(Bool<true>{});
                 if (pass == 1) total += sum - 64u * MAGIC_BITS;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();

@@ -256,6 +256,7 @@ int kv_attention(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_bat
         return fail(ctx, KTMOE_ERR_ARG, "softmax_scale must be positive and finite, window and sinks not negative");
     const int64_t width = (int64_t)n_heads * a.c.dim;
     if (ld_q < width || ld_o < width) return fail(ctx, KTMOE_ERR_ARG, "a row stride is below n_heads * head_dim");
+    if (batch->rows * (n_heads / a.c.heads) > INT32_MAX) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "too many query rows for one launch");
     if (batch->n_seqs == 0 || batch->rows == 0) return KTMOE_OK;
     if (!q || !o || !o_scale || !scale || !aligned(q, 4) || !aligned(o, 4) || !aligned(o_scale, 16))
         return fail(ctx, KTMOE_ERR_ARG, "queries, scales or outputs are null or not aligned");

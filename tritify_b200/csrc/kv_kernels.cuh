@@ -43,12 +43,18 @@ struct Rope {
     int interleaved;  // pairs (2i, 2i + 1) instead of (i, i + half)
 };
 
-// The error word and what to raise in it (the codes of context.cuh).
+// The context's error words: `word` ends its waits, the one behind it takes what is wrong in a batch (the codes of
+// context.cuh).
 struct Error {
     int* word;
     int bad_page, bad_length, bad_position;
-    __device__ __forceinline__ void raise(int code) const { atomicCAS(word, 0, code); }
+    __device__ __forceinline__ void raise(int code) const { atomicCAS(word + 1, 0, code); }
 };
+
+// Whether a sequence's length fits its row of the page table (which holds 2^24 tokens at most).
+__device__ __forceinline__ bool length_fits(const Batch& b, int len, int page_shift) {
+    return len >= 0 && len <= b.max_pages << page_shift;
+}
 
 // The sequence that row t belongs to, found by a whole warp: begin[] is sampled 32 ways a step, so 64 sequences take
 // two rounds of independent loads instead of six dependent ones. -1: t lies before the first or behind the last.
@@ -78,7 +84,7 @@ __device__ __forceinline__ bool locate(const Batch& b, const Error& err, int t, 
     if (p.seq < 0) return false;
     const int begin = b.begin[p.seq], end = b.begin[p.seq + 1], len = b.kv_len[p.seq];
     // the offsets around t have to ascend and stay within the rows, the length has to fit the page table
-    if (t < begin || t >= end || end > b.begin[b.n_seqs] || end > b.rows || len < 0 || ((len + (1 << page_shift) - 1) >> page_shift) > b.max_pages) {
+    if (t < begin || t >= end || end > b.begin[b.n_seqs] || end > b.rows || !length_fits(b, len, page_shift)) {
         err.raise(err.bad_length);
         return false;
     }
