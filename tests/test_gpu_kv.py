@@ -82,16 +82,37 @@ class Setup:
         return np.stack([mant, self.rng.integers(lo, hi, self.rows) + 31], -1).astype(np.int64)
 
     def attend(self, q, scale, table=None, interleaved=False, window=0, sinks=0, softmax_scale=None, stream=None):
-        """(codes, scales) from the GPU and from the restatement, both on outputs that held 77 before."""
+        """(codes, scales) from the GPU and from the restatement, both on outputs that held 77 before. Enough rows a
+        sequence go to the tile kernel once the blocks fill the GPU: those run a second time with as many copies of
+        all heads (its launches are two, the few-row kernel's one)."""
         torch = _torch()
         rope = None if table is None else tb.Rope(torch.from_numpy(table).cuda(), interleaved)
-        out = torch.full((self.rows, self.heads * self.dim), 77, dtype=torch.int32, device="cuda")
-        os_ = torch.full((self.rows, self.hk, 2), 77, dtype=torch.int64, device="cuda")
+        sd = torch.from_numpy(scale).cuda()
         qd = torch.from_numpy(q).cuda() if isinstance(q, np.ndarray) else q
-        self.cache.attention(self.batch, qd, torch.from_numpy(scale).cuda(), out, os_, self.heads, rope=rope,
-                             softmax_scale=softmax_scale, window=window, sinks=sinks, stream=stream)
-        self.ctx.sync()
-        torch.cuda.synchronize()
+
+        def run(cache, qd, copies):
+            out = torch.full((self.rows, copies * self.heads * self.dim), 77, dtype=torch.int32, device="cuda")
+            os_ = torch.full((self.rows, copies * self.hk, 2), 77, dtype=torch.int64, device="cuda")
+            before = self.ctx.launch_count()
+            cache.attention(self.batch, qd, sd, out, os_, copies * self.heads, rope=rope, softmax_scale=softmax_scale,
+                            window=window, sinks=sinks, stream=stream)
+            launches = self.ctx.launch_count() - before
+            self.ctx.sync()
+            torch.cuda.synchronize()
+            return out.reshape(self.rows, copies, -1), os_.reshape(self.rows, copies, -1), launches
+
+        out, os_, _ = run(self.cache, qd, 1)
+        if (self.begin[-1] - self.begin[0]) * (self.heads // self.hk) > 32 * len(self.lens):
+            copies = -(-148 // self.hk)
+            cache = tb.KvCache(self.ctx, self.cache.n_pages, self.page, copies * self.hk, self.dim, pools=[
+                t.repeat(1, copies, *[1] * (t.dim() - 2)) for t in (self.cache.k, self.cache.v, self.cache.k_scale, self.cache.v_scale)])
+            skew = 0 if qd.is_contiguous() else 1  # unaligned rows stay unaligned
+            wide = torch.zeros(self.rows, copies * qd.shape[1] + skew, dtype=torch.int32, device="cuda")[:, skew:]
+            wide.copy_(qd.repeat(1, copies))
+            torch.cuda.synchronize()
+            o, s, launches = run(cache, wide, copies)
+            assert launches == 2
+            assert (o == out).all() and (s == os_).all(), "the two kernels differ"
         want = np.full((self.rows, self.heads, self.dim), 77, np.int64)
         want_s = np.full((self.rows, self.hk, 2), 77, np.int64)
         R.attention(q.reshape(self.rows, self.heads, self.dim) if isinstance(q, np.ndarray) else
@@ -99,7 +120,7 @@ class Setup:
                     want, want_s, self.dim ** -0.5 if softmax_scale is None else softmax_scale, window, sinks, table,
                     interleaved)
         want_s[..., 1] &= 0xFFFFFFFF
-        return out.cpu().numpy().reshape(want.shape), os_.cpu().numpy(), want, want_s
+        return out.cpu().numpy().reshape(want.shape), os_.cpu().numpy().reshape(want_s.shape), want, want_s
 
     def check(self, *a, **k):
         got, got_s, want, want_s = self.attend(*a, **k)
@@ -299,28 +320,32 @@ def test_attention_of_millions_of_keys(ctx):
     s.check(s.codes(16), s.scales())
 
 
-def test_attention_takes_strided_and_unaligned_queries(ctx):
+@pytest.mark.parametrize("hk", [2, 150])
+def test_attention_takes_strided_and_unaligned_queries(ctx, hk):
     torch = _torch()
-    s = Setup(ctx, [(5, 90), (30, 200)], 4, 2, 48, 16)
-    wide = torch.from_numpy(s.rng.integers(-2 ** 28, 2 ** 28, (s.rows, 4 * 48 + 3)).astype(np.int32)).cuda()
-    s.check(wide[:, 1:-2], s.scales())
+    s = Setup(ctx, [(5, 90), (30, 200)], 2 * hk, hk, 48, 16)
+    n = 2 * hk * 48
+    wide = torch.from_numpy(s.rng.integers(-2 ** 28, 2 ** 28, (s.rows, n + 3)).astype(np.int32)).cuda()
+    if hk == 2:
+        s.check(wide[:, 1:-2], s.scales())
     scale = torch.from_numpy(s.scales()).cuda()
     outs = []
     for pad in (0, 7):  # the output's rows may be strided too
-        o = torch.zeros(s.rows, 4 * 48 + pad, dtype=torch.int32, device="cuda")
-        os_ = torch.zeros(s.rows, 2, 2, dtype=torch.int64, device="cuda")
-        s.cache.attention(s.batch, wide[:, 1:-2], scale, o[:, pad // 2:pad // 2 + 4 * 48], os_, 4)
-        outs.append((o[:, pad // 2:pad // 2 + 4 * 48].cpu(), os_.cpu()))
-        assert (o[:, :pad // 2] == 0).all() and (o[:, pad // 2 + 4 * 48:] == 0).all()
+        o = torch.zeros(s.rows, n + pad, dtype=torch.int32, device="cuda")
+        os_ = torch.zeros(s.rows, hk, 2, dtype=torch.int64, device="cuda")
+        s.cache.attention(s.batch, wide[:, 1:-2], scale, o[:, pad // 2:pad // 2 + n], os_, 2 * hk)
+        outs.append((o[:, pad // 2:pad // 2 + n].cpu(), os_.cpu()))
+        assert (o[:, :pad // 2] == 0).all() and (o[:, pad // 2 + n:] == 0).all()
     ctx.sync()
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
 
 
 @pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
-def test_chunks_equal_the_whole_prompt(ctx, window, sinks):
+@pytest.mark.parametrize("hk", [2, 60])  # 60: the long chunks go to the tile kernel
+def test_chunks_equal_the_whole_prompt(ctx, hk, window, sinks):
     """A prompt written and attended in chunks of any size, down to single tokens, gives the bits of one call."""
     torch = _torch()
-    n, heads, hk, dim, page = 200, 6, 2, 64, 16
+    n, heads, dim, page = 200, 3 * hk, 64, 16
     rng = np.random.default_rng(8)
     kv = torch.from_numpy(rng.integers(-2 ** 28, 2 ** 28, (n, 2 * hk * dim)).astype(np.int32)).cuda()
     q = torch.from_numpy(rng.integers(-2 ** 28, 2 ** 28, (n, heads * dim)).astype(np.int32)).cuda()
@@ -435,12 +460,13 @@ def test_two_streams_and_a_replayed_graph(ctx):
 
 
 @pytest.mark.parametrize("what", ["page", "negative_page", "long", "longest", "negative", "descending", "rows", "position"])
-@pytest.mark.parametrize("new", [1, 40])
-def test_wrong_batches_are_reported_and_harmless(ctx, what, new):
+@pytest.mark.parametrize("new,hk", [(1, 2), (40, 2), (40, 150)])
+def test_wrong_batches_are_reported_and_harmless(ctx, what, new, hk):
     """What only the device can see: the calls touch nothing outside their buffers, sync reports it, and the context
     serves on."""
     torch = _torch()
-    s = Setup(ctx, [(new, 100), (new, 90)], 4, 2, 64, 16, rows_behind=1)
+    s = Setup(ctx, [(new, 100), (new, 90)], 2 * hk, hk, 64, 16, rows_behind=1)
+    n = hk * 64
     rope = None
     if what == "page":
         s.batch.page_table[1, 2] = s.cache.n_pages
@@ -458,12 +484,12 @@ def test_wrong_batches_are_reported_and_harmless(ctx, what, new):
         s.batch.q_begin[2] = 2 * new + 5
     elif what == "position":
         rope = tb.Rope(torch.from_numpy(tb.rope_table(1e4, 64, 80)).cuda())
-    q = torch.from_numpy(s.codes(256)).cuda()
-    kv = torch.from_numpy(s.codes(256)).cuda()
+    q = torch.from_numpy(s.codes(2 * n)).cuda()
+    kv = torch.from_numpy(s.codes(2 * n)).cuda()
     scale = torch.from_numpy(s.scales()).cuda()
-    guard = torch.full((s.rows + 2, 256), 77, dtype=torch.int32, device="cuda")
-    os_ = torch.zeros(s.rows, 2, 2, dtype=torch.int64, device="cuda")
-    ko = torch.full((s.rows + 2, 128), 7.0, device="cuda")
+    guard = torch.full((s.rows + 2, 2 * n), 77, dtype=torch.int32, device="cuda")
+    os_ = torch.zeros(s.rows, hk, 2, dtype=torch.int64, device="cuda")
+    ko = torch.full((s.rows + 2, n), 7.0, device="cuda")
 
     def reported(call):
         call()
@@ -473,11 +499,11 @@ def test_wrong_batches_are_reported_and_harmless(ctx, what, new):
         assert e.value.status == _native.ERR_ARG
         ctx.sync()  # reported once
 
-    reported(lambda: s.cache.attention(s.batch, q, scale, guard[1:-1], os_, 4, rope=rope))
+    reported(lambda: s.cache.attention(s.batch, q, scale, guard[1:-1], os_, 2 * hk, rope=rope))
     if what in ("page", "negative_page"):
         # a page that no new row lies in is no business of the write
         s.batch.page_table[:] = s.cache.n_pages if what == "page" else -7
-    reported(lambda: s.cache.append(s.batch, kv[:, :128], kv[:, 128:], scale, rope))
+    reported(lambda: s.cache.append(s.batch, kv[:, :n], kv[:, n:], scale, rope))
     if what != "position":
         reported(lambda: s.cache.read(s.batch, ko[1:-1], ko[1:-1].clone()))
     assert (guard[0] == 77).all() and (guard[-1] == 77).all()

@@ -2,6 +2,7 @@
 // over the cache. All on device buffers, ordered on the caller's stream, nothing allocated and no workspace kept, so
 // calls on several streams and captured graphs share nothing but the caller's own buffers.
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -122,14 +123,41 @@ int launch_tile(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
     return KTMOE_OK;
 }
 
-// Blocks of a cluster: twice as many while they do not fill the GPU and each would keep two tiles or more (as far as the
-// page table tells: the lengths are on the device). Clusters of 16 leave SMs of a GPC idle: four sequences of 65536 keys
-// by 8 KV heads took 211 us in sixteens, 155 in eights, 240 in fours; a batch that fills the GPU by itself, 64 sequences of
-// 4096, 127 us in ones, 121 in twos, 162 in fours.
-int few_cluster(const ktmoe_ctx* ctx, int64_t tiles, int64_t jobs, int per_sm) {
+// Clusters of the few-row kernel: the sixteens of all rows, and one more a sequence, by the KV heads.
+int64_t few_jobs(const kv::AttendArgs& a) { return (a.b.rows * a.group / kv::FEW_ROWS + a.b.n_seqs) * a.c.heads; }
+
+// Tiles of keys that a row may see, as far as the host knows: the lengths are on the device.
+int64_t key_tiles(const kv::AttendArgs& a) {
+    const int64_t tiles = (((int64_t)a.b.max_pages << a.c.page_shift) + kv::TILE_KEYS - 1) / kv::TILE_KEYS;
+    return a.window ? std::min(tiles, ((int64_t)a.window + a.sinks) / kv::TILE_KEYS + 2) : tiles;
+}
+
+// Blocks of a cluster: twice as many while they do not fill the GPU and each would keep two tiles or more. Clusters of 16
+// leave SMs of a GPC idle: four sequences of 65536 keys by 8 KV heads took 211 us in sixteens, 155 in eights, 240 in
+// fours; a batch that fills the GPU by itself, 64 sequences of 4096, 127 us in ones, 121 in twos, 162 in fours.
+int few_cluster(const ktmoe_ctx* ctx, const kv::AttendArgs& a, int per_sm) {
+    const int64_t jobs = few_jobs(a), tiles = key_tiles(a);
     int c = 1;
     while (c < 8 && tiles >= 2 * c && jobs * c < (int64_t)per_sm * ctx->num_sms) c *= 2;
     return c;
+}
+
+// Which kernel. Where the GPU is full, a block of 128 rows is the better one (three times for many rows), but it walks
+// all keys alone, while sixteens of rows spread over more SMs and split the keys in clusters. Both times are rounds of
+// blocks by tiles of keys and a start; an SM passes a tile by 16 rows in 3/7 of the time it takes by 128, and starts
+// count as 8 and 6 tiles. Measured (us) at a head_dim of 128, 8 KV heads and 8192 keys: 1 sequence of 64 rows 39 against
+// 159, of 256 90 against 162, of 512 150 against 163, of 1024 264 against 163; 16 sequences of 32 rows 152 against 167, of
+// 64 277 against 169; at 512 keys 1 sequence of 256 rows 43 against 32. Over 304 such sizes, head_dim 256 among them, the
+// rule loses 0.05 % to the better choice of each.
+bool few_rows(const ktmoe_ctx* ctx, const kv::AttendArgs& a, int per_sm) {
+    const int64_t rows = (a.b.rows * a.group + a.b.n_seqs - 1) / a.b.n_seqs;  // of a sequence, if all had as many
+    auto rounds = [&](int64_t block, int64_t split, int64_t at_once) {
+        const int64_t blocks = a.b.n_seqs * ((rows + block - 1) / block) * a.c.heads * split;
+        return (blocks + at_once - 1) / at_once;
+    };
+    const int64_t c = few_cluster(ctx, a, per_sm), tiles = key_tiles(a);
+    return 3 * per_sm * rounds(kv::FEW_ROWS, c, (int64_t)per_sm * ctx->num_sms) * (8 * c + tiles) <=
+           7 * c * rounds(kv::TILE_ROWS, 1, ctx->num_sms) * (6 + tiles);
 }
 
 template <int NK, int PER_SM>
@@ -141,8 +169,8 @@ int launch_few(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
         CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
         attr_set[ctx->device & 63] = true;
     }
-    const int64_t jobs = (a.b.rows * a.group / kv::FEW_ROWS + a.b.n_seqs) * a.c.heads;
-    const int c = few_cluster(ctx, ((int64_t)a.b.max_pages << a.c.page_shift) / kv::TILE_KEYS, jobs, PER_SM);
+    const int64_t jobs = few_jobs(a);
+    const int c = few_cluster(ctx, a, PER_SM);
     if (jobs * c > INT32_MAX) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "too many query rows for one launch");
     CUtensorMap mk, mv;
     if (int r = make_pool_map(ctx, &mk, a.c.k, a.c)) return r;
@@ -276,8 +304,6 @@ int kv_attention(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_bat
     a.o_scale = (longlong2*)o_scale;
     a.vec_o = aligned(o, 16) && ld_o % 4 == 0;
     cudaStream_t st = stream ? (cudaStream_t)stream : ctx->stream;
-    // few rows a sequence: bound by the keys' and values' bytes; many: by the arithmetic on the scores
-    if ((int64_t)a.group * batch->rows > (int64_t)2 * kv::FEW_ROWS * batch->n_seqs)
-        return a.c.dim <= 128 ? launch_tile<1>(ctx, st, a) : launch_tile<2>(ctx, st, a);
-    return a.c.dim <= 128 ? launch_few<1, 2>(ctx, st, a) : launch_few<2, 1>(ctx, st, a);
+    if (a.c.dim <= 128) return few_rows(ctx, a, 2) ? launch_few<1, 2>(ctx, st, a) : launch_tile<1>(ctx, st, a);
+    return few_rows(ctx, a, 1) ? launch_few<2, 1>(ctx, st, a) : launch_tile<2>(ctx, st, a);
 }
