@@ -123,22 +123,30 @@ int launch_tile(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
     return KTMOE_OK;
 }
 
-// Clusters of the few-row kernel: the sixteens of all rows, and one more a sequence, by the KV heads.
-int64_t few_jobs(const kv::AttendArgs& a) { return (a.b.rows * a.group / kv::FEW_ROWS + a.b.n_seqs) * a.c.heads; }
-
 // Tiles of keys that a row may see, as far as the host knows: the lengths are on the device.
 int64_t key_tiles(const kv::AttendArgs& a) {
     const int64_t tiles = (((int64_t)a.b.max_pages << a.c.page_shift) + kv::TILE_KEYS - 1) / kv::TILE_KEYS;
     return a.window ? std::min(tiles, ((int64_t)a.window + a.sinks) / kv::TILE_KEYS + 2) : tiles;
 }
 
-// Blocks of a cluster: twice as many while they do not fill the GPU and each would keep two tiles or more. Clusters of 16
-// leave SMs of a GPC idle: four sequences of 65536 keys by 8 KV heads took 211 us in sixteens, 155 in eights, 240 in
-// fours; a batch that fills the GPU by itself, 64 sequences of 4096, 127 us in ones, 121 in twos, 162 in fours.
+// Blocks of `block` rows, if all sequences had as many rows.
+int64_t even_blocks(const kv::AttendArgs& a, int64_t block) {
+    const int64_t rows = (a.b.rows * a.group + a.b.n_seqs - 1) / a.b.n_seqs;
+    return a.b.n_seqs * ((rows + block - 1) / block) * a.c.heads;
+}
+
+// Blocks of a cluster: twice as many while they are less than 4/3 of what the GPU holds at once. Eights are harder to
+// place (a GPC's SMs do not divide by them; with one block an SM, 16 clusters of eight already take two rounds): only
+// where they fill half of the GPU at most, or where the keys are long. Measured (us), clusters of 1, 2, 4, 8 at 4 query
+// heads to one of 8 KV heads of 128: 1 sequence of 1000 keys 21, 18, 16, 16, of 8000 86, 49, 29, 23; 4 of 2000 30, 23,
+// 20, 23; 8 of 16384 176, 105, 82, 86; 16 of 4096 59, 49, 55, 94; 64 of 1024 53, 74, 121, 121, of 4096 145, 145, 180, 285.
+// Over 444 such sizes the rule loses 2 % to the best choice of each.
 int few_cluster(const ktmoe_ctx* ctx, const kv::AttendArgs& a, int per_sm) {
-    const int64_t jobs = few_jobs(a), tiles = key_tiles(a);
+    const int64_t jobs = even_blocks(a, kv::FEW_ROWS), tiles = key_tiles(a), at_once = (int64_t)per_sm * ctx->num_sms;
     int c = 1;
-    while (c < 8 && tiles >= 2 * c && jobs * c < (int64_t)per_sm * ctx->num_sms) c *= 2;
+    while (c < 4 && tiles > c && 3 * jobs * c < 2 * at_once) c *= 2;
+    const bool few_eights = 2 * 8 * jobs <= at_once;
+    if (c == 4 && tiles > 4 && (few_eights || (per_sm == 2 && tiles >= 64 && 3 * jobs * 4 < 2 * at_once))) c = 8;
     return c;
 }
 
@@ -148,16 +156,12 @@ int few_cluster(const ktmoe_ctx* ctx, const kv::AttendArgs& a, int per_sm) {
 // count as 8 and 6 tiles. Measured (us) at a head_dim of 128, 8 KV heads and 8192 keys: 1 sequence of 64 rows 39 against
 // 159, of 256 90 against 162, of 512 150 against 163, of 1024 264 against 163; 16 sequences of 32 rows 152 against 167, of
 // 64 277 against 169; at 512 keys 1 sequence of 256 rows 43 against 32. Over 304 such sizes, head_dim 256 among them, the
-// rule loses 0.05 % to the better choice of each.
+// rule loses less than 0.1 % to the better choice of each.
 bool few_rows(const ktmoe_ctx* ctx, const kv::AttendArgs& a, int per_sm) {
-    const int64_t rows = (a.b.rows * a.group + a.b.n_seqs - 1) / a.b.n_seqs;  // of a sequence, if all had as many
-    auto rounds = [&](int64_t block, int64_t split, int64_t at_once) {
-        const int64_t blocks = a.b.n_seqs * ((rows + block - 1) / block) * a.c.heads * split;
-        return (blocks + at_once - 1) / at_once;
-    };
+    auto rounds = [](int64_t blocks, int64_t at_once) { return (blocks + at_once - 1) / at_once; };
     const int64_t c = few_cluster(ctx, a, per_sm), tiles = key_tiles(a);
-    return 3 * per_sm * rounds(kv::FEW_ROWS, c, (int64_t)per_sm * ctx->num_sms) * (8 * c + tiles) <=
-           7 * c * rounds(kv::TILE_ROWS, 1, ctx->num_sms) * (6 + tiles);
+    return 3 * per_sm * rounds(even_blocks(a, kv::FEW_ROWS) * c, (int64_t)per_sm * ctx->num_sms) * (8 * c + tiles) <=
+           7 * c * rounds(even_blocks(a, kv::TILE_ROWS), ctx->num_sms) * (6 + tiles);
 }
 
 template <int NK, int PER_SM>
@@ -169,7 +173,8 @@ int launch_few(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
         CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
         attr_set[ctx->device & 63] = true;
     }
-    const int64_t jobs = few_jobs(a);
+    // the sixteens of all rows, and one more a sequence, by the KV heads
+    const int64_t jobs = (a.b.rows * a.group / kv::FEW_ROWS + a.b.n_seqs) * a.c.heads;
     const int c = few_cluster(ctx, a, PER_SM);
     if (jobs * c > INT32_MAX) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "too many query rows for one launch");
     CUtensorMap mk, mv;
