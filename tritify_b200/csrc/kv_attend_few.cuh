@@ -233,7 +233,11 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
             const int at = tile_at(min(i, n - 1)) * per_tile + lane;
             return lane < per_tile && at <= last_page ? __ldg(pages + at) : 0;
         };
-        auto load = [&](const CUtensorMap* map, int i, int page) {
+        // Of K that is read again as much as fits should be in L2 by then: what is read for the last time, and by no other
+        // block (one group of rows a head), leaves it first.
+        const bool alone = n_new * g <= FEW_ROWS;
+        const uint64_t policy = once_policy();
+        auto load = [&](const CUtensorMap* map, int i, int page, bool last) {
             const int np = min(per_tile, last_page - tile_at(i) * per_tile + 1);
             if ((unsigned)page >= (unsigned long long)a.c.n_pages) {
                 a.err.raise(a.err.bad_page);
@@ -248,8 +252,11 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
                 }
                 alive = __shfl_sync(0xffffffffu, (int)ok, 0);
                 if (!alive) return;
-                if (lane < np)
-                    tma_load_4d(smem_u32(sm + C::RING + s * C::SLOT + lane * ps * 128), map, x * 128, 0, head, page, &full[s]);
+                if (lane < np) {
+                    const uint32_t dst = smem_u32(sm + C::RING + s * C::SLOT + lane * ps * 128);
+                    if (last && alone) tma_load_4d_once(dst, map, x * 128, 0, head, page, &full[s], policy);
+                    else tma_load_4d(dst, map, x * 128, 0, head, page, &full[s]);
+                }
                 ++q;
                 if (++s == C::SLOTS) s = 0, phase ^= 1;
             }
@@ -259,10 +266,10 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
             for (int i = 0; alive && i < n; ++i) {
                 const int pc = page_of(i + 2);
                 if (ph == 0) {
-                    load(&map_k, i, pa);
+                    load(&map_k, i, pa, i < C::KEEP);
                 } else {
-                    if (i + 1 >= C::KEEP && i + 1 < n) load(&map_k, i + 1, pb);
-                    if (alive) load(&map_v, i, pa);
+                    if (i + 1 >= C::KEEP && i + 1 < n) load(&map_k, i + 1, pb, true);
+                    if (alive) load(&map_v, i, pa, true);
                 }
                 pa = pb;
                 pb = pc;
