@@ -7,13 +7,14 @@
 // digits of the weights in one product of 32 columns). A thread has one key of a tile.
 //
 // The row maxima must be known before the first weight is rounded, so there are two phases; K is read once all the same,
-// because the scores wait in TMEM, 16 columns a tile. Only tiles beyond what a block has room for are formed again. While
-// the cluster exchanges its maxima, V is already on its way. Sums over the keys are integers, so the shares of a cluster
+// because the scores wait in TMEM, 4, 8 or 16 columns a tile for as many rows (with 16 for any number the decode of 64
+// sequences of 4096 by 4 rows took 111 us, not 96). Only tiles beyond what a block has room for are formed again. While the
+// cluster exchanges its maxima, V is already on its way. Sums over the keys are integers, so the shares of a cluster
 // add up to the same bits in any order: each block adds its own into the shared memory of the block that writes them out.
 //
 // A block's start, exchange and end are latency (10 us of a block's 26 at 12 tiles), so two blocks share an SM, one's waits
-// under the other's stream, although each then has room for the scores of 12 tiles only (28 alone): four sequences of
-// 65536 keys take 155 us, against 264 with one block an SM and every score kept.
+// under the other's stream, although each then has room for the scores of 12 to 48 tiles only (26 to 104 alone): four
+// sequences of 65536 keys by 12 rows took 155 us, against 264 with one block an SM.
 //
 // Roles: softmax warps, in one or two groups of four that take the tiles in turn; then one warp each for TMA, the
 // products and the keys' scales.
@@ -35,8 +36,8 @@ struct FewCfg {
     static constexpr int COLS = 512 / PER_SM;  // of TMEM
     static constexpr int SCALES = 4;
     static constexpr int SUMS = COLS - 32 * NK;        // O^T of each 128 columns: 16 hi, 16 lo
-    static constexpr int KEEP = (SUMS - 32) / 16;      // tiles whose scores stay in TMEM: 12 (NK 1, PER_SM 2), 26 (NK 2, PER_SM 1)
-    static constexpr int AGAIN = 16 * KEEP;            // two more score buffers, for the others
+    static constexpr int KEEP = SUMS - 32;             // columns for scores that stay: 192 (NK 1, PER_SM 2), 416 (NK 2, PER_SM 1)
+    static constexpr int FRESH = KEEP;                 // two score buffers of 16 columns, written by the products
     static constexpr int RING = 0;
     static constexpr int Q = RING + SLOTS * SLOT;               // [NK][16 rows][128]
     static constexpr int P = Q + NK * 16 * 128;                 // [2][16 hi, 16 lo][128 keys]
@@ -47,7 +48,6 @@ struct FewCfg {
     // the row's (max, -theta, 2^-E, 2^E); 2^21 / L
     static constexpr int BARS = ROWS + FEW_ROWS * (4 + 4 + 64 + 64 + 8 + 16 + 8);
     static constexpr int BYTES = 1024 + BARS + 512;
-    static_assert(AGAIN + 32 <= SUMS, "TMEM columns");
     static_assert(PER_SM * (BYTES + 1024) <= 233472, "shared memory of an SM");
 };
 
@@ -102,6 +102,17 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int
 __device__ __forceinline__ void peer_add(uint32_t a, uint64_t v) {
     asm volatile("red.relaxed.cluster.shared::cluster.add.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
+// The first 4, 8 or 16 of a thread's scores to that many columns of TMEM.
+__device__ __forceinline__ void tmem_put(uint32_t taddr, int width, const int32_t (&r)[16]) {
+    if (width == 4)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                     "r"(r[3]));
+    else if (width == 8)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+                     "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]));
+    else
+        tmem_st16(taddr, r);
+}
 // A float as an integer of the same order, and back.
 __device__ __forceinline__ int ordered(int b) { return b ^ ((b >> 31) & 0x7fffffff); }
 
@@ -127,9 +138,8 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
     // [SLOTS] the products of a block are done: its slot is free, the scores of its tile are there (K), the digits of its
     // tile have been read (V). One arrival for all: each costs the issuing warp 130 clocks.
     uint64_t* empty = full + C::SLOTS;
-    uint64_t* s_free = empty + C::SLOTS;         // [2] scores that stay have been seen (the products run two tiles ahead)
-    uint64_t* r_free = s_free + 2;               // [2] scores formed again have been read
-    uint64_t* p_full = r_free + 2;               // [2]
+    uint64_t* s_free = empty + C::SLOTS;         // [2] scores have been read
+    uint64_t* p_full = s_free + 2;               // [2]
     uint64_t* k_full = p_full + 2;               // [SCALES]
     uint64_t* k_free = k_full + C::SCALES;       // [SCALES]
     uint64_t* q_full = k_free + C::SCALES;
@@ -173,7 +183,6 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_free[i], 4);
-            mbar_init(&r_free[i], 4);
             mbar_init(&p_full[i], 4);
         }
         for (int i = 0; i < C::SCALES; ++i) {
@@ -196,7 +205,9 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
     const KeyTiles all_tiles(p0, p1, a.window, a.sinks);
     // this block's share of the tiles
     const int i_first = (int)((long long)all_tiles.n * rank / ranks), i_last = (int)((long long)all_tiles.n * (rank + 1) / ranks);
-    const int n = i_last - i_first, n_again = max(0, n - C::KEEP);
+    const int n = i_last - i_first;
+    // the scores of the first `keep` tiles stay, `width` columns a tile
+    const int width = n_rows <= 4 ? 4 : n_rows <= 8 ? 8 : 16, keep = C::KEEP / width;
     auto tile_at = [&](int i) { return all_tiles.at(i_first + i); };
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(C::COLS));
@@ -217,8 +228,8 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
     // Blocks of K and V in the order in which they are loaded and used: all K, then V of tile i, preceded by K of tile
     // i + 1 where its scores did not stay. The number of the last block of K (first, again) and of V of tile i:
     auto k_block = [&](int i) { return (i + 1) * NK - 1; };
-    auto k_again = [&](int i) { return (n + i - 1 + (i - C::KEEP) + 1) * NK - 1; };
-    auto v_block = [&](int i) { return (n + i + max(0, min(i + 2, n) - C::KEEP) + 1) * NK - 1; };
+    auto k_again = [&](int i) { return (n + i - 1 + (i - keep) + 1) * NK - 1; };
+    auto v_block = [&](int i) { return (n + i + max(0, min(i + 2, n) - keep) + 1) * NK - 1; };
     const bool soft = warp < C::SOFT;
 
     if (warp == C::SOFT) {
@@ -266,9 +277,9 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
             for (int i = 0; alive && i < n; ++i) {
                 const int pc = page_of(i + 2);
                 if (ph == 0) {
-                    load(&map_k, i, pa, i < C::KEEP);
+                    load(&map_k, i, pa, i < keep);
                 } else {
-                    if (i + 1 >= C::KEEP && i + 1 < n) load(&map_k, i + 1, pb, true);
+                    if (i + 1 >= keep && i + 1 < n) load(&map_k, i + 1, pb, true);
                     if (alive) load(&map_v, i, pa, true);
                 }
                 pa = pb;
@@ -287,15 +298,15 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
             const uint32_t qd = desc_k(smem_u32(sm + C::Q)), kd = desc_k(smem_u32(sm + C::RING)),
                            pd = desc_k(smem_u32(sm + C::P)), vd = desc_mn(smem_u32(sm + C::RING));
             int s = 0;
-            uint32_t phase = 0, again = 0, oc = 0;
+            uint32_t phase = 0, number = 0, oc = 0;
             bool ok = warp_wait(q_full, 0, err, dg::ERR_TIMEOUT_FULL);
             auto next = [&]() {
                 if (++s == C::SLOTS) s = 0, phase ^= 1;
             };
-            auto scores = [&](int i, bool stays) {
-                const uint32_t b = stays ? i & 1 : again & 1, use = stays ? i >> 1 : again >> 1;
-                ok = ok && warp_wait(stays ? &s_free[b] : &r_free[b], (use & 1u) ^ 1u, err, dg::ERR_TIMEOUT_ACCUM);
-                const uint32_t d = tmem + (stays ? 16 * i : C::AGAIN + 16 * b);
+            auto scores = [&]() {  // number `number` over both phases: two ahead of their readers
+                const uint32_t b = number & 1, d = tmem + C::FRESH + 16 * b;
+                ok = ok && warp_wait(&s_free[b], ((number >> 1) & 1u) ^ 1u, err, dg::ERR_TIMEOUT_ACCUM);
+                ++number;
 #pragma unroll
                 for (int x = 0; x < NK; ++x) {
                     ok = ok && warp_wait(&full[s], phase, err, dg::ERR_TIMEOUT_FULL);
@@ -308,11 +319,10 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
                     umma_arrive(issue, &empty[s]);
                     next();
                 }
-                if (!stays) ++again;
             };
-            for (int i = 0; ok && i < n; ++i) scores(i, i < C::KEEP);
+            for (int i = 0; ok && i < n; ++i) scores();
             for (int i = 0; ok && i < n; ++i) {
-                if (i + 1 >= C::KEEP && i + 1 < n) scores(i + 1, false);
+                if (i + 1 >= keep && i + 1 < n) scores();
                 ok = ok && warp_wait(&p_full[i & 1], (i >> 1) & 1u, err, dg::ERR_TIMEOUT_ACCUM);
 #pragma unroll
                 for (int x = 0; x < NK; ++x) {
@@ -407,18 +417,19 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
     auto block_done = [&](int q) {
         return wait(&empty[q % C::SLOTS], (uint32_t)(q / C::SLOTS) & 1u, err, dg::ERR_TIMEOUT_ACCUM);
     };
-    // the scores of tile i and its keys' scales; `stays` tiles of phase 1 are in TMEM already
+    // the scores of tile i and its keys' scales, for the u'th time
     auto next_scores = [&](int i, int u) {
-        const bool stays = i < C::KEEP;
-        // the scores that do not stay are numbered over both phases
-        const uint32_t again = (uint32_t)(i - C::KEEP + (u < n ? 0 : n_again)), b = again & 1;
-        if (!stays || u < n) ok = block_done(u < n ? k_block(i) : k_again(i));
+        const bool fresh = u < n || i >= keep;
+        const uint32_t b = (uint32_t)(u < n ? i : n + i - keep) & 1;
+        if (fresh) ok = block_done(u < n ? k_block(i) : k_again(i));
         ok = ok && wait(&k_full[u & 3], (u >> 2) & 1u, err, dg::ERR_TIMEOUT_FULL);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
         asm volatile("tcgen05.fence::after_thread_sync;");
-        dg::tmem_ld16(lane_addr + (stays ? 16 * i : C::AGAIN + 16 * b), s16);
+        const uint32_t kept = lane_addr + width * i;
+        dg::tmem_ld16(fresh ? lane_addr + C::FRESH + 16 * b : kept, s16);  // what lies behind the rows is not looked at
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (u < n && i < keep) tmem_put(kept, width, s16);
         asm volatile("tcgen05.fence::before_thread_sync;");
         const uint32_t* f = (const uint32_t*)(sm + C::KEY_SCALES) + (u & 3) * 2 * TILE_KEYS;
         kf = __uint_as_float(f[key]);
@@ -426,11 +437,7 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
         __syncwarp();
         if (lane == 0) {
             mbar_arrive(&k_free[u & 3]);
-            if (!stays) {
-                mbar_arrive(&r_free[b]);
-            } else if (u < n) {
-                mbar_arrive(&s_free[i & 1]);
-            }
+            if (fresh) mbar_arrive(&s_free[b]);
         }
     };
     // bit r: row r sees this thread's key of the tile
@@ -499,6 +506,7 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
                 }
             }
         }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");  // what was kept
 #pragma unroll
         for (int r = 0; r < FEW_ROWS; ++r) {
             if (r >= n_rows) break;
