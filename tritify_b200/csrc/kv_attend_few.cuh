@@ -452,9 +452,10 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
         return m;
     };
     if (soft) {
-        // the queries, up to B rows of one token at a time
+        // the queries, up to B rows of one token at a time: two a warp, since the
+        // block waits for them (with four, one sequence of 1000 keys took 16.4 us, not 15.4)
         if (threadIdx.x < FEW_ROWS) s_pos[threadIdx.x] = threadIdx.x < n_rows ? len - n_new + (row0 + (int)threadIdx.x) / g : -1;
-        constexpr int B = RowBatch<NK>::B;
+        constexpr int B = 2;
 #pragma unroll 1
         for (int rb = B * warp; rb < n_rows; rb += C::SOFT * B) {
             int count = 0;
@@ -464,11 +465,11 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
                 count = min(min(rb + B, n_rows) - r, g - hq);
                 if (pos < 0) continue;
                 const int32_t* x = a.q + ((long long)begin + t) * a.ld_q + (long long)(head * g + hq) * dim;
-                const RawBatch<NK> raw = fetch_rows<NK>(x, count, dim, a.vec, a.rope);
+                const RawBatch<NK, B> raw = fetch_rows<NK, B>(x, count, dim, a.vec, a.rope);
                 const longlong2 sc = a.scale[((long long)begin + t) * a.scale_stride];
                 const int2* cs = rope_row(a.rope, a.err, pos);
-                RowBatch<NK> rows;
-                turn_rows<NK>(rows, raw, x, count, dim, a.rope, cs);
+                RowBatch<NK, B> rows;
+                turn_rows(rows, raw, x, count, dim, a.rope, cs);
                 const double m = __ddiv_rn(127.0, fmax(rows.top, 1.0));
                 if (lane < count) s_theta[r + lane] = row_theta(rows.top, scale_value(sc, cs ? 30 : 0), a.soft);
 #pragma unroll

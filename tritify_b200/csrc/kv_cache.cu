@@ -84,7 +84,7 @@ int row_blocks(ktmoe_ctx* ctx, int64_t rows, int chunks, unsigned* blocks) {
 
 template <int NB>
 int launch_append(ktmoe_ctx* ctx, cudaStream_t st, const kv::AppendArgs& a) {
-    const int chunks = 2 * ((a.c.heads + kv::RowBatch<NB>::B - 1) / kv::RowBatch<NB>::B);  // of keys and of values
+    const int chunks = 2 * ((a.c.heads + kv::BATCH<NB> - 1) / kv::BATCH<NB>);  // of keys and of values
     unsigned blocks;
     if (int r = row_blocks(ctx, a.b.rows, chunks, &blocks)) return r;
     KLAUNCH(st, blocks, 32 * kv::ROW_WARPS, 0, (kv::append_kernel<NB>), a, (unsigned)chunks);
@@ -114,7 +114,7 @@ int launch_tile(ktmoe_ctx* ctx, cudaStream_t st, const kv::AttendArgs& a) {
     CUtensorMap mk, mv;
     if (int r = make_pool_map(ctx, &mk, a.c.k, a.c)) return r;
     if (int r = make_pool_map(ctx, &mv, a.c.v, a.c)) return r;
-    const int chunks = (a.c.heads * a.group + kv::RowBatch<NK>::B - 1) / kv::RowBatch<NK>::B;
+    const int chunks = (a.c.heads * a.group + kv::BATCH<NK> - 1) / kv::BATCH<NK>;
     unsigned blocks;
     if (int r = row_blocks(ctx, a.b.rows, chunks, &blocks)) return r;
     KLAUNCH(st, blocks, 32 * kv::ROW_WARPS, 0, (kv::query_kernel<NK>), a, (unsigned)chunks);

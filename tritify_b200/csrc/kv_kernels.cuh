@@ -167,8 +167,9 @@ __device__ __forceinline__ uint32_t uabs(int32_t v) { return v < 0 ? 0u - (uint3
 // the elements 4 l .. 4 l + 3 of each 128 (NB of them). Elements are turned into RN64 of their codes at once, which is
 // all that what follows needs: RN64 keeps the order, so the largest element's is the largest.
 template <int NB>
+constexpr int BATCH = NB == 1 ? 4 : 2;
+template <int NB, int B = BATCH<NB>>
 struct RowBatch {
-    static constexpr int B = NB == 1 ? 4 : 2;
     double y[B][NB][4];
     double top;  // lane i: of head i
 };
@@ -187,18 +188,18 @@ __device__ __forceinline__ void fetch_turn(int2 (&c)[4], const Rope& r, const in
 
 // The elements as they lie and those that the rotation mixes them with: asked for before anything is known of the row's
 // place, so that both arrive together. x: the first head's row, `heads` of them (the others count as zeros).
-template <int NB>
+template <int NB, int B = BATCH<NB>>
 struct RawBatch {
-    int4 v[RowBatch<NB>::B][NB], o[RowBatch<NB>::B][NB];
+    int4 v[B][NB], o[B][NB];
 };
-template <int NB>
-__device__ __forceinline__ RawBatch<NB> fetch_rows(const int32_t* __restrict__ x, int heads, int dim, int vec, const Rope& r) {
+template <int NB, int B = BATCH<NB>>
+__device__ __forceinline__ RawBatch<NB, B> fetch_rows(const int32_t* __restrict__ x, int heads, int dim, int vec, const Rope& r) {
     const int lane = threadIdx.x & 31;
     const bool far = r.table && turns_by_four(r) && !r.interleaved;
-    RawBatch<NB> w;
+    RawBatch<NB, B> w;
     auto fetch = [&](auto four) {
 #pragma unroll
-        for (int i = 0; i < RowBatch<NB>::B; ++i)
+        for (int i = 0; i < B; ++i)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const int e = 4 * lane + 128 * b;
@@ -213,10 +214,9 @@ __device__ __forceinline__ RawBatch<NB> fetch_rows(const int32_t* __restrict__ x
 }
 
 // cs: the rotation table's row (null: none).
-template <int NB>
-__device__ __forceinline__ void turn_rows(RowBatch<NB>& out, const RawBatch<NB>& w, const int32_t* __restrict__ x, int heads,
+template <int NB, int B>
+__device__ __forceinline__ void turn_rows(RowBatch<NB, B>& out, const RawBatch<NB, B>& w, const int32_t* __restrict__ x, int heads,
                                           int dim, const Rope& r, const int2* cs) {
-    constexpr int B = RowBatch<NB>::B;
     const int lane = threadIdx.x & 31;
     const bool by_four = cs && turns_by_four(r);
     const auto& v = w.v;
@@ -317,7 +317,7 @@ constexpr int ROW_WARPS = 4;
 template <int NB>
 __global__ void __launch_bounds__(32 * ROW_WARPS, 8) append_kernel(const AppendArgs a, unsigned chunks) {
     kt::pdl_enter();
-    constexpr int B = RowBatch<NB>::B;
+    constexpr int B = BATCH<NB>;
     const int lane = threadIdx.x & 31, dim = a.c.dim;
     const unsigned u = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
     const int t = (int)(u / chunks), c = (int)(u % chunks);
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, 8) append_kernel(const AppendA
     const long long page = pool_page(a.b, a.c, a.err, p.seq, p.pos >> a.c.page_shift);
     const int2* cs = rope_row(rope, a.err, p.pos);
     RowBatch<NB> rows;
-    turn_rows<NB>(rows, raw, x, heads, dim, rope, cs);
+    turn_rows(rows, raw, x, heads, dim, rope, cs);
     const double s = scale_value(sc, cs ? 30 : 0);
     const double want = __ddiv_rn(__dmul_rn(rows.top, s), 127.0);
     const uint32_t sg = sigma_bits(want);
@@ -481,7 +481,7 @@ __device__ __forceinline__ float row_theta(double top, double s, double soft) {
 template <int NB>
 __global__ void __launch_bounds__(32 * ROW_WARPS, 8) query_kernel(const AttendArgs a, unsigned chunks) {
     kt::pdl_enter();
-    constexpr int B = RowBatch<NB>::B;
+    constexpr int B = BATCH<NB>;
     const int lane = threadIdx.x & 31, dim = a.c.dim;
     const unsigned u = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
     const int t = (int)(u / chunks), h0 = (int)(u % chunks) * B, heads = min(B, a.c.heads * a.group - h0);
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, 8) query_kernel(const AttendAr
     const longlong2 sc = a.scale[(long long)t * a.scale_stride];
     const int2* cs = rope_row(a.rope, a.err, p.pos);
     RowBatch<NB> rows;
-    turn_rows<NB>(rows, raw, x, heads, dim, a.rope, cs);
+    turn_rows(rows, raw, x, heads, dim, a.rope, cs);
     const double m = __ddiv_rn(127.0, fmax(rows.top, 1.0));
     int32_t* out = a.o + (long long)t * a.ld_o + (long long)h0 * dim;
     const float theta = row_theta(rows.top, scale_value(sc, cs ? 30 : 0), a.soft);
