@@ -243,6 +243,8 @@ def test_refusals(ctx):
         a.set_mask(window=-1)
     with pytest.raises(tb.KtmoeError):
         a.set_mask(softmax_scale=float("nan"))
+    with pytest.raises(ValueError):
+        a.set_mask(window=1 << 32)
     with pytest.raises(tb.KtmoeError) as e:  # another head size
         a.forward_dev(tb.KvCache(ctx, 2, 16, 1, 32), batch, 16, 16, 16, 16)
     assert e.value.status == _native.ERR_ARG

@@ -134,7 +134,7 @@ def test_the_classes_refuse_what_does_not_fit():
             ok.append(b, k, v, sc)
     with pytest.raises(ValueError):
         ok.read(b, kv, kv)  # float32 outputs
-    for kw in (dict(n_heads=3), dict(n_heads=0), dict(n_heads=2), dict(window=-1), dict(sinks=-2),
+    for kw in (dict(n_heads=3), dict(n_heads=0), dict(n_heads=2), dict(window=-1), dict(sinks=-2), dict(window=1 << 32), dict(sinks=1 << 31),
                dict(out_scale=_cpu(6, 2, 2, dtype="int64")), dict(out_scale=_cpu(7, 4, dtype="int64")),
                dict(out=_cpu(7, 127)), dict(q=_cpu(3, 128))):
         a = dict(q=q, scale=s, out=o, out_scale=os_, n_heads=4)

@@ -848,6 +848,8 @@ class AttentionHalf:
 
     def set_mask(self, window: int = 0, sinks: int = 0, softmax_scale: float = 0.0) -> None:
         """A sliding window with the first ``sinks`` positions kept; softmax_scale 0: head_dim ** -0.5."""
+        if max(abs(int(window)), abs(int(sinks))) >= 1 << 31:
+            raise ValueError("window and sinks: below 2^31")
         self.ctx.check(lib().ktmoe_attn_set_mask(self._h, float(softmax_scale), int(window), int(sinks)))
 
     def forward_dev(self, cache: KvCache, batch: KvBatch, x_ptr: int, x_scale_ptr: int, y_ptr: int, y_scale_ptr: int,

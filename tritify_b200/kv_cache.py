@@ -199,8 +199,8 @@ class KvCache:
         cache, which already holds their keys and values, into ``out`` (int32 [rows][n_heads * head_dim]) at
         ``out_scale`` (int64 [rows][n_kv_heads][2]). ``softmax_scale`` defaults to head_dim ** -0.5; ``window`` > 0
         keeps the last ``window`` positions and the first ``sinks``."""
-        if n_heads < 1 or n_heads % self.n_kv_heads != 0 or window < 0 or sinks < 0:
-            raise ValueError("n_heads: a multiple of n_kv_heads; window and sinks: not negative")
+        if n_heads < 1 or n_heads % self.n_kv_heads != 0 or not (0 <= window < 1 << 31 and 0 <= sinks < 1 << 31):
+            raise ValueError("n_heads: a multiple of n_kv_heads; window and sinks: from 0 to 2^31 - 1")
         width, rows, int32 = n_heads * self.head_dim, batch.rows, _torch.int32
         ld_q = _matrix(q, "q", int32, rows, width)
         ld_o = _matrix(out, "out", int32, rows, width)
