@@ -7,7 +7,7 @@
 // digits of the weights in one product of 32 columns). A thread has one key of a tile.
 //
 // The row maxima must be known before the first weight is rounded, so there are two phases; K is read once all the same,
-// because the scores wait in TMEM, 4, 8 or 16 columns a tile for as many rows (with 16 for any number the decode of 64
+// because the scores wait in TMEM, 4, 8, 12 or 16 columns a tile for as many rows (with 16 for any number the decode of 64
 // sequences of 4096 by 4 rows took 111 us, not 96). Only tiles beyond what a block has room for are formed again. While the
 // cluster exchanges its maxima, V is already on its way. Sums over the keys are integers, so the shares of a cluster
 // add up to the same bits in any order: each block adds its own into the shared memory of the block that writes them out.
@@ -102,12 +102,15 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int
 __device__ __forceinline__ void peer_add(uint32_t a, uint64_t v) {
     asm volatile("red.relaxed.cluster.shared::cluster.add.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
-// The first 4, 8 or 16 of a thread's scores to that many columns of TMEM.
+// The first 4, 8, 12 or 16 of a thread's scores to that many columns of TMEM.
 __device__ __forceinline__ void tmem_put(uint32_t taddr, int width, const int32_t (&r)[16]) {
+    if (width == 12)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr + 8), "r"(r[8]), "r"(r[9]),
+                     "r"(r[10]), "r"(r[11]));
     if (width == 4)
         asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                      "r"(r[3]));
-    else if (width == 8)
+    else if (width <= 12)
         asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
                      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]));
     else
@@ -207,7 +210,7 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
     const int i_first = (int)((long long)all_tiles.n * rank / ranks), i_last = (int)((long long)all_tiles.n * (rank + 1) / ranks);
     const int n = i_last - i_first;
     // the scores of the first `keep` tiles stay, `width` columns a tile
-    const int width = n_rows <= 4 ? 4 : n_rows <= 8 ? 8 : 16, keep = C::KEEP / width;
+    const int width = (n_rows + 3) & ~3, keep = C::KEEP / width;
     auto tile_at = [&](int i) { return all_tiles.at(i_first + i); };
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(C::COLS));
