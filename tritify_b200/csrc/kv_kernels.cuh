@@ -163,7 +163,7 @@ __device__ __forceinline__ int to_int(double v) { return __double2loint(__dadd_r
 __device__ __forceinline__ uint32_t uabs(int32_t v) { return v < 0 ? 0u - (uint32_t)v : (uint32_t)v; }
 
 // ── rows of codes: rotation, largest element, quantisation ──
-// A warp takes up to B heads of one token, which share the rotation's entries, the scale and one division; lane l has
+// A warp takes up to B heads of one token (BATCH, fewer where there are no more), which share the rotation's entries, the scale and one division; lane l has
 // the elements 4 l .. 4 l + 3 of each 128 (NB of them). Elements are turned into RN64 of their codes at once, which is
 // all that what follows needs: RN64 keeps the order, so the largest element's is the largest.
 template <int NB>
@@ -314,10 +314,9 @@ struct AppendArgs {
 
 constexpr int ROW_WARPS = 4;
 
-template <int NB>
+template <int NB, int B>
 __global__ void __launch_bounds__(32 * ROW_WARPS, 8) append_kernel(const AppendArgs a, unsigned chunks) {
     kt::pdl_enter();
-    constexpr int B = BATCH<NB>;
     const int lane = threadIdx.x & 31, dim = a.c.dim;
     const unsigned u = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
     const int t = (int)(u / chunks), c = (int)(u % chunks);
@@ -328,13 +327,13 @@ __global__ void __launch_bounds__(32 * ROW_WARPS, 8) append_kernel(const AppendA
     const int32_t* x = (is_v ? a.v + (long long)t * a.ld_v : a.k + (long long)t * a.ld_k) + (long long)h0 * dim;
     Rope rope = a.rope;
     if (is_v) rope.table = nullptr;
-    const RawBatch<NB> raw = fetch_rows<NB>(x, heads, dim, a.vec, rope);
+    const RawBatch<NB, B> raw = fetch_rows<NB, B>(x, heads, dim, a.vec, rope);
     Place p;
     if (!locate(a.b, a.err, t, a.c.page_shift, p) || p.pos < 0) return;
     const longlong2 sc = a.scale[is_v][(long long)t * a.scale_stride];
     const long long page = pool_page(a.b, a.c, a.err, p.seq, p.pos >> a.c.page_shift);
     const int2* cs = rope_row(rope, a.err, p.pos);
-    RowBatch<NB> rows;
+    RowBatch<NB, B> rows;
     turn_rows(rows, raw, x, heads, dim, rope, cs);
     const double s = scale_value(sc, cs ? 30 : 0);
     const double want = __ddiv_rn(__dmul_rn(rows.top, s), 127.0);
