@@ -1,0 +1,104 @@
+"""Attention over the paged cache where a key that a row does not see could show in it all the same: value scales far
+above those that it sees, on a B200, against the plain 64-bit restatement (tests/kv_reference.py). All arithmetic is exact
+by definition, so the tolerance is zero. Setup.check runs each batch through the few-row kernel and, with copies of all
+heads, through the tile kernel."""
+
+import numpy as np
+import pytest
+
+import tritify_b200 as tb
+from test_gpu_kv import Setup, _torch
+
+pytestmark = pytest.mark.gpu
+
+
+def positions_of(s, b):
+    """Pool pages and places of a sequence's positions."""
+    j = np.arange(s.kv_len[b])
+    return s.table[b, j // s.page], j % s.page
+
+
+def set_value_scales(s, b, sigma):
+    """sigma [kv_len]: of every KV head."""
+    page, place = positions_of(s, b)
+    s.pool["vs"][page, :, place] = sigma[:, None]
+
+
+SHAPES = [  # new, total, query heads, KV heads, dim, page
+    (64, 64, 4, 1, 64, 16),
+    (150, 150, 3, 1, 128, 64),
+    (70, 200, 4, 2, 48, 32),
+    (64, 64, 4, 1, 256, 16),
+]
+
+
+@pytest.mark.parametrize("step", [17, 20, 40, 126])
+@pytest.mark.parametrize("shape", SHAPES, ids=[str(i) for i in range(len(SHAPES))])
+def test_later_tokens_of_larger_scales(ctx, shape, step):
+    """Value scales that rise by 2^step every few tokens, and fall back: what a row does not see yet weighs nothing."""
+    new, kv, heads, hk, dim, page = shape
+    s = Setup(ctx, [(new, kv)], heads, hk, dim, page, seed=step)
+    j = np.arange(kv)
+    set_value_scales(s, 0, np.exp2((step * (j // 5)) % 127 - 64.0) * (1 + (j % 3) / 4))
+    s.push()
+    s.check(s.codes(heads * dim), s.scales())
+
+
+@pytest.mark.parametrize("first", [0, 30])
+def test_a_first_value_of_zeros(ctx, first):
+    """The first value row is zeros (at 2^-64, as the cache writes it) and stands alone for row 0: zeros, at its scale."""
+    s = Setup(ctx, [(64, 64 + first)], 4, 1, 64, 16, seed=first)
+    page, place = positions_of(s, 0)
+    s.pool["v"][page[:first + 1], :, place[:first + 1]] = 0
+    s.pool["vs"][page[:first + 1], :, place[:first + 1]] = 2.0 ** -64
+    s.push()
+    got, got_s, want, want_s = s.attend(s.codes(4 * 64), s.scales())
+    assert (want[0] == 0).all() and (want[1] != 0).any()
+    assert (got == want).all() and (got_s == want_s).all()
+
+
+@pytest.mark.parametrize("window,sinks", [(10, 0), (10, 3), (100, 1)])
+@pytest.mark.parametrize("step", [20, 40, 110])
+@pytest.mark.parametrize("since", [236, 240])  # 236: the first new token sees its own
+def test_larger_scales_outside_the_window(ctx, since, window, sinks, step):
+    s = Setup(ctx, [(64, 300)], 4, 1, 64, 32, seed=window + step)
+    sigma = np.full(300, 2.0 ** -50)
+    sigma[sinks:236 - window + 1] = 2.0 ** (step - 50)  # what no new token sees, but tiles hold with what they see
+    sigma[since:260:7] = 2.0 ** (step - 50)  # what some of them see
+    set_value_scales(s, 0, sigma)
+    s.push()
+    s.check(s.codes(4 * 64), s.scales(), window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("hk", [2, 60])  # 60: the whole prompt goes to the tile kernel
+def test_a_prompt_equals_its_tokens(ctx, hk):
+    """A written prompt whose values grow from zeros over 2^80, at once and token by token."""
+    torch = _torch()
+    n, heads, dim, page = 140, 3 * hk, 64, 16
+    rng = np.random.default_rng(4)
+    kv = torch.from_numpy(rng.integers(-2 ** 28, 2 ** 28, (n, 2 * hk * dim)).astype(np.int32)).cuda()
+    kv[0, hk * dim:] = 0
+    q = torch.from_numpy(rng.integers(-2 ** 28, 2 ** 28, (n, heads * dim)).astype(np.int32)).cuda()
+    scale = torch.from_numpy(np.stack([rng.integers(2 ** 31, 2 ** 32, n), rng.integers(59, 63, n)], -1)).cuda()
+    v_scale = torch.from_numpy(np.stack([rng.integers(2 ** 31, 2 ** 32, n), 110 - 80 * np.arange(n) // n], -1)).cuda()
+    pages = torch.arange(-(-n // page), dtype=torch.int32, device="cuda")[None]
+    results = []
+    for sizes in ([n], [1] * n):
+        cache = tb.KvCache(ctx, pages.shape[1], page, hk, dim)
+        o = torch.zeros(n, heads * dim, dtype=torch.int32, device="cuda")
+        os_ = torch.zeros(n, hk, 2, dtype=torch.int64, device="cuda")
+        at = 0
+        for c in sizes:
+            b = tb.KvBatch(torch.tensor([0, c], dtype=torch.int32, device="cuda"),
+                           torch.tensor([at + c], dtype=torch.int32, device="cuda"), pages, c)
+            x = kv[at:at + c]
+            cache.append(b, x[:, :hk * dim], x[:, hk * dim:], scale[at:at + c], v_scale=v_scale[at:at + c])
+            before = ctx.launch_count()
+            cache.attention(b, q[at:at + c], scale[at:at + c], o[at:at + c], os_[at:at + c], heads)
+            assert ctx.launch_count() - before == (2 if c == n and hk == 60 else 1)
+            at += c
+        ctx.sync()
+        torch.cuda.synchronize()
+        results.append((o.cpu(), os_.cpu()))
+    assert int((results[1][0][0] != 0).sum()) == 0
+    assert all(torch.equal(a, b) for a, b in zip(*results))

@@ -178,7 +178,8 @@ __device__ __forceinline__ RowWeights row_weights(float top, float theta, int e)
     return r;
 }
 
-// weight() for a pair, times 2^-E. MASK: keys whose bit of `seen` is clear weigh nothing.
+// weight() for a pair, times 2^-E. MASK: keys whose bit of `seen` is clear weigh nothing, exactly: even 2^-32 of a weight
+// would show, since 2^E bounds the value scales of visible keys alone.
 template <bool MASK>
 __device__ __forceinline__ f2 weight2(f2 x, const RowWeights& w, uint32_t seen) {
     const f2 minus = pk(-1.0f, -1.0f);
@@ -187,10 +188,6 @@ __device__ __forceinline__ f2 weight2(f2 x, const RowWeights& w, uint32_t seen) 
     upk(fma2(d, w.ntheta, pk(12288.0f, 12288.0f)), a, b);
     a = fmaxf(a, 12256.0f);
     b = fmaxf(b, 12256.0f);
-    if (MASK) {
-        a = (seen & 1) ? a : 12256.0f;
-        b = (seen & 2) ? b : 12256.0f;
-    }
     const f2 f = pk(a, b);
     const f2 f0 = add2(f, pk(12570624.0f, 12570624.0f));
     const f2 r = fma2(add2(f0, pk(-12570624.0f, -12570624.0f)), minus, f);
@@ -200,8 +197,13 @@ __device__ __forceinline__ f2 weight2(f2 x, const RowWeights& w, uint32_t seen) 
     float e0, e1, n0, n1;
     upk(e, e0, e1);
     upk(f0, n0, n1);
-    return pk(__uint_as_float(__float_as_uint(e0) + (__float_as_uint(n0) << 23)),
-              __uint_as_float(__float_as_uint(e1) + (__float_as_uint(n1) << 23)));
+    e0 = __uint_as_float(__float_as_uint(e0) + (__float_as_uint(n0) << 23));
+    e1 = __uint_as_float(__float_as_uint(e1) + (__float_as_uint(n1) << 23));
+    if (MASK) {
+        e0 = (seen & 1) ? e0 : 0.0f;
+        e1 = (seen & 2) ? e1 : 0.0f;
+    }
+    return pk(e0, e1);
 }
 
 // The keys that a tile's rows at positions p0 .. p1 see, as a list of 128-key tiles: first those of the sinks, then
