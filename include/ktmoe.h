@@ -268,7 +268,8 @@ typedef struct ktmoe_kv_cache {
 /* The new tokens of a batch of sequences, described in device memory: sequence b's rows are q_begin[b] to
  * q_begin[b + 1] - 1 (ascending offsets) of the calls' buffers, which hold `rows` rows; its length with them is
  * kv_len[b], so row t stands at position kv_len[b] - (q_begin[b + 1] - t); position p lies in pool page
- * page_table[b * max_pages + p / page_tokens]. Rows before the first and behind the last sequence are left as they
+ * page_table[b * max_pages + p / page_tokens]. Pages up to kv_len are pages of the pool, seen through a window or not;
+ * places that no row sees may hold anything. Rows before the first and behind the last sequence are left as they
  * are. A row at a negative position (a length below the new tokens) has no place in the cache: append and read skip
  * it, attention gives zeros. What only the device can see wrong (a page outside the pool, offsets that do not ascend
  * or leave the rows, a length beyond the page table, a position beyond the rotation table) touches nothing outside

@@ -102,3 +102,31 @@ def test_a_prompt_equals_its_tokens(ctx, hk):
         results.append((o.cpu(), os_.cpu()))
     assert int((results[1][0][0] != 0).sum()) == 0
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+GARBAGE = [np.nan, np.inf, -np.inf, 2.0 ** 127, -1.0]
+
+
+@pytest.mark.parametrize("garbage", GARBAGE, ids=[str(g) for g in GARBAGE])
+@pytest.mark.parametrize("lens,heads,hk,dim,window,sinks", [
+    ([(1, 1), (1, 5), (1, 126), (1, 131)], 4, 1, 64, 0, 0),
+    ([(1, 198), (1, 67)], 4, 2, 128, 20, 2),
+    ([(64, 65)], 4, 1, 64, 0, 0),
+    ([(90, 201), (64, 64)], 4, 1, 128, 0, 0),
+    ([(64, 398)], 4, 1, 256, 100, 5),
+])
+def test_places_that_were_never_written(ctx, lens, heads, hk, dim, window, sinks, garbage):
+    """Pools of memory that nothing cleared: whatever lies behind a sequence's last token, and outside every window of
+    the call, shows nowhere."""
+    s = Setup(ctx, lens, heads, hk, dim, 16, seed=dim)
+    seen = np.zeros(s.pool["vs"].shape, bool)
+    for b, (new, kv) in enumerate(lens):
+        j = np.arange(kv)
+        if window:
+            j = j[(j > kv - new - window) | (j < sinks)]
+        seen[s.table[b, j // 16], :, j % 16] = True
+    for n in "kv":
+        s.pool[n][~seen] = -1
+        s.pool[n + "s"][~seen] = garbage
+    s.push()
+    s.check(s.codes(heads * dim), s.scales(), window=window, sinks=sinks)

@@ -395,7 +395,9 @@ __global__ void __launch_bounds__(FewCfg<NK, PER_SM>::THREADS, PER_SM)
                     alive = __all_sync(0xffffffffu, alive);
                     if (!alive) break;
                     uint32_t* f = (uint32_t*)(sm + C::KEY_SCALES) + j * 2 * TILE_KEYS;
-                    const uint4 w = val[j];
+                    uint4 w = val[j];
+                    w.z = held_scales(w.z);
+                    w.w = held_scales(w.w);
                     const uint32_t hi16 = 0xffff0000u;
                     *(uint4*)(f + 4 * lane) = make_uint4(w.x << 16, w.x & hi16, w.y << 16, w.y & hi16);
                     *(uint4*)(f + TILE_KEYS + 4 * lane) = make_uint4(w.z << 16, w.z & hi16, w.w << 16, w.w & hi16);

@@ -231,6 +231,10 @@ __device__ __forceinline__ uint32_t seen_bits(int j0, int pos, int window, int s
     return m;
 }
 
+// Two value scales (bfloat16) held at the largest there is, 2^63. A tile may hold places that no row sees and that were
+// never written: whatever lies there, 0xffff among it, is then a number, which a hidden key's weight of zero takes away.
+__device__ __forceinline__ uint32_t held_scales(uint32_t v) { return __vminu2(v, 0x5f005f00u); }
+
 // The last i in [0, n) with f(i) <= target (f ascends), by a whole warp; 0 when there is none.
 template <class F>
 __device__ __forceinline__ int warp_search(int n, long long target, F f) {
@@ -566,7 +570,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
                     alive = __all_sync(0xffffffffu, alive);
                     if (!alive) break;
                     float* f = (float*)(sm + C::KEY_SCALES) + j * C::KEY_STAGE;
-                    const uint4 w = val[j];
+                    uint4 w = val[j];
+                    w.z = held_scales(w.z);
+                    w.w = held_scales(w.w);
                     const uint32_t hi16 = 0xffff0000u;
                     const float4 kf = {__uint_as_float(w.x << 16), __uint_as_float(w.x & hi16),
                                        __uint_as_float(w.y << 16), __uint_as_float(w.y & hi16)};
