@@ -130,3 +130,15 @@ def test_places_that_were_never_written(ctx, lens, heads, hk, dim, window, sinks
         s.pool[n + "s"][~seen] = garbage
     s.push()
     s.check(s.codes(heads * dim), s.scales(), window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5, 2 ** 30])
+@pytest.mark.parametrize("sinks", [0, 3, 2 ** 31 - 1])
+def test_the_widest_windows(ctx, window, sinks):
+    """Rows at negative positions, which see nothing, in one group with rows that see keys, and a window near 2^31: it
+    hides nothing."""
+    s = Setup(ctx, [(19, 8), (41, 40)], 4, 1, 64, 16, rows_behind=1)
+    q, scale = s.codes(4 * 64), s.scales()
+    s.check(q, scale, window=window, sinks=sinks)
+    wide, narrow = s.attend(q, scale, window=window, sinks=sinks), s.attend(q, scale)
+    assert (wide[0] == narrow[0]).all() and (wide[1] == narrow[1]).all()

@@ -211,7 +211,7 @@ __device__ __forceinline__ f2 weight2(f2 x, const RowWeights& w, uint32_t seen) 
 struct KeyTiles {
     int n, n_sink, first;
     __device__ __forceinline__ KeyTiles(int p0, int p1, int window, int sinks) {
-        const int lo = window ? max(0, p0 + 1 - window) : 0;
+        const int lo = window && p0 >= window ? p0 + 1 - window : 0;  // p0 may lie far below zero
         first = lo / TILE_KEYS;
         n_sink = min((min(sinks, lo) + TILE_KEYS - 1) / TILE_KEYS, first);
         n = p1 < 0 ? 0 : n_sink + p1 / TILE_KEYS - first + 1;
