@@ -3459,6 +3459,8 @@ int ktmoe_attn_set_norm(ktmoe_attn* A, const int32_t* w_codes, ktmoe_scale w_sca
     ktmoe_ctx* ctx = A->ctx;
     std::lock_guard<std::mutex> lk(ctx->mu);
     if (int r = set_device(ctx)) return r;
+    for (int64_t i = 0; i < A->d; ++i)
+        if (w_codes[i] > kt::WLEVELS || w_codes[i] < -kt::WLEVELS) return fail(ctx, KTMOE_ERR_RANGE, "norm code");
     CK(A->b_norm.ensure(A->d * 4));
     CK(cudaMemcpy(A->b_norm.p, w_codes, A->d * 4, cudaMemcpyHostToDevice));
     A->norm_ws = S(w_scale);
