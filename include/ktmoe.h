@@ -341,7 +341,9 @@ typedef struct ktmoe_attn_config {
 int ktmoe_attn_create(ktmoe_ctx* ctx, const ktmoe_attn_config* cfg, ktmoe_attn** out);
 int ktmoe_attn_destroy(ktmoe_attn* attn);
 /* Codes and scales of QuantLinear::from_weights: q [n_heads * head_dim][d_model], k and v [n_kv_heads * head_dim]
- * [d_model], out [d_model][n_heads * head_dim]; the norm's as for ktmoe_layer_set_norm. Host pointers. */
+ * [d_model], out [d_model][n_heads * head_dim]; the norm's as for ktmoe_layer_set_norm. Host pointers. These and the
+ * rotation's setter wait for everything in flight on the device first. A forward that was captured before them reads the
+ * new codes at its own scales: capture it again. */
 int ktmoe_attn_set_qkv(ktmoe_attn* attn, const int32_t* q, ktmoe_scale q_scale, const int32_t* k, ktmoe_scale k_scale,
                        const int32_t* v, ktmoe_scale v_scale);
 int ktmoe_attn_set_out(ktmoe_attn* attn, const int32_t* out, ktmoe_scale out_scale);

@@ -1,4 +1,4 @@
-"""Setting an attention half's weights on a B200: what is refused."""
+"""Setting an attention half's weights: what is refused, and that a forward in flight keeps what it began with."""
 
 import numpy as np
 import pytest
@@ -20,3 +20,64 @@ def test_norm_codes_beyond_their_range(ctx, bad):
     with pytest.raises(tb.KtmoeError) as e:
         a.set_norm(codes, tb.Scale(1, 0), tb.Scale(0, 0))
     assert e.value.status == _native.ERR_RANGE
+
+
+def _linear(seed, out, k):
+    return tb.QuantLinear.from_weights("w", tb.synth_normal(seed, 1.0, out * k), out, k)
+
+
+def _half(ctx, seed):
+    a = tb.AttentionHalf(ctx, 64, 2, 1, 32)
+    set_all(a, seed)
+    return a
+
+
+def set_all(a, seed, only=None):
+    if only in (None, "qkv"):
+        a.set_qkv(_linear(seed, 64, 64), _linear(seed + 1, 32, 64), _linear(seed + 2, 32, 64))
+    if only in (None, "out"):
+        a.set_out(_linear(seed + 3, 64, 64))
+    if only in (None, "norm"):
+        norm = tb.QuantLinear.from_weights("n", tb.synth_normal(seed + 4, 1.0, 64), 1, 64)
+        a.set_norm(norm.w_codes, norm.w_scale, tb.scale_from_f64(1e-6))
+    if only in (None, "rope"):
+        a.set_rope(1e4 + 5e3 * seed, 32, 64)
+
+
+@pytest.mark.parametrize("what", ["norm", "rope", "qkv", "out"])
+def test_a_forward_in_flight_keeps_its_weights(ctx, what):
+    """A forward that waits on the caller's stream while a setter is called: it gives what it gave before the call, and
+    the next one what the new weights give."""
+    import torch
+
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    batch = tb.KvBatch(i32(0, 9), i32(9), i32(0).reshape(1, 1), 9)
+    x = torch.from_numpy(tb.IntTensor.from_reals(tb.synth_normal(9, 1.0, 9 * 64)).data.reshape(9, 64).copy()).cuda()
+    xs = torch.tensor([1, 28], dtype=torch.int64, device="cuda")
+    side = torch.cuda.Stream()
+
+    def forward(a, y, ys, wait):
+        with torch.cuda.stream(side):
+            if wait:
+                torch.cuda._sleep(200_000_000)  # about a tenth of a second
+            a.forward_dev(cache, batch, x.data_ptr(), xs.data_ptr(), y.data_ptr(), ys.data_ptr(), side.cuda_stream)
+
+    def results(n):
+        return [(torch.zeros_like(x), torch.zeros(2, dtype=torch.int64, device="cuda")) for _ in range(n)]
+
+    cache = tb.KvCache(ctx, 1, 16, 1, 32)
+    fresh = _half(ctx, 100)
+    set_all(fresh, 200, what)
+    a = _half(ctx, 100)
+    (first, delayed, after, want) = results(4)
+    torch.cuda.synchronize()
+    forward(a, *first, wait=False)
+    torch.cuda.synchronize()
+    forward(a, *delayed, wait=True)
+    set_all(a, 200, what)
+    forward(a, *after, wait=False)
+    forward(fresh, *want, wait=False)
+    ctx.sync(side.cuda_stream)
+    assert torch.equal(first[0], delayed[0]) and torch.equal(first[1], delayed[1])
+    assert torch.equal(after[0], want[0]) and torch.equal(after[1], want[1])
+    assert not torch.equal(first[0], after[0])

@@ -3247,6 +3247,13 @@ namespace {
 enum AttnScale { A_NORM = 0, A_XN = 2, A_HEADS = 3, A_MERGED = 5, A_ROWS = 6, A_M = 8, A_ADD = 9, A_NSCALES = 12 };
 enum AttnWord { AU_NORM = 0, AU_HEADS, AU_ROWS, AU_ADD, AU_N };
 
+// Before a setter overwrites what a forward reads: nothing is in flight on the device, whatever stream or graph it is on.
+// And after it: a copy from pageable memory returns once it is staged, and forwards on other streams do not wait for it.
+int attn_idle(ktmoe_ctx* ctx) {
+    CK(cudaDeviceSynchronize());
+    return KTMOE_OK;
+}
+
 cudaError_t attn_ensure(ktmoe_attn* A, DevBuf& b, size_t bytes) {
     if (A->captured && b.p && bytes > b.bytes) {
         A->retired.push_back(b);
@@ -3431,6 +3438,7 @@ int ktmoe_attn_set_qkv(ktmoe_attn* A, const int32_t* q, ktmoe_scale q_scale, con
     ktmoe_ctx* ctx = A->ctx;
     std::lock_guard<std::mutex> lk(ctx->mu);
     if (int r = set_device(ctx)) return r;
+    if (int r = attn_idle(ctx)) return r;
     A->qkv_set = false;
     if (int r = upload_matrix(ctx, A->w_qkv, 0, q, A->q, A->d, 0)) return r;
     if (int r = upload_matrix(ctx, A->w_qkv, 0, k, A->kv, A->d, A->q)) return r;
@@ -3447,6 +3455,7 @@ int ktmoe_attn_set_out(ktmoe_attn* A, const int32_t* out, ktmoe_scale out_scale)
     ktmoe_ctx* ctx = A->ctx;
     std::lock_guard<std::mutex> lk(ctx->mu);
     if (int r = set_device(ctx)) return r;
+    if (int r = attn_idle(ctx)) return r;
     A->out_set = false;
     if (int r = upload_matrix(ctx, A->w_out, 0, out, A->d, A->q, 0)) return r;
     A->out_ws = S(out_scale);
@@ -3461,8 +3470,10 @@ int ktmoe_attn_set_norm(ktmoe_attn* A, const int32_t* w_codes, ktmoe_scale w_sca
     if (int r = set_device(ctx)) return r;
     for (int64_t i = 0; i < A->d; ++i)
         if (w_codes[i] > kt::WLEVELS || w_codes[i] < -kt::WLEVELS) return fail(ctx, KTMOE_ERR_RANGE, "norm code");
+    if (int r = attn_idle(ctx)) return r;
     CK(A->b_norm.ensure(A->d * 4));
     CK(cudaMemcpy(A->b_norm.p, w_codes, A->d * 4, cudaMemcpyHostToDevice));
+    if (int r = attn_idle(ctx)) return r;
     A->norm_ws = S(w_scale);
     A->norm_eps = S(eps_scale);
     A->norm_set = true;
@@ -3483,13 +3494,14 @@ int ktmoe_attn_set_rope(ktmoe_attn* A, double theta, int32_t rot_dim, int64_t po
     std::vector<int32_t> table((size_t)positions * rot_dim);
     if (ktmoe_rope_table(theta, rot_dim, positions, table.data()) != KTMOE_OK)
         return fail(ctx, KTMOE_ERR_ARG, "theta must be positive and finite");
-    CK(cudaStreamSynchronize(ctx->stream));
+    if (int r = attn_idle(ctx)) return r;
     if (A->captured && A->b_rope.p) {  // a captured forward keeps the table that it was captured with
         A->retired.push_back(A->b_rope);
         A->b_rope = DevBuf{};
     }
     CK(A->b_rope.ensure(table.size() * 4));
     CK(cudaMemcpy(A->b_rope.p, table.data(), table.size() * 4, cudaMemcpyHostToDevice));
+    if (int r = attn_idle(ctx)) return r;
     A->rope = ktmoe_rope{A->b_rope.as<int32_t>(), positions, rot_dim, interleaved ? 1 : 0};
     return KTMOE_OK;
 }
