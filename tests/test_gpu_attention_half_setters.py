@@ -81,3 +81,35 @@ def test_a_forward_in_flight_keeps_its_weights(ctx, what):
     assert torch.equal(first[0], delayed[0]) and torch.equal(first[1], delayed[1])
     assert torch.equal(after[0], want[0]) and torch.equal(after[1], want[1])
     assert not torch.equal(first[0], after[0])
+
+
+def test_rotation_tables_that_grow_shrink_and_fail(ctx):
+    """Each set_rope gives what a half with that table alone gives; one that is refused leaves the last one."""
+    import torch
+
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    batch = tb.KvBatch(i32(0, 9), i32(9), i32(0).reshape(1, 1), 9)
+    x = torch.from_numpy(tb.IntTensor.from_reals(tb.synth_normal(9, 1.0, 9 * 64)).data.reshape(9, 64).copy()).cuda()
+    xs = torch.tensor([1, 28], dtype=torch.int64, device="cuda")
+    cache = tb.KvCache(ctx, 1, 16, 1, 32)
+
+    def result(a):
+        y, ys = torch.zeros_like(x), torch.zeros(2, dtype=torch.int64, device="cuda")
+        torch.cuda.synchronize()
+        a.forward_dev(cache, batch, x.data_ptr(), xs.data_ptr(), y.data_ptr(), ys.data_ptr())
+        ctx.sync()
+        return y.cpu(), ys.cpu()
+
+    a, seen = _half(ctx, 300), []
+    for theta, rot, positions in ((1e4, 32, 64), (2e4, 32, 5000), (3e4, 16, 20), (3e4, 8, 100000)):
+        a.set_rope(theta, rot, positions)
+        with pytest.raises(tb.KtmoeError):
+            a.set_rope(-1.0, 32, 64)
+        fresh = tb.AttentionHalf(ctx, 64, 2, 1, 32)
+        for what in ("qkv", "out", "norm"):
+            set_all(fresh, 300, what)
+        fresh.set_rope(theta, rot, positions)
+        got, want = result(a), result(fresh)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert all(not torch.equal(got[0], s) for s in seen)
+        seen.append(got[0])

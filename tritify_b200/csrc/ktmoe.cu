@@ -20,6 +20,7 @@
 #include <cstring>
 #include <list>
 #include <mutex>
+#include <new>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -3491,17 +3492,29 @@ int ktmoe_attn_set_rope(ktmoe_attn* A, double theta, int32_t rot_dim, int64_t po
     if (positions < 0 || positions > (int64_t)1 << 24 || rot_dim < 2 || rot_dim % 2 != 0 || rot_dim > A->cfg.head_dim)
         return fail(ctx, KTMOE_ERR_ARG, "rot_dim must be even, from 2 to head_dim, positions from 0 to 2^24");
     if (int r = set_device(ctx)) return r;
-    std::vector<int32_t> table((size_t)positions * rot_dim);
+    std::vector<int32_t> table;
+    try {
+        table.resize((size_t)positions * rot_dim);
+    } catch (const std::bad_alloc&) {
+        return fail(ctx, KTMOE_ERR_UNSUPPORTED, "no host memory for the rotation table");
+    }
     if (ktmoe_rope_table(theta, rot_dim, positions, table.data()) != KTMOE_OK)
         return fail(ctx, KTMOE_ERR_ARG, "theta must be positive and finite");
     if (int r = attn_idle(ctx)) return r;
-    if (A->captured && A->b_rope.p) {  // a captured forward keeps the table that it was captured with
-        A->retired.push_back(A->b_rope);
-        A->b_rope = DevBuf{};
+    // What forwards read stays until the new table is there: one that cannot be allocated changes nothing, and one that a
+    // captured forward holds is kept with it.
+    DevBuf fresh = A->captured ? DevBuf{} : A->b_rope;
+    if (fresh.bytes < table.size() * 4) {
+        fresh = DevBuf{};
+        CK(fresh.ensure(table.size() * 4));
     }
-    CK(A->b_rope.ensure(table.size() * 4));
-    CK(cudaMemcpy(A->b_rope.p, table.data(), table.size() * 4, cudaMemcpyHostToDevice));
+    CK(cudaMemcpy(fresh.p, table.data(), table.size() * 4, cudaMemcpyHostToDevice));
     if (int r = attn_idle(ctx)) return r;
+    if (fresh.p != A->b_rope.p) {
+        if (A->captured) A->retired.push_back(A->b_rope);
+        else A->b_rope.release();
+        A->b_rope = fresh;
+    }
     A->rope = ktmoe_rope{A->b_rope.as<int32_t>(), positions, rot_dim, interleaved ? 1 : 0};
     return KTMOE_OK;
 }
