@@ -6,6 +6,7 @@ heads, through the tile kernel."""
 import numpy as np
 import pytest
 
+import kv_reference as R
 import tritify_b200 as tb
 from test_gpu_kv import Setup, _torch
 
@@ -142,3 +143,24 @@ def test_the_widest_windows(ctx, window, sinks):
     s.check(q, scale, window=window, sinks=sinks)
     wide, narrow = s.attend(q, scale, window=window, sinks=sinks), s.attend(q, scale)
     assert (wide[0] == narrow[0]).all() and (wide[1] == narrow[1]).all()
+
+
+def test_pools_are_cleared_before_anything_is_written(ctx):
+    """A cache made while torch's stream is busy and written at once on the context's stream: the clearing of its pools
+    does not come after the writing."""
+    torch = _torch()
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    batch = tb.KvBatch(i32(0, 9), i32(9), i32(0).reshape(1, 1), 9)
+    kv = torch.full((9, 64), 2 ** 20, dtype=torch.int32, device="cuda")
+    scale = torch.tensor([1, 20], dtype=torch.int64, device="cuda")
+    tb.KvCache(ctx, 1, 16, 2, 32).append(batch, kv, kv, scale, stream=0)  # loads the kernel, which waits for the device
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)  # about a tenth of a second
+    cache = tb.KvCache(ctx, 1, 16, 2, 32)
+    cache.append(batch, kv, kv, scale, stream=0)  # the context's stream
+    ctx.sync()
+    torch.cuda.synchronize()
+    codes, sigma = R.quantise_row(np.full(32, 2 ** 20), 2.0 ** -20)
+    assert codes[0] == 126  # 1 / 127 is 1.0079 2^-7, sigma 1.015625 2^-7, and 128 / 1.015625 is 126.03
+    assert (cache.k[0, :, :9] == 126).all() and (cache.v[0, :, :9] == 126).all()
+    assert (cache.k_scale[0, :, :9] == sigma).all() and (cache.v_scale[0, :, 9:] == 0).all()

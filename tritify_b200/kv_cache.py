@@ -125,6 +125,9 @@ class KvCache:
             dev = torch.device("cuda", ctx.device)
             pools = [torch.zeros(*shape, head_dim, dtype=torch.int8, device=dev) for _ in range(2)]
             pools += [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+            # cleared before anything can write them: the context's stream does not wait for torch's
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(dev).synchronize()
         self.k, self.v, self.k_scale, self.v_scale = pools
         for t, name in ((self.k, "k pool"), (self.v, "v pool")):
             _tensor(t, name, "int8", 4)
