@@ -146,3 +146,21 @@ def test_the_classes_refuse_what_does_not_fit():
         ok.append(b, kv, kv, s)
     with pytest.raises(ValueError, match="device"):
         ok.attention(b, q, s, o, os_, 4)
+
+
+def test_a_half_refuses_other_devices():
+    """Host tensors, or another device's, in a half's batch or cache: refused before anything is launched."""
+    half = object.__new__(tb.AttentionHalf)
+    half.ctx, half._h = _Ctx(), None
+    batch, cache = tb.KvBatch(_cpu(3), _cpu(2), _cpu(2, 4), 7), _cache()
+    cache.ctx = half.ctx
+    with pytest.raises(ValueError, match="device"):
+        half.forward_dev(cache, batch, 16, 16, 16, 16)
+    batch.device_index = 0
+    with pytest.raises(ValueError, match="device"):
+        half.forward_dev(cache, batch, 16, 16, 16, 16)
+    batch.device_index, cache.device_index = 1, 0
+    with pytest.raises(ValueError, match="device"):
+        half.forward_dev(cache, batch, 16, 16, 16, 16)
+    with pytest.raises(ValueError, match="context"):
+        half.forward_dev(_cache(), batch, 16, 16, 16, 16)

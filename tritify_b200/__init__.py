@@ -857,6 +857,8 @@ class AttentionHalf:
         """Device buffers [batch.rows][d_model] (raw pointers), stream-ordered, not synchronised."""
         if cache.ctx is not self.ctx:
             raise ValueError("the cache lies on another context")
+        if batch.device_index != self.ctx.device or cache.device_index != self.ctx.device:
+            raise ValueError(f"the batch's tensors and the cache's pools lie on the context's device (cuda:{self.ctx.device})")
         self.ctx.check(lib().ktmoe_attn_forward_dev(self._h, cache._c, batch._c, ctypes.c_void_p(x_ptr),
                                                     ctypes.c_void_p(x_scale_ptr), ctypes.c_void_p(y_ptr),
                                                     ctypes.c_void_p(y_scale_ptr),
