@@ -274,7 +274,8 @@ typedef struct ktmoe_kv_cache {
  * it, attention gives zeros. What only the device can see wrong (a page outside the pool, offsets that do not ascend
  * or leave the rows, a length beyond the page table, a position beyond the rotation table) touches nothing outside
  * the buffers and makes the next ktmoe_sync on the context return KTMOE_ERR_ARG; results of that batch are undefined,
- * other work on the context is not disturbed. At most 2^30 rows and 2^24 tokens a sequence (max_pages * page_tokens). */
+ * other work on the context is not disturbed. At most 2^30 sequences, 2^30 rows and 2^24 tokens a sequence (max_pages *
+ * page_tokens). */
 typedef struct ktmoe_kv_batch {
     int32_t n_seqs;
     int32_t max_pages;

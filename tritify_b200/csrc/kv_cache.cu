@@ -32,9 +32,9 @@ int check_cache(ktmoe_ctx* ctx, const ktmoe_kv_cache* c, const ktmoe_kv_batch* b
     if ((1 << shift) != c->page_tokens) return fail(ctx, KTMOE_ERR_UNSUPPORTED, "page_tokens must be 16, 32, 64 or 128");
     if (c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->n_pages < 1 || c->n_pages > INT32_MAX)
         return fail(ctx, KTMOE_ERR_ARG, "the cache needs 1 to 1024 KV heads and 1 to 2^31 - 1 pages");
-    if (b->n_seqs < 0 || b->rows < 0 || b->rows > (int64_t)1 << 30 || b->max_pages < 0 ||
+    if (b->n_seqs < 0 || b->n_seqs > 1 << 30 || b->rows < 0 || b->rows > (int64_t)1 << 30 || b->max_pages < 0 ||
         (int64_t)b->max_pages * c->page_tokens > (int64_t)1 << 24)
-        return fail(ctx, KTMOE_ERR_ARG, "a batch holds at most 2^30 rows and a page table at most 2^24 tokens a sequence, none of them negative");
+        return fail(ctx, KTMOE_ERR_ARG, "a batch holds at most 2^30 sequences, 2^30 rows and a page table at most 2^24 tokens a sequence, none of them negative");
     if (b->n_seqs > 0 && (!b->q_begin || !b->kv_len || (b->max_pages > 0 && !b->page_table)))
         return fail(ctx, KTMOE_ERR_ARG, "the batch's offsets, lengths or page table are null");
     *kc = kv::Cache{c->k, c->v, c->k_scale, c->v_scale, c->n_pages, shift, c->n_kv_heads, c->head_dim};
