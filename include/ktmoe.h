@@ -313,7 +313,8 @@ int ktmoe_kv_read_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_k
                       float* v, int64_t ld_v, void* stream);
 /* Attention of the batch's new tokens over the cache (which holds them already: append first). q [rows][n_heads]
  * [head_dim] int32 codes, query head h reading KV head h / (n_heads / n_kv_heads); o [rows][n_heads][head_dim] int32
- * codes, o_scale [rows][n_kv_heads] the scale of each KV head's group of outputs. A row at position p sees the
+ * codes, o_scale [rows][n_kv_heads] the scale of each KV head's group of outputs; o may be q, at the same row stride, and
+ * overlaps nothing else that the call reads. A row at position p sees the
  * positions j <= p, and with window > 0 only those with j > p - window or j < sinks. Per row and head, with y and s as
  * for the cache: codes rne(RN64(y RN64(127 / max|y|))), theta = RN24(min(2^60, RN64(RN64(RN64(max|y| s) / 127)
  * RN64(softmax_scale log2 e)))); x_j = RN24((q . k_j) sigma_j), d_j = RN24(max x - x_j), z_j = min(32 * 2^10,

@@ -297,6 +297,8 @@ int kv_attention(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_bat
     if (batch->n_seqs == 0 || batch->rows == 0) return KTMOE_OK;
     if (!q || !o || !o_scale || !scale || !aligned(q, 4) || !aligned(o, 4) || !aligned(o_scale, 16))
         return fail(ctx, KTMOE_ERR_ARG, "queries, scales or outputs are null or not aligned");
+    if (o == q && ld_o != ld_q && batch->rows > 1)
+        return fail(ctx, KTMOE_ERR_ARG, "o may be q at the same row stride only");
     if (int r = set_device(ctx)) return r;
     a.err = error_of(ctx);
     a.q = q;
