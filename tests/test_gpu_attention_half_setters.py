@@ -1,4 +1,4 @@
-"""Setting an attention half's weights: what is refused, and that a forward in flight keeps what it began with."""
+"""Setting an attention half's weights on a B200: what is refused, and that a forward in flight keeps what it began with."""
 
 import numpy as np
 import pytest
@@ -113,3 +113,21 @@ def test_rotation_tables_that_grow_shrink_and_fail(ctx):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         assert all(not torch.equal(got[0], s) for s in seen)
         seen.append(got[0])
+
+
+@pytest.mark.parametrize("rows", [1, 9])
+def test_a_half_over_its_own_input(ctx, rows):
+    """y is x, with its scale: what separate buffers give."""
+    import torch
+
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    batch = tb.KvBatch(i32(0, rows), i32(rows), i32(0).reshape(1, 1), rows)
+    x = torch.from_numpy(tb.IntTensor.from_reals(tb.synth_normal(9, 1.0, rows * 64)).data.reshape(rows, 64).copy()).cuda()
+    xs = torch.tensor([1, 28], dtype=torch.int64, device="cuda")
+    cache, a = tb.KvCache(ctx, 1, 16, 1, 32), _half(ctx, 400)
+    y, ys = torch.zeros_like(x), torch.zeros_like(xs)
+    torch.cuda.synchronize()
+    a.forward_dev(cache, batch, x.data_ptr(), xs.data_ptr(), y.data_ptr(), ys.data_ptr())
+    a.forward_dev(cache, batch, x.data_ptr(), xs.data_ptr(), x.data_ptr(), xs.data_ptr())
+    ctx.sync()
+    assert torch.equal(x, y) and torch.equal(xs, ys)

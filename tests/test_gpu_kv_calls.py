@@ -69,3 +69,58 @@ def test_outputs_over_the_queries_at_another_stride(ctx):
             s.cache.attention(s.batch, a, scale, b, os_, 2)
         assert e.value.status == _native.ERR_ARG
     ctx.sync()
+
+
+@pytest.mark.parametrize("dim", [144, 160, 208, 240])
+def test_heads_between_128_and_256(ctx, dim):
+    """Rows of one whole 128-byte block and a part, rotated, windowed, written, read and attended."""
+    torch = _torch()
+    s = Setup(ctx, [(70, 70), (1, 300), (35, 200)], 4, 2, dim, 32, seed=dim, rows_behind=1)
+    table = tb.rope_table(1e4, dim - 16, 301)
+    rope = tb.Rope(torch.from_numpy(table).cuda(), dim == 160)
+    k, v, scale = s.codes(2 * dim), s.codes(2 * dim), s.scales()
+    R.append(k.reshape(s.rows, 2, dim), v.reshape(s.rows, 2, dim), scale, s.begin, s.kv_len, s.write, table, dim == 160)
+    s.cache.append(s.batch, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), torch.from_numpy(scale).cuda(), rope)
+    ko, vo = torch.zeros(s.rows, 2 * dim, device="cuda"), torch.zeros(s.rows, 2 * dim, device="cuda")
+    s.cache.read(s.batch, ko, vo)
+    ctx.sync()
+    torch.cuda.synchronize()
+    for n, t in (("k", s.cache.k), ("v", s.cache.v), ("ks", s.cache.k_scale), ("vs", s.cache.v_scale)):
+        assert (t.double().cpu().numpy() == s.pool[n].astype(np.float64)).all(), n
+    page, place = s.place(0, 69)
+    for n, o in (("k", ko), ("v", vo)):
+        assert (o[69].reshape(2, dim).cpu().numpy() == s.pool[n][page, :, place] * s.pool[n + "s"][page, :, place][:, None]).all()
+    s.check(s.codes(4 * dim), scale, table, dim == 160)
+    s.check(s.codes(4 * dim), scale, table, dim == 160, window=50, sinks=3)
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 2)])
+@pytest.mark.parametrize("heads,hk", [(4, 2), (8, 1)])
+def test_a_chunk_among_decoding_sequences(ctx, heads, hk, window, sinks):
+    """One long chunk in a batch of single tokens, sequences that add nothing between them, and a page table far wider
+    than any sequence."""
+    lens = [(1, 1 + 37 * i % 200) for i in range(9)] + [(280, 333), (0, 50)] + [(1, 300 - 13 * i) for i in range(14)]
+    s = Setup(ctx, lens, heads, hk, 64, 16, seed=heads, rows_before=2, rows_behind=3)
+    wide = _torch().full((len(lens), 3000), 2 ** 31 - 1, dtype=_torch().int32, device="cuda")  # no page of the pool
+    wide[:, :s.max_pages] = s.batch.page_table
+    s.batch = tb.KvBatch(s.batch.q_begin, s.batch.kv_len, wide, s.rows)
+    q, scale = s.codes(heads * 64), s.scales()
+    torch = _torch()
+    for copies, launches in ((1, None), (-(-148 // hk), 2)):
+        cache = tb.KvCache(ctx, s.cache.n_pages, 16, copies * hk, 64, pools=[
+            t.repeat(1, copies, *[1] * (t.dim() - 2)) for t in (s.cache.k, s.cache.v, s.cache.k_scale, s.cache.v_scale)])
+        o = torch.full((s.rows, copies * heads * 64), 77, dtype=torch.int32, device="cuda")
+        os_ = torch.full((s.rows, copies * hk, 2), 77, dtype=torch.int64, device="cuda")
+        before = ctx.launch_count()
+        cache.attention(s.batch, torch.from_numpy(q).cuda().repeat(1, copies), torch.from_numpy(scale).cuda(), o, os_,
+                        copies * heads, window=window, sinks=sinks)
+        assert launches is None or heads < 8 or ctx.launch_count() - before == launches  # the tile kernel
+        ctx.sync()
+        torch.cuda.synchronize()
+        want = np.full((s.rows, heads, 64), 77, np.int64)
+        want_s = np.full((s.rows, hk, 2), 77, np.int64)
+        R.attention(q.reshape(s.rows, heads, 64), scale, s.begin, s.kv_len, s.keys, want, want_s, 64 ** -0.5, window, sinks)
+        want_s[..., 1] &= 0xFFFFFFFF
+        for got, w in ((o, want.reshape(s.rows, -1)), (os_, want_s)):
+            got = got.reshape(s.rows, copies, -1).cpu().numpy()
+            assert (got == w.reshape(s.rows, 1, -1)).all()
