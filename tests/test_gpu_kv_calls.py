@@ -124,3 +124,52 @@ def test_a_chunk_among_decoding_sequences(ctx, heads, hk, window, sinks):
         for got, w in ((o, want.reshape(s.rows, -1)), (os_, want_s)):
             got = got.reshape(s.rows, copies, -1).cpu().numpy()
             assert (got == w.reshape(s.rows, 1, -1)).all()
+
+
+def test_a_busy_stream_is_waited_for_where_it_is_given(ctx):
+    """A wrong batch on a stream that is busy: the sync that is given the stream raises it."""
+    torch = _torch()
+    s = Setup(ctx, [(1, 100)], 4, 2, 64, 16)
+    q, scale = torch.from_numpy(s.codes(256)).cuda(), torch.from_numpy(s.scales()).cuda()
+    out, os_ = torch.zeros_like(q), torch.zeros(1, 2, 2, dtype=torch.int64, device="cuda")
+    s.cache.attention(s.batch, q, scale, out, os_, 4)
+    ctx.sync()
+    s.batch.page_table[0, 2] = s.cache.n_pages
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # about a tenth of a second
+        s.cache.attention(s.batch, q, scale, out, os_, 4)
+    with pytest.raises(tb.KtmoeError) as e:
+        ctx.sync(side.cuda_stream)
+    assert e.value.status == _native.ERR_ARG
+    ctx.sync()
+
+
+def test_the_cache_in_order_with_a_half(ctx):
+    """A half's forward on the context's stream and, unsynchronised behind it, the rows that it wrote read back on that
+    stream (stream=0): what they are once everything has come to rest."""
+    torch = _torch()
+    d, n = 2048, 64
+    lin = lambda seed, out, k: tb.QuantLinear.from_weights("w", tb.synth_normal(seed, 0.05, out * k), out, k)
+    half = tb.AttentionHalf(ctx, d, 4, 2, 64)
+    half.set_qkv(lin(1, 256, d), lin(2, 128, d), lin(3, 128, d))
+    half.set_out(lin(4, d, 256))
+    norm = tb.QuantLinear.from_weights("n", tb.synth_normal(5, 1.0, d), 1, d)
+    half.set_norm(norm.w_codes, norm.w_scale, tb.scale_from_f64(1e-6))
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    batch = tb.KvBatch(i32(0, n), i32(n), i32(2, 0, 1, 3).reshape(1, 4), n)
+    cache = tb.KvCache(ctx, 4, 16, 2, 64)
+    x = torch.from_numpy(tb.IntTensor.from_reals(tb.synth_normal(6, 1.0, n * d)).data.copy()).cuda()
+    xs = torch.tensor([1, 28], dtype=torch.int64, device="cuda")
+    y, ys = torch.zeros_like(x), torch.zeros_like(xs)
+    got = [torch.zeros(n, 128, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    half.forward_dev(cache, batch, x.data_ptr(), xs.data_ptr(), y.data_ptr(), ys.data_ptr())
+    cache.read(batch, got[0], got[1], stream=0)
+    ctx.sync()
+    torch.cuda.synchronize()
+    cache.read(batch, got[2], got[3])
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], got[2]) and torch.equal(got[1], got[3])
+    assert int((got[0] != 0).sum()) > n * 64

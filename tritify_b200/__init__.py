@@ -854,7 +854,8 @@ class AttentionHalf:
 
     def forward_dev(self, cache: KvCache, batch: KvBatch, x_ptr: int, x_scale_ptr: int, y_ptr: int, y_scale_ptr: int,
                     stream: int = 0) -> None:
-        """Device buffers [batch.rows][d_model] (raw pointers), stream-ordered, not synchronised."""
+        """Device buffers [batch.rows][d_model] (raw pointers), not synchronised, ordered on ``stream`` (0: the context's own,
+        which torch's streams do not wait for nor it for them)."""
         if cache.ctx is not self.ctx:
             raise ValueError("the cache lies on another context")
         if batch.device_index != self.ctx.device or cache.device_index != self.ctx.device:
@@ -917,7 +918,9 @@ class MoeStack:
     def forward_dev(self, x_ptr: int, rows: int, x_scale_ptr: int, y_ptr: int, y_scale_ptr: int,
                     batch: Optional[KvBatch] = None) -> None:
         """Device buffers (raw pointers; a Scale is 16 bytes {i64 mant, i32 shift}); ordered on the context's stream,
-        not synchronised. ``batch``: where the rows stand in their sequences (a stack with attention)."""
+        not synchronised. ``batch``: where the rows stand in their sequences (a stack with attention). Torch's streams do
+        not wait for the context's nor it for them: calls on the caches around this one take ``stream=0``, and what torch
+        writes for it (the batch's tensors too) is synchronised first."""
         self._check_batch(rows, batch)
         _, xb, sb = self._buffers(rows)
         src, src_s = x_ptr, x_scale_ptr
