@@ -131,3 +131,26 @@ def test_a_half_over_its_own_input(ctx, rows):
     a.forward_dev(cache, batch, x.data_ptr(), xs.data_ptr(), x.data_ptr(), xs.data_ptr())
     ctx.sync()
     assert torch.equal(x, y) and torch.equal(xs, ys)
+
+
+@pytest.mark.parametrize("rows", [2 ** 30 + 1, 2 ** 40, 2 ** 62, 2 ** 63 - 1, -1])
+def test_more_rows_than_a_batch_holds(ctx, rows):
+    """Refused before the scratch is sized for them, where 2^62 rows by four heads would count as none; the half serves on."""
+    import torch
+
+    a = tb.AttentionHalf(ctx, 64, 4, 4, 16)
+    a.set_qkv(*(_linear(i, 64, 64) for i in range(3)))
+    a.set_out(_linear(4, 64, 64))
+    a.set_norm(np.ones(64, np.int32), tb.Scale(1, 0), tb.Scale(0, 0))
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    batch = tb.KvBatch(i32(0, 2), i32(2), i32(0).reshape(1, 1), 2)
+    cache = tb.KvCache(ctx, 1, 16, 4, 16)
+    x = torch.ones(2, 64, dtype=torch.int32, device="cuda")
+    xs = torch.tensor([1, 0], dtype=torch.int64, device="cuda")
+    wrong = _native.KtmoeKvBatch.from_buffer_copy(batch._c)
+    wrong.rows = rows
+    torch.cuda.synchronize()
+    status = tb.lib().ktmoe_attn_forward_dev(a._h, cache._c, wrong, x.data_ptr(), xs.data_ptr(), x.data_ptr(), xs.data_ptr(), None)
+    assert status == _native.ERR_ARG
+    a.forward_dev(cache, batch, x.data_ptr(), xs.data_ptr(), x.data_ptr(), xs.data_ptr())
+    ctx.sync()

@@ -3539,7 +3539,8 @@ int ktmoe_attn_forward_dev(ktmoe_attn* A, const ktmoe_kv_cache* cache, const ktm
         return fail(ctx, KTMOE_ERR_STATE, "a weight of the attention half is not set");
     if (cache->n_kv_heads != A->cfg.n_kv_heads || cache->head_dim != A->cfg.head_dim)
         return fail(ctx, KTMOE_ERR_ARG, "the cache's heads are not the attention's");
-    if (batch->rows < 0 || batch->rows * A->cfg.n_kv_heads > INT32_MAX || batch->rows * A->d > (int64_t)1 << 40)
+    if (batch->rows < 0 || batch->rows > (int64_t)1 << 30 || batch->rows * A->cfg.n_kv_heads > INT32_MAX ||
+        batch->rows * A->d > (int64_t)1 << 40)
         return fail(ctx, KTMOE_ERR_ARG, "too many rows");
     if (batch->rows == 0) return KTMOE_OK;
     if (!x_dev || !x_scale_dev || !y_dev || !y_scale_dev) return KTMOE_ERR_ARG;
