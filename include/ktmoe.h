@@ -299,7 +299,7 @@ int ktmoe_rope_table(double theta, int32_t rot_dim, int64_t positions, int32_t* 
 
 /* Write the batch's new keys and values: k, v [rows][n_kv_heads][head_dim] int32 codes with row strides ld_k and ld_v
  * (in elements) at k_scale[row * scale_stride] and v_scale[row * scale_stride] (NULL v_scale: as the keys; scale_stride
- * 1: a scale per row; 0: one for all), keys rotated when rope is not NULL. With y a row's codes after the rotation and s its scale (2^-30 of it after a rotation):
+ * 1: a scale per row; 0: one for all), keys rotated when rope is not NULL. With y RN64 of a row's codes after the rotation and s its scale (2^-30 of it after a rotation):
  * t = RN64(RN64(max|y| s) / 127) held within [2^-64, 2^63], sigma = t rounded up to 8 significant bits, codes
  * rne(RN64(y RN64(s / sigma))) held within +-127. A scale's shift counts as at least -900 and at most 2000, here and in
  * ktmoe_attention_dev. Stream-ordered (NULL: the context stream), not synchronised. Two
@@ -321,7 +321,9 @@ int ktmoe_kv_read_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_k
  * rne(2^10 d_j theta)), n_j = rne(z_j / 2^10), r_j = n_j - z_j / 2^10, w_j = 2^-n_j e(r_j), where e, about 32512 * 2^r,
  * is RN24(RN24(RN24(c3 r + c2) r + c1) r + 32512) with c1, c2, c3 = 127/256 times 45435, 15874, 3605; L = sum rne(w_j);
  * 2^E the least power of two no smaller than any visible sigma of V; O = sum rne(w_j sigma_j 2^-E) v_j;
- * o = rne(RN64(O RN64(2^21 / L))) (within +-2^28) at the scale {1, 21 - E}. A row that sees nothing is zeros at {0, 0}. */
+ * o = rne(RN64(O RN64(2^21 / L))) (within +-2^28) at the scale {1, 21 - E}. A row that sees nothing is zeros at {0, 0}.
+ * A weight counts in units of 1/32512 of the row's largest: n keys put L off by n / 2 at most, and keys 16 octaves below
+ * the largest weigh nothing, however many (n of them would hold up to n 2^-16 of the largest's weight). */
 int ktmoe_attention_dev(ktmoe_ctx* ctx, const ktmoe_kv_cache* cache, const ktmoe_kv_batch* batch, const int32_t* q,
                         int64_t ld_q, const ktmoe_scale* scale, int32_t scale_stride, const ktmoe_rope* rope,
                         int32_t n_heads, double softmax_scale, int32_t window, int32_t sinks, int32_t* o, int64_t ld_o,

@@ -164,3 +164,22 @@ def test_a_half_refuses_other_devices():
         half.forward_dev(cache, batch, 16, 16, 16, 16)
     with pytest.raises(ValueError, match="context"):
         half.forward_dev(_cache(), batch, 16, 16, 16, 16)
+
+
+def test_what_long_rows_lose():
+    """A weight is rounded to a unit of 1/32512 of the row's largest: over n keys the total is off by n / 2 units at most
+    (and 4.4e-4 of itself, above). With scores a few octaves apart that is little at any length; but keys 16 octaves below
+    the largest (32512 2^-16 < 1/2) weigh nothing however many they are, up to n 2^-16 of the largest's weight."""
+    n = 65536
+    rng = np.random.default_rng(2)
+    for spread in (0.0, 1.0, 3.0):
+        x = R.rn24(spread * rng.standard_normal(n))
+        w = np.rint(R.weights(x, np.ones(n), 1.0)).sum()
+        exact = 32512 * np.exp2(x - x.max()).sum()
+        assert abs(w - exact) <= 4.4e-4 * exact + n / 2
+    assert n / 2 < 1e-2 * 32512 * np.exp2(R.rn24(rng.standard_normal(n)) - 4.5).sum()  # one octave's spread: below 1 %
+    x = np.full(n, -16.05)
+    x[7] = 0.0
+    w = np.rint(R.weights(R.rn24(x), np.ones(n), 1.0))
+    assert w[7] == 32512 and w.sum() == 32512
+    assert 0.9 < np.exp2(x).sum() - 1 <= n * 2.0 ** -16

@@ -141,10 +141,11 @@ int64_t even_blocks(const kv::AttendArgs& a, int64_t block) {
 
 // Blocks of a cluster: twice as many while they are less than 4/3 of what the GPU holds at once. Eights are harder to
 // place (a GPC's SMs do not divide by them; with one block an SM, 16 clusters of eight already take two rounds): only
-// where they fill half of the GPU at most, or where the keys are long. Measured (us), clusters of 1, 2, 4, 8 at 4 query
-// heads to one of 8 KV heads of 128: 1 sequence of 1000 keys 21, 18, 16, 16, of 8000 86, 49, 29, 23; 4 of 2000 30, 23,
-// 20, 23; 8 of 16384 176, 105, 82, 86; 16 of 4096 59, 49, 55, 94; 64 of 1024 53, 74, 121, 121, of 4096 145, 145, 180, 285.
-// Over 444 such sizes the rule loses 2 % to the best choice of each.
+// where they fill half of the GPU at most, or where the keys are long. Measured (us, from a flushed L2), clusters of 1, 2,
+// 4, 8 at 4 query heads to one of 8 KV heads of 128: 1 sequence of 1000 keys 18, 16, 14, 12, of 8000 76, 43, 29, 20; 4 of
+// 2000 29, 20, 18, 20; 8 of 16384 164, 84, 61, 74; 16 of 4096 45, 39, 51, 72; 64 of 1024 47, 68, 108, 209, of 4096 113, 129,
+// 168, 262. Over 160 sizes drawn at random (1 to 128 sequences of one token, 100 to 65536 keys, heads of 64 to 256) the
+// choice of cluster and kernel takes 7 % more than the best of each, in 41 of them more than 10 %.
 int few_cluster(const ktmoe_ctx* ctx, const kv::AttendArgs& a, int per_sm) {
     const int64_t jobs = even_blocks(a, kv::FEW_ROWS), tiles = key_tiles(a), at_once = (int64_t)per_sm * ctx->num_sms;
     int c = 1;
@@ -157,10 +158,12 @@ int few_cluster(const ktmoe_ctx* ctx, const kv::AttendArgs& a, int per_sm) {
 // Which kernel. Where the GPU is full, a block of 128 rows is the better one (three times for many rows), but it walks
 // all keys alone, while sixteens of rows spread over more SMs and split the keys in clusters. Both times are rounds of
 // blocks by tiles of keys and a start; an SM passes a tile by 16 rows in 3/7 of the time it takes by 128, and starts
-// count as 8 and 6 tiles. Measured (us) at a head_dim of 128, 8 KV heads and 8192 keys: 1 sequence of 64 rows 39 against
-// 159, of 256 90 against 162, of 512 150 against 163, of 1024 264 against 163; 16 sequences of 32 rows 152 against 167, of
-// 64 277 against 169; at 512 keys 1 sequence of 256 rows 43 against 32. Over 304 such sizes, head_dim 256 among them, the
-// rule loses less than 0.1 % to the better choice of each.
+// count as 8 and 6 tiles. Measured (us, from a flushed L2) at 8 KV heads of 128, one query head each, and 8192 keys: 1
+// sequence of 64 rows 39 against 156, of 256 80 against 156, of 512 137 against 156, of 1024 258 against 160; 16 sequences
+// of 32 rows 154 against 166, of 64 279 against 168; at 512 keys 1 sequence of 256 rows 25 against 29. Over 160 sizes drawn at
+// random (2 to 1024 tokens a sequence) the choice of kernel and cluster takes 3 % more than the best of each, in 12 of them
+// more than 10 %. The host knows neither lengths nor rows: a page table wider than the sequences, or one chunk among
+// single tokens, counts as if every sequence were as long and had as many rows, which changes the time alone.
 bool few_rows(const ktmoe_ctx* ctx, const kv::AttendArgs& a, int per_sm) {
     auto rounds = [](int64_t blocks, int64_t at_once) { return (blocks + at_once - 1) / at_once; };
     const int64_t c = few_cluster(ctx, a, per_sm), tiles = key_tiles(a);
