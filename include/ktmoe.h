@@ -273,9 +273,9 @@ typedef struct ktmoe_kv_cache {
  * are. A row at a negative position (a length below the new tokens) has no place in the cache: append and read skip
  * it, attention gives zeros. What only the device can see wrong (a page outside the pool, offsets that do not ascend
  * or leave the rows, a length beyond the page table, a position beyond the rotation table) touches nothing outside
- * the buffers and makes the next ktmoe_sync that waits for the call's stream return KTMOE_ERR_ARG; results of that batch are undefined,
- * other work on the context is not disturbed. At most 2^30 sequences, 2^30 rows and 2^24 tokens a sequence (max_pages *
- * page_tokens). */
+ * the buffers and makes the next ktmoe_sync that waits for the call's stream return KTMOE_ERR_ARG; results of that batch
+ * are undefined, other work on the context is not disturbed. At most 2^30 sequences, 2^30 rows and 2^24 tokens a
+ * sequence (max_pages * page_tokens). */
 typedef struct ktmoe_kv_batch {
     int32_t n_seqs;
     int32_t max_pages;

@@ -2,11 +2,12 @@
 ``ktmoe_attention_dev`` of ``include/ktmoe.h``, which states the arithmetic).
 
 Device buffers are torch tensors (memory only; every value comes from libktmoe.so's kernels). Calls are ordered on
-torch's current stream unless ``stream`` gives another (a raw CUDA stream handle; 0: the context's own stream), and are not
-synchronised. AttentionHalf and MoeStack run on the context's stream by default, which does not wait for torch's nor torch's
-for it: give ``stream=0`` to the calls on a cache that go with them, or synchronise in between. What only the device can
-find wrong in a batch (a page outside the pool, lengths that do not fit) is raised by the next ``Context.sync`` that waits
-for the call: ``sync(stream)`` for one on another stream. A scale is two int64 words, {mant, shift}: one pair, or one pair a row.
+torch's current stream unless ``stream`` gives another (a raw CUDA stream handle; 0: the context's own stream), and are
+not synchronised. AttentionHalf and MoeStack run on the context's stream by default, which does not wait for torch's nor
+torch's for it: give ``stream=0`` to the calls on a cache that go with them, or synchronise in between. What only the
+device can find wrong in a batch (a page outside the pool, lengths that do not fit) is raised by the next
+``Context.sync`` that waits for the call: ``sync(stream)`` for one on another stream. A scale is two int64 words, {mant,
+shift}: one pair, or one pair a row.
 """
 
 from __future__ import annotations
